@@ -10,7 +10,7 @@ import subprocess
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.path.join(_HERE, "libgraspbal_hip.so")
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 GB_OK = 0
 _ERRNAMES = {-1: "GB_EINVAL", -2: "GB_ELAUNCH", -3: "GB_ERANGE"}
@@ -116,6 +116,10 @@ SIGNATURES = {
     "gb_affine_relu_maxpool_members": [_P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _P],
     "gb_bn_bwd_apply_members": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _L, _I, _P, _P],
     "gb_bn_bwd_apply_w": [_P, _P, _P, _P, _P, _L, _L, _I, _I, _P, _P, _P],
+    "gb_dropout": [_P, _P, _P, _L, _I, _I, _P, _L, _L, _P, _P],
+    "gb_group_norm_workspace": [_P, _I, _P],
+    "gb_group_norm_fwd": [_P, _P, _P, _L, _P],
+    "gb_group_norm_bwd": [_P, _P, _P, _P, _P, _P, _P, _L, _P],
 }
 
 
@@ -173,7 +177,16 @@ class WgradItem(_c.Structure):
                 ("P", _c.c_longlong), ("K", _c.c_int), ("N", _c.c_int), ("ldw", _c.c_int)]
 
 
+class GroupNorm(_c.Structure):
+    """GbGroupNorm of include/graspbal.h: one gb_group_norm_* call."""
+    _fields_ = [(n, _c.c_void_p) for n in ("x", "residual", "weight", "bias", "offsets", "mean", "rstd", "rng", "used")] \
+        + [(n, _c.c_longlong) for n in ("rows", "seed", "call")] \
+        + [(n, _c.c_int) for n in ("samples", "channels", "groups", "dtype", "act", "q")] \
+        + [("eps", _c.c_float), ("slope", _c.c_float)]
+
+
 PREC_F32, PREC_BF16, PREC_F32_SPLIT3 = 0, 1, 2
+ACTIVATIONS = {"none": 0, "relu": 1, "leaky_relu": 2, "silu": 3, "gelu": 4}   # GB_ACT_*
 GEMM_NO_RING = 1   # GbGemmOpts.flags
 GEMM_NO_PAIR = 2
 GEMM_NO_DIRECT = 4

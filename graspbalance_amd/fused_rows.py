@@ -1,0 +1,232 @@
+"""Channel-last row operators beside the BatchNorm stacks of fused_mlp (no reference counterpart): group norm with an
+activation, dropout from a counter-based generator.
+
+Rows are (..., C) tensors in fp32, bf16 or fp16 with the channels last, as everywhere on the fused path.  Kernels run on the
+current stream of the tensors' device; workspaces come from torch's allocator inside the call, so that every captured graph
+has its own.  CPU tensors raise, like every operator of this package.  Gradients are exact to rounding and repeat bit for
+bit (no atomics); differentiating them again is refused.
+"""
+import ctypes
+
+import torch
+import torch.nn as nn
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .fused_mlp import _call, _s
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # GB_T_*
+
+
+def _refuse(what, why):
+    raise RuntimeError("%s: %s" % (what, why))
+
+
+def _rows_tensor(what, name, t):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _refuse(what, "CPU not supported (%s)" % name)
+    if t.dtype not in _TYPES:
+        _refuse(what, "%s must be float32, bfloat16 or float16, not %s" % (name, t.dtype))
+
+
+def _like(what, name, t, x):
+    """A tensor that goes with x element by element."""
+    if not isinstance(t, torch.Tensor) or t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
+        _refuse(what, "%s must have the input's shape, type and device" % name)
+
+
+def _channel_vector(what, name, t, n, x):
+    """A per-channel parameter as contiguous fp32 (None stays None); its gradient comes back in its own type."""
+    if t is None:
+        return None
+    if t.shape != (n,) or t.device != x.device or not t.is_floating_point():
+        _refuse(what, "%s must be a float tensor of %d elements on the input's device" % (name, n))
+    return t.float().contiguous()
+
+
+def _rate(what, p, rng, x):
+    """(q, rng) of a dropout rate: q / 65536 is the rate, rng an int64 pair on the device or a pair of ints."""
+    if not 0.0 <= p <= 1.0:
+        _refuse(what, "a dropout rate of %r is not in [0, 1]" % (p,))
+    q = int(p * 65536 + 0.5)
+    if q == 0:
+        return 0, (0, 0)
+    if isinstance(rng, torch.Tensor):
+        if rng.shape != (2,) or rng.dtype != torch.int64 or rng.device != x.device or not rng.is_contiguous():
+            _refuse(what, "rng must be an int64 tensor [seed, call] on the input's device, or a pair of ints")
+        return q, rng
+    try:
+        seed, call = (int(v) for v in rng)
+    except (TypeError, ValueError):
+        _refuse(what, "rng must be an int64 tensor [seed, call] on the input's device, or a pair of ints")
+    wrap = lambda v: (v + (1 << 63)) % (1 << 64) - (1 << 63)   # noqa: E731  (64 bits as C's signed type holds them)
+    return q, (wrap(seed), wrap(call))
+
+
+def _rng_args(rng):
+    """(device pointer | None, seed, call) of a launch."""
+    return (_lib.ptr(rng), 0, 0) if isinstance(rng, torch.Tensor) else (None, rng[0], rng[1])
+
+
+class _Dropout(Function):
+    @staticmethod
+    def forward(ctx, x, residual, q, rng):
+        y = torch.empty_like(x)
+        at, seed, call = _rng_args(rng)
+        # the numbers' key is kept as it was used: the owner may write the next call's into rng before the backward pass
+        used = torch.empty_like(rng) if at is not None else None
+        _call("gb_dropout", x.device, _lib.ptr(x), _lib.ptr(residual), _lib.ptr(y), x.numel(), _TYPES[x.dtype], q, at, seed,
+              call, _lib.ptr(used), _s(x))
+        ctx.q, ctx.rng, ctx.has_residual = q, None if used is not None else rng, residual is not None
+        ctx.save_for_backward(*(() if used is None else (used,)))
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dy = dy.contiguous()
+            dx = torch.empty_like(dy)
+            at, seed, call = _rng_args(ctx.saved_tensors[0] if ctx.rng is None else ctx.rng)
+            _call("gb_dropout", dy.device, _lib.ptr(dy), None, _lib.ptr(dx), dy.numel(), _TYPES[dy.dtype], ctx.q, at, seed,
+                  call, None, _s(dy))
+        return dx, dy if ctx.has_residual and ctx.needs_input_grad[1] else None, None, None
+
+
+def dropout(x, p, rng, residual=None):
+    """x with every element dropped (zero, whatever it held) with probability p and the others divided by 1 - p, plus
+    `residual`.  p is taken to the nearest 65536th.  rng: [seed, call] - an int64 tensor on the device, which a captured
+    graph reads at every replay, or two ints.  Element i (in the order of the contiguous tensor) is kept by number i of
+    that pair alone (Philox4x32-10, include/graspbal.h gb_dropout): equal pairs drop equal places, pairs that differ in
+    either number are independent.  Nothing of the mask is stored; the backward pass computes it again."""
+    _rows_tensor("dropout", "x", x)
+    q, rng = _rate("dropout", p, rng, x)
+    if residual is not None:
+        _like("dropout", "residual", residual, x)
+    if q == 0:
+        return x if residual is None else x + residual
+    return _Dropout.apply(x.contiguous(), None if residual is None else residual.contiguous(), q, rng)
+
+
+class Dropout(nn.Module):
+    """dropout() as a layer: owns its [seed, call] pair on the device as the buffer ``rng`` (saved with the module) and moves
+    to the next call at every training forward - also at every replay of a captured one.  Without a seed, one is drawn from
+    torch's CPU generator."""
+
+    def __init__(self, p=0.5, seed=None):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            _refuse("Dropout", "a dropout rate of %r is not in [0, 1]" % (p,))
+        self.p = p
+        if seed is None:
+            seed = int(torch.randint(0, 1 << 62, (1,)))
+        self.register_buffer("rng", torch.tensor([seed, 0], dtype=torch.int64))
+        self.register_buffer("_next", torch.tensor([0, 1], dtype=torch.int64), persistent=False)
+
+    def extra_repr(self):
+        return "p=%g" % self.p
+
+    def take(self):
+        """The pair for one call; the next call gets another.  (A copy: what the caller's kernels read later is not
+        moved.)"""
+        used = self.rng.clone()
+        self.rng.add_(self._next)
+        return used
+
+    def forward(self, x, residual=None):
+        if not self.training or self.p == 0.0:
+            return x if residual is None else x + residual
+        return dropout(x, self.p, self.take(), residual)
+
+
+class _GroupNormAct(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, offsets, samples, groups, eps, act, slope, q, rng):
+        dev, C = x.device, x.shape[-1]
+        rows = x.numel() // C
+        y = torch.empty_like(x)
+        stats = torch.empty((2, samples, groups), dtype=torch.float32, device=dev)
+        at, seed, call = _rng_args(rng)
+        used = torch.empty_like(rng) if at is not None else None
+        n = _lib.GroupNorm(x=_lib.ptr(x), residual=_lib.ptr(residual), weight=_lib.ptr(weight), bias=_lib.ptr(bias),
+                           offsets=_lib.ptr(offsets), mean=stats.data_ptr(), rstd=stats[1].data_ptr(), rng=at,
+                           used=_lib.ptr(used), rows=rows, seed=seed, call=call, samples=samples, channels=C, groups=groups,
+                           dtype=_TYPES[x.dtype], act=act, q=q, eps=eps, slope=slope)
+        ws, size = _norm_workspace(n, 0, dev)
+        _call("gb_group_norm_fwd", dev, ctypes.byref(n), _lib.ptr(y), _lib.ptr(ws), size, _s(x))
+        ctx.save_for_backward(x, weight, bias, residual, offsets, stats, used)
+        ctx.cfg = (samples, groups, eps, act, slope, q, None if used is not None else rng)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, residual, offsets, stats, used = ctx.saved_tensors
+        samples, groups, eps, act, slope, q, rng = ctx.cfg
+        dev, C = x.device, x.shape[-1]
+        dy = dy.contiguous()
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dx = torch.empty_like(x)
+        # (the residual's gradient is dy itself where nothing stands between it and y)
+        plain = act == 0 and q == 0 and offsets is None
+        dres = torch.empty_like(x) if need_r and not plain else None
+        grads = torch.zeros((2, C), dtype=torch.float32, device=dev) if x.numel() == 0 else \
+            torch.empty((2, C), dtype=torch.float32, device=dev)
+        at, seed, call = _rng_args(used if rng is None else rng)
+        n = _lib.GroupNorm(x=_lib.ptr(x), residual=_lib.ptr(residual), weight=_lib.ptr(weight), bias=_lib.ptr(bias),
+                           offsets=_lib.ptr(offsets), mean=stats.data_ptr(), rstd=stats[1].data_ptr(), rng=at, used=None,
+                           rows=x.numel() // C, seed=seed, call=call, samples=samples, channels=C, groups=groups,
+                           dtype=_TYPES[x.dtype], act=act, q=q, eps=eps, slope=slope)
+        ws, size = _norm_workspace(n, 1, dev)
+        _call("gb_group_norm_bwd", dev, ctypes.byref(n), _lib.ptr(dy), _lib.ptr(dx), _lib.ptr(dres), grads.data_ptr(),
+              grads[1].data_ptr(), _lib.ptr(ws), size, _s(x))
+        return (dx if need_x else None, grads[0] if need_w else None, grads[1] if need_b else None,
+                (dy if plain else dres) if need_r else None) + (None,) * 8
+
+
+def _norm_workspace(n, backward, dev):
+    size = ctypes.c_longlong()
+    _lib.check(_lib.lib().gb_group_norm_workspace(ctypes.byref(n), backward, ctypes.byref(size)), "group_norm_act")
+    return (torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None), size.value
+
+
+def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", negative_slope=0.01, residual=None,
+                   offsets=None, dropout_p=0.0, rng=None):
+    """act(group_norm(x) * weight + bias + residual) on channel-last rows, then dropout when dropout_p > 0, in one pass.
+
+    x: (B, ..., C), every x[b] a sample of its own; or with `offsets` (S + 1 ascending row numbers, int64 on the device)
+    packed rows (R, C), sample s being rows offsets[s] up to offsets[s + 1] - none, where they are equal.  Rows outside
+    every sample give zeros and get zero gradients.  Statistics are taken over all rows of a sample and the C / num_groups
+    channels of a group, biased, as nn.GroupNorm does; a single element per group is legal and gives act(bias).
+    act: "none", "relu", "leaky_relu" (negative_slope), "silu", "gelu" (the erf form).  weight, bias: (C,) or None.
+    dropout_p, rng: as in dropout().  -> like x."""
+    what = "group_norm_act"
+    _rows_tensor(what, "x", x)
+    if x.dim() < 2:
+        _refuse(what, "x must be (samples, ..., channels)")
+    C, groups = x.shape[-1], int(num_groups)
+    if groups <= 0 or C <= 0 or C % groups:
+        _refuse(what, "%d channels do not make %d groups" % (C, groups))
+    if act not in _lib.ACTIVATIONS:
+        _refuse(what, "act must be one of %s" % ", ".join(_lib.ACTIVATIONS))
+    if not eps >= 0:
+        _refuse(what, "eps must not be negative")
+    if offsets is not None:
+        if x.dim() != 2:
+            _refuse(what, "packed rows must be (rows, channels)")
+        if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.numel() < 2 \
+                or offsets.dtype != torch.int64 or offsets.device != x.device:
+            _refuse(what, "offsets must be an int64 tensor of samples + 1 row numbers on the input's device")
+        offsets = offsets.contiguous()
+        samples = offsets.numel() - 1
+    else:
+        samples = max(1, x.shape[0])
+    if residual is not None:
+        _like(what, "residual", residual, x)
+        residual = residual.contiguous()
+    q, rng = _rate(what, dropout_p, rng, x)
+    return _GroupNormAct.apply(x.contiguous(), _channel_vector(what, "weight", weight, C, x),
+                               _channel_vector(what, "bias", bias, C, x), residual, offsets, samples, groups, float(eps),
+                               _lib.ACTIVATIONS[act], float(negative_slope), q, rng)

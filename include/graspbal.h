@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define GB_ABI_VERSION 7
+#define GB_ABI_VERSION 8
 
 enum {
   GB_OK = 0,
@@ -697,6 +697,55 @@ int gb_grasp_loss_bwd(const float *obj_score, const float *view_score, const flo
                       const float *aux, const int64_t *graspable, const float *den, const float *grad_out,
                       float *d_obj, float *d_view, float *d_score, float *d_angle, float *d_width, float *d_tol,
                       void *stream);
+
+/* ---- channel-last row operators beside the BatchNorm layers: group norm + activation, dropout, 8-bit products ----------
+ * Tensors are contiguous rows of fp32, bf16 or fp16 (GB_T_*), at any address that is a multiple of the element's size;
+ * sums and statistics are fp32 or fp64 and a result is rounded once.  Workspaces are caller-owned, need no clearing, and
+ * hold nothing between calls: calls on one stream may share one, calls that may run at the same time may not.          */
+#define GB_T_F32 0
+#define GB_T_BF16 1
+#define GB_T_F16 2
+#define GB_ACT_NONE 0
+#define GB_ACT_RELU 1
+#define GB_ACT_LEAKY_RELU 2 /* slope below zero: GbGroupNorm.slope */
+#define GB_ACT_SILU 3
+#define GB_ACT_GELU 4 /* 0.5 z (1 + erf(z / sqrt 2)) */
+
+/* y = keep(x) * 65536 / (65536 - q) (+ residual): element i (of n, in memory order) is kept when its 16-bit number is >= q,
+ * 0 <= q <= 65536 (a rate of q / 65536); a dropped element gives 0 whatever it holds.  The numbers are Philox4x32-10 (Salmon
+ * et al., SC 2011) under the key `seed` of the counter (i >> 3, call): 128 bits = the eight numbers of elements 8b .. 8b+7,
+ * the low half of the first word first.  No mask is stored: the backward pass is the same call on dy (without residual).
+ * rng: NULL, or a DEVICE pair [seed, call] read instead of the arguments (a captured launch follows what is written
+ * there); used: NULL, or a DEVICE pair that receives what this call used.                                              */
+int gb_dropout(const void *x, const void *residual, void *y, long long n, int dtype, int q, const int64_t *rng,
+               long long seed, long long call, int64_t *used, void *stream);
+
+/* Group norm over channel-last rows x (rows, channels): statistics per sample and group of channels / groups channels,
+ * z = weight * (x - mean) / sqrt(var + eps) + bias (+ residual), y = act(z), then dropout as in gb_dropout when q > 0.
+ *   samples / offsets: NULL offsets = `samples` samples of rows / samples rows each; else samples + 1 ascending DEVICE row
+ *     numbers, sample s = rows [offsets[s], offsets[s+1]) - none for an empty one.  Rows outside every sample get zeros (y,
+ *     dx, dresidual).  Values outside [0, rows] are brought into it.
+ *   weight, bias: (channels) fp32 or NULL (1 / 0); mean, rstd: (samples, groups) fp32, written by _fwd, read by _bwd.
+ *   channels: <= 4096, and channels / gcd(channels, 8) <= 1024 (odd counts up to 1024); samples <= 65534 - else GB_ERANGE.
+ *   rng / seed / call / used: as gb_dropout; _bwd takes the pair that _fwd used (as rng or by value; `used` is not written).
+ * _bwd: dx, dresidual (may be NULL) like x; dweight, dbias (channels) fp32 (either may be NULL), zeros' worth of rows give
+ * zeros.  x, residual, act, q must be those of _fwd.  ws: gb_group_norm_workspace bytes, 16-byte aligned.  All sums are
+ * added in a fixed order: results repeat bit for bit.  rows == 0: nothing is launched or written.                      */
+typedef struct GbGroupNorm {
+  const void *x, *residual;
+  const float *weight, *bias;
+  const int64_t *offsets;
+  float *mean, *rstd;
+  const int64_t *rng;
+  int64_t *used;
+  long long rows, seed, call;
+  int samples, channels, groups, dtype, act, q;
+  float eps, slope;
+} GbGroupNorm;
+int gb_group_norm_workspace(const GbGroupNorm *n, int backward, long long *bytes);
+int gb_group_norm_fwd(const GbGroupNorm *n, void *y, void *ws, long long ws_bytes, void *stream);
+int gb_group_norm_bwd(const GbGroupNorm *n, const void *dy, void *dx, void *dresidual, float *dweight, float *dbias,
+                      void *ws, long long ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }
