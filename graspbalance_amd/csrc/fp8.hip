@@ -1,0 +1,740 @@
+// Products in 8-bit floats with a power-of-two scale for each block of 128 (graspbal.h gb_fp8_*).
+//
+//   Y = deq(Q(X)) deq(Q(W))^T + bias;   dX = deq(Q(dY)) deq(Q(W));   dW = deq(Q(dY))^T deq(Q(X));   db = sum of dY
+//
+// Q of a block: e = the least integer with max|x| <= 448 2^e over the block's finite values (at least -126; 0 for a block of
+// zeros), codes = e4m3(x 2^-e).  X and dY have a block per 128 elements of a row, W per 128 x 128.  A power of two costs a
+// floating format nothing (scaling by it is exact), is what the matrix instructions take beside their operands, and is
+// exact in bf16.
+//
+// Two inner products, chosen by the output's type:
+//   16-bit outputs: v_mfma_scale_f32_32x32x64_f8f6f4 - 4.7 PFLOP/s on this card, scales applied by the instruction.  It adds
+//     the products of a step with about 14 bits below the largest one (measured: 5e-5 of the result's norm for codes over
+//     the whole range, 0 where they span 2^4), then accumulates in fp32: a twentieth of bf16's half step, a quarter of
+//     fp16's.
+//   fp32 outputs: the codes are turned into bf16 (exact) in registers, scale included, and go through
+//     v_mfma_f32_32x32x16_bf16 (2.35 PFLOP/s; 8e-8 of the norm).
+#include "row_common.h"
+
+#pragma clang fp contract(on)
+
+namespace gb {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+
+static constexpr int FP8_FEW_ROWS = 64;          // rows up to which the products run without LDS tiles
+static constexpr int FP8_FUSED_CODES = 16384;    // bytes of codes a workgroup quantises for itself
+static constexpr int FP8_FUSED_ROWS = 16;
+
+__host__ __device__ inline int blocks128(int k) { return (k + 127) / 128; }
+__host__ __device__ inline int scale_stride(int k) { return (blocks128(k) + 3) / 4 * 4; }   // whole dwords per row
+
+// ---- quantisers -----------------------------------------------------------------------------------------------------
+
+// biased exponent (e + 127) of a block whose largest finite magnitude is `top`: 448 = 1.75 * 2^8
+__device__ __forceinline__ int block_exponent(float top) {
+  const unsigned b = __float_as_uint(top);
+  if (b == 0) return 127;
+  const int e = (int)(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return e < 1 ? 1 : e;
+}
+__device__ __forceinline__ float power_of(int biased) { return __uint_as_float((unsigned)biased << 23); }  // 1 <= biased <= 254
+__device__ __forceinline__ float finite_magnitude(float x) {
+  const float a = fabsf(x);
+  return a <= 3.4028235e38f ? a : 0.0f;
+}
+__device__ __forceinline__ float top8(const F8 &f) {
+  float m = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_magnitude(f.v[k]));
+  return m;
+}
+// eight codes; x * 2^-e is exact wherever it reaches the codes' range; what is not finite becomes NaN
+__device__ __forceinline__ uint2 encode8(const F8 &f, int biased) {
+  const float inv = power_of(254 - biased);
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = fabsf(f.v[k]) <= 3.4028235e38f ? f.v[k] * inv : __uint_as_float(0x7fc00000u);
+  uint2 r;
+  int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false), hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+  r.x = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
+  r.y = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], hi, true);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ F8 load_upto8(const T *p, int n) {
+  if (n >= 8) return load8(p);
+  return load_tail(p, n);   // (n <= 0: nothing is read)
+}
+
+// Rows [r0, r0 + per) x block kb of 128 columns: sixteen lanes x eight elements a row.  SUM: also the column sums of these
+// rows, fp32 over per / 16 rows a lane, to part[chunk][K].
+template <typename T, bool SUM>
+__global__ __launch_bounds__(256) void fp8_rows_kernel(const T *__restrict__ x, long long P, int K, unsigned char *__restrict__ codes,
+                                                       unsigned char *__restrict__ scales, int per, float *__restrict__ part) {
+  const int cl = (int)threadIdx.x & 15, rl = (int)threadIdx.x >> 4, kb = (int)blockIdx.y, col = kb * 128 + cl * 8;
+  const long long r0 = (long long)blockIdx.x * per, r1 = r0 + per < P ? r0 + per : P;
+  const int Kp = blocks128(K) * 128, ss = scale_stride(K), n = K - col;
+  F8 sum = {};
+  for (long long r = r0 + rl; r < r1; r += 16) {
+    const F8 f = load_upto8(x + r * K + col, n);
+    const int e = block_exponent(row_max_f32(top8(f)));
+    *reinterpret_cast<uint2 *>(codes + r * Kp + col) = encode8(f, e);
+    if (cl == 0) scales[r * ss + kb] = (unsigned char)e;
+    if (SUM)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum.v[k] += f.v[k];
+  }
+  if (SUM) {
+    __shared__ float lds[16][128];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) lds[rl][cl * 8 + k] = sum.v[k];
+    __syncthreads();
+    const int c = (int)threadIdx.x;
+    if (c < 128 && kb * 128 + c < K) {
+      float s = 0;
+      for (int i = 0; i < 16; ++i) s += lds[i][c];
+      part[(long long)blockIdx.x * K + kb * 128 + c] = s;
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void fp8_colsum_kernel(const float *__restrict__ part, int chunks, int K, float *__restrict__ out) {
+  __shared__ double lds[8][32];
+  const int i = (int)threadIdx.x & 31, q = (int)threadIdx.x >> 5, c = (int)blockIdx.x * 32 + i;
+  double s = 0;
+  if (c < K)
+    for (int j = q; j < chunks; j += 8) s += part[(long long)j * K + c];
+  lds[q][i] = s;
+  __syncthreads();
+  if (q == 0 && c < K) {
+    for (int j = 1; j < 8; ++j) s += lds[j][i];
+    out[c] = (float)s;
+  }
+}
+
+// One 128 x 128 block of a weight: codes (N, Kp) and, for the product with dY, codes_t (K, Np); one exponent.
+template <typename T>
+__global__ __launch_bounds__(256) void fp8_weight_kernel(const T *__restrict__ w, int N, int K, unsigned char *__restrict__ codes,
+                                                         unsigned char *__restrict__ codes_t, unsigned char *__restrict__ scales) {
+  __shared__ float top[4];
+  __shared__ unsigned char tile[128][136];
+  const int cl = (int)threadIdx.x & 15, rl = (int)threadIdx.x >> 4, kb = (int)blockIdx.x, nb = (int)blockIdx.y;
+  const int Kb = blocks128(K), Np = blocks128(N) * 128, col = kb * 128 + cl * 8;
+  F8 f[8];
+  float m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int n = nb * 128 + i * 16 + rl;
+    f[i] = load_upto8(w + (long long)n * K + col, n < N ? K - col : 0);
+    m = fmaxf(m, top8(f[i]));
+  }
+  m = wave_max_f32(m);
+  if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
+  __syncthreads();
+  const int e = block_exponent(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+  if (threadIdx.x == 0) scales[nb * Kb + kb] = (unsigned char)e;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int n = i * 16 + rl;
+    const uint2 c = encode8(f[i], e);
+    if (nb * 128 + n < N) *reinterpret_cast<uint2 *>(codes + (long long)(nb * 128 + n) * (Kb * 128) + col) = c;
+    if (codes_t) *reinterpret_cast<uint2 *>(&tile[n][cl * 8]) = c;
+  }
+  if (!codes_t) return;
+  __syncthreads();
+  const int k = (int)threadIdx.x >> 1, h = ((int)threadIdx.x & 1) * 64;
+  if (kb * 128 + k < K)
+    for (int j = 0; j < 64; j += 16) {
+      unsigned v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = h + j + 4 * q;
+        v[q] = tile[n][k] | tile[n + 1][k] << 8 | tile[n + 2][k] << 16 | (unsigned)tile[n + 3][k] << 24;
+      }
+      *reinterpret_cast<uint4 *>(codes_t + (long long)(kb * 128 + k) * Np + nb * 128 + h + j) = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+// ---- fragments ------------------------------------------------------------------------------------------------------
+
+// Codes 8j .. 8j+7 of a lane's 32 as bf16 times 2^scale (exact): one operand of a 32x32x16 / 16x16x32 bf16 step.  Which
+// element of the reduction a lane holds does not matter as long as both operands hold the same one.
+__device__ __forceinline__ bf16x8 decode8(unsigned lo, unsigned hi, float scale) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true),
+               c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+  bf16x8 r;
+  r[0] = a[0], r[1] = a[1], r[2] = b[0], r[3] = b[1], r[4] = c[0], r[5] = c[1], r[6] = d[0], r[7] = d[1];
+  return r;
+}
+
+template <typename T>
+struct Exact {  // fp32 outputs take the bf16 products
+  static constexpr bool value = sizeof(T) == 4;
+};
+
+// ---- tiles ----------------------------------------------------------------------------------------------------------
+// A workgroup of WM x WN waves, each with TM x TN tiles of 32 x 32, steps through the reduction 128 codes (one scale block)
+// at a time: two LDS stages filled by LDS-DMA, the next one in flight while this one is multiplied.  An LDS row is 128
+// codes, eight chunks of 16 bytes; chunk c of row r lies at place c ^ key(r) (the DMA writes lane-linearly, so the lane's
+// SOURCE is permuted), which spreads the eight rows that a group of lanes reads over all banks.  key(r) = r & 7 for rows of
+// X and (r >> 1) & 7 for rows of W: the tiles of W come in pairs and lane j of a pair takes rows 2j and 2j + 1, so that a
+// lane ends up with two neighbouring outputs.
+
+struct GemmArgs8 {
+  const unsigned char *a, *a_scales, *b, *b_scales;  // a (P, Kp), b (N, Kp); a_scales (P, stride), b_scales by block
+  const float *bias;
+  void *y;
+  long long P;
+  int N, Kb, a_stride, bs_n, bs_k, tiles_n;
+  long long tiles;
+};
+
+__device__ __forceinline__ void dma16(const unsigned char *src, unsigned char *lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)lds,
+                                   16, 0, 0);
+}
+
+template <typename T, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(GemmArgs8 g) {
+  constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, WAVES = WM * WN, ROWS = BM + BN, LOADS = ROWS / (8 * WAVES);
+  constexpr bool EXACT = Exact<T>::value;
+  static_assert(TN % 2 == 0 && ROWS % (8 * WAVES) == 0 && (32 * TN) <= 128, "tile");
+  __shared__ __attribute__((aligned(128))) unsigned char lds[2][ROWS * 128];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave / WN, wn = wave % WN, j = lane & 31, h = lane >> 5;
+  // neighbouring tiles on one XCD (workgroups go to the eight XCDs in turn): its L2 then holds their common rows
+  const long long per = g.tiles >> 3, extra = g.tiles & 7, x = blockIdx.x & 7;
+  const long long tile = x * per + (x < extra ? x : extra) + (blockIdx.x >> 3);
+  const long long p0 = tile / g.tiles_n * BM;
+  const int n0 = (int)(tile % g.tiles_n) * BN, Kp = g.Kb * 128;
+  const unsigned char *a = g.a + p0 * Kp, *b = g.b + (long long)n0 * Kp;
+  const int last_a = (int)(g.P - p0 < BM ? g.P - p0 : BM) - 1, last_b = (g.N - n0 < BN ? g.N - n0 : BN) - 1;
+
+  // the lane's share of a stage: 16 bytes of LOADS rows (rows behind the last repeat it; their outputs are not stored)
+  int off[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int row = (i * WAVES + wave) * 8 + (lane >> 3);
+    const bool of_a = row < BM;
+    const int r = of_a ? row : row - BM, key = of_a ? r & 7 : r >> 1 & 7, last = of_a ? last_a : last_b;
+    off[i] = (r < last ? r : last) * Kp + ((lane & 7) ^ key) * 16;
+  }
+  auto request = [&](int kb, unsigned char *stage) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int first = (i * WAVES + wave) * 8;
+      dma16((first < BM ? a : b) + off[i] + kb * 128, stage + first * 128);
+    }
+  };
+
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int m = 0; m < TM; ++m)
+#pragma unroll
+    for (int n = 0; n < TN; ++n) acc[m][n] = f32x16{};
+  const unsigned char *as[TM];
+  unsigned sa[TM];
+#pragma unroll
+  for (int m = 0; m < TM; ++m) {
+    const int r = wm * 32 * TM + 32 * m + j;
+    as[m] = g.a_scales + (p0 + (r < last_a ? r : last_a)) * g.a_stride;
+  }
+  const int nb = (n0 + wn * 32 * TN) / 128, nbs = nb < (g.N + 127) / 128 ? nb : (g.N + 127) / 128 - 1;
+  const unsigned char *bs = g.b_scales + (long long)nbs * g.bs_n;
+
+  request(0, lds[0]);
+  for (int kb = 0; kb < g.Kb; ++kb) {
+    if ((kb & 3) == 0)
+#pragma unroll
+      for (int m = 0; m < TM; ++m) sa[m] = *reinterpret_cast<const unsigned *>(as[m] + kb);
+    const unsigned sb = bs[(long long)kb * g.bs_k];
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();   // this stage is complete, and nobody reads the other one any more
+    if (kb + 1 < g.Kb) request(kb + 1, lds[(kb + 1) & 1]);
+    const unsigned char *st = lds[kb & 1];
+    const unsigned char *la = st + (wm * 32 * TM + j) * 128, *lb = st + (BM + wn * 32 * TN + 2 * j) * 128;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {   // 64 codes: lane half h holds 32 of them
+      const int c0 = ((4 * s + 2 * h) ^ (j & 7)) * 16, c1 = ((4 * s + 2 * h + 1) ^ (j & 7)) * 16;
+      i32x4 fa[TM][2], fb[TN][2];
+#pragma unroll
+      for (int n = 0; n < TN; ++n) {
+        const unsigned char *r = lb + (n / 2 * 64 + n % 2) * 128;
+        fb[n][0] = *reinterpret_cast<const i32x4 *>(r + c0);
+        fb[n][1] = *reinterpret_cast<const i32x4 *>(r + c1);
+      }
+#pragma unroll
+      for (int m = 0; m < TM; ++m) {
+        const unsigned char *r = la + 32 * m * 128;
+        fa[m][0] = *reinterpret_cast<const i32x4 *>(r + c0);
+        fa[m][1] = *reinterpret_cast<const i32x4 *>(r + c1);
+      }
+      if (EXACT) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          bf16x8 db[TN];
+#pragma unroll
+          for (int n = 0; n < TN; ++n)
+            db[n] = decode8((unsigned)fb[n][q / 2][q % 2 * 2], (unsigned)fb[n][q / 2][q % 2 * 2 + 1], power_of((int)sb));
+#pragma unroll
+          for (int m = 0; m < TM; ++m) {
+            const bf16x8 da = decode8((unsigned)fa[m][q / 2][q % 2 * 2], (unsigned)fa[m][q / 2][q % 2 * 2 + 1],
+                                      power_of((int)(sa[m] >> (8 * (kb & 3)) & 0xff)));
+#pragma unroll
+            for (int n = 0; n < TN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(da, db[n], acc[m][n], 0, 0, 0);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int m = 0; m < TM; ++m) {
+          const i32x8 va = __builtin_shufflevector(fa[m][0], fa[m][1], 0, 1, 2, 3, 4, 5, 6, 7);
+          const int s8 = (int)(sa[m] >> (8 * (kb & 3)) & 0xff);
+#pragma unroll
+          for (int n = 0; n < TN; ++n) {
+            const i32x8 vb = __builtin_shufflevector(fb[n][0], fb[n][1], 0, 1, 2, 3, 4, 5, 6, 7);
+            acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va, vb, acc[m][n], 0, 0, 0, s8, 0, (int)sb);
+          }
+        }
+      }
+    }
+  }
+
+  T *y = (T *)g.y + p0 * g.N;
+#pragma unroll
+  for (int n = 0; n < TN; n += 2) {
+    const int col = n0 + wn * 32 * TN + 32 * n + 2 * j;
+    const bool two = col + 1 < g.N;
+    if (col >= g.N) continue;
+    const float b0 = g.bias ? g.bias[col] : 0.0f, b1 = g.bias && two ? g.bias[col + 1] : 0.0f;
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = wm * 32 * TM + 32 * m + i / 4 * 8 + h * 4 + i % 4;
+        if (r > last_a) continue;
+        const T v[2] = {(T)(acc[m][n][i] + b0), (T)(acc[m][n + 1][i] + b1)};
+        T *to = y + (long long)r * g.N + col;
+        if (two)
+          __builtin_memcpy(to, v, sizeof(v));
+        else
+          *to = v[0];
+      }
+  }
+}
+
+// ---- few rows -------------------------------------------------------------------------------------------------------
+// Up to 64 rows: bound by reading W once.  A workgroup takes 16 outputs; its waves take the blocks of 128 in turn, a lane
+// reads 32 codes of W straight into the operand of a 16-row step (the four lanes of a row read one 128-byte line), and the
+// waves' sums meet in LDS.  FUSED: every workgroup quantises the few rows of X for itself (one launch instead of two).
+template <typename T, int PT, bool FUSED>
+__global__ __launch_bounds__(256) void fp8_few_kernel(GemmArgs8 g, const T *__restrict__ x, int K) {
+  constexpr bool EXACT = Exact<T>::value;
+  __shared__ float sums[4][PT][64][4];
+  extern __shared__ __attribute__((aligned(16))) unsigned char codes[];   // FUSED: P x Kp codes, P x Kb exponents
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, j = lane & 15, q = lane >> 4;
+  const int n0 = (int)blockIdx.x * 16, Kp = g.Kb * 128, P = (int)g.P;
+  const unsigned char *ex = codes + P * Kp;
+  if (FUSED) {
+    const int cl = (int)threadIdx.x & 15;
+    for (int i = (int)threadIdx.x >> 4; i < P * g.Kb; i += 16) {
+      const int r = i / g.Kb, kb = i - r * g.Kb, col = kb * 128 + cl * 8;
+      const F8 f = load_upto8(x + (long long)r * K + col, K - col);
+      const int e = block_exponent(row_max_f32(top8(f)));
+      *reinterpret_cast<uint2 *>(codes + r * Kp + col) = encode8(f, e);
+      if (cl == 0) codes[P * Kp + r * g.Kb + kb] = (unsigned char)e;
+    }
+    __syncthreads();
+  }
+  const int n = n0 + j < g.N ? n0 + j : g.N - 1;
+  const unsigned char *w = g.b + (long long)n * Kp + q * 32, *bs = g.b_scales + (long long)(n0 / 128) * g.bs_n;
+  f32x4 acc[PT];
+  int row[PT];
+#pragma unroll
+  for (int t = 0; t < PT; ++t) {
+    acc[t] = f32x4{};
+    row[t] = 16 * t + j < P ? 16 * t + j : P - 1;
+  }
+  for (int kb = wave; kb < g.Kb; kb += 4) {
+    const i32x4 w0 = *reinterpret_cast<const i32x4 *>(w + kb * 128), w1 = *reinterpret_cast<const i32x4 *>(w + kb * 128 + 16);
+    const int sw = bs[(long long)kb * g.bs_k];
+#pragma unroll
+    for (int t = 0; t < PT; ++t) {
+      const unsigned char *c = (FUSED ? codes : g.a) + (long long)row[t] * Kp + kb * 128 + q * 32;
+      const int sx = FUSED ? ex[row[t] * g.Kb + kb] : g.a_scales[(long long)row[t] * g.a_stride + kb];
+      const i32x4 x0 = *reinterpret_cast<const i32x4 *>(c), x1 = *reinterpret_cast<const i32x4 *>(c + 16);
+      if (EXACT) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const i32x4 &wq = i < 2 ? w0 : w1, &xq = i < 2 ? x0 : x1;
+          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              decode8((unsigned)wq[i % 2 * 2], (unsigned)wq[i % 2 * 2 + 1], power_of(sw)),
+              decode8((unsigned)xq[i % 2 * 2], (unsigned)xq[i % 2 * 2 + 1], power_of(sx)), acc[t], 0, 0, 0);
+        }
+      } else {
+        acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7),
+                                                                  __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7), acc[t], 0,
+                                                                  0, 0, sw, 0, sx);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < PT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[wave][t][lane][i] = acc[t][i];
+  __syncthreads();
+  if (wave >= PT) return;
+  for (int t = wave; t < PT; t += 4) {   // lane: row 16 t + j, outputs n0 + 4 q ..
+    const int r = 16 * t + j;
+    if (r >= P) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = n0 + 4 * q + i;
+      if (c >= g.N) break;
+      const float s = (sums[0][t][lane][i] + sums[1][t][lane][i]) + (sums[2][t][lane][i] + sums[3][t][lane][i]);
+      ((T *)g.y)[(long long)r * g.N + c] = (T)(s + (g.bias ? g.bias[c] : 0.0f));
+    }
+  }
+}
+
+// ---- weight gradient ------------------------------------------------------------------------------------------------
+// dW[n][k] = sum over rows p of deq(dY)[p][n] deq(X)[p][k].  The scales belong to rows, i.e. to the reduction, and cannot leave
+// the sum: the codes become bf16 with their scale (exact) on the way into LDS, and the bf16 matrix instructions do the
+// rest in fp32.  Both operands lie in memory with the reduction as the slow index; ds_read_b64_tr_b16 hands every lane four
+// rows of its column.  An LDS row is padded by 64 bytes: the four rows that sixteen lanes read then start 16 banks apart.
+// Many rows and few outputs: the rows are cut into `splits` ranges, each range's sum goes to the workspace and a second
+// kernel adds them in order.
+struct WgradArgs8 {
+  const unsigned char *dy, *dys, *x, *xs;
+  float *out;
+  long long P, rows;   // rows per split (a multiple of the step)
+  int N, K, tiles_k;
+};
+
+typedef __attribute__((address_space(3))) bf16x4_t lds_bf16x4;
+
+template <int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void fp8_wgrad_kernel(WgradArgs8 g) {
+  constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, THREADS = 64 * WM * WN, STEP = 32;
+  constexpr int CA = BM / 16, CH = (BM + BN) / 16, LOADS = STEP * CH / THREADS;
+  constexpr int SA = BM * 2 + 64, SB = BN * 2 + 64, STAGE = STEP * (SA + SB);
+  static_assert(STEP * CH % THREADS == 0, "loads");
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2][STAGE];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+  const int n0 = (int)(blockIdx.x / g.tiles_k) * BM, k0 = (int)(blockIdx.x % g.tiles_k) * BN;
+  const int Np = blocks128(g.N) * 128, Kp = blocks128(g.K) * 128, sn = scale_stride(g.N), sk = scale_stride(g.K);
+  const long long p0 = g.rows * blockIdx.y, p1 = p0 + g.rows < g.P ? p0 + g.rows : g.P;
+
+  // the lane's share of a step: sixteen codes of LOADS rows, as they are in memory
+  int row[LOADS], to[LOADS];
+  const unsigned char *src[LOADS], *scl[LOADS];
+  int ld[LOADS], sld[LOADS];
+  bool in[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int c = i * THREADS + (int)threadIdx.x, cc = c % CH;
+    row[i] = c / CH;
+    const bool of_a = cc < CA;
+    const int col = of_a ? n0 + cc * 16 : k0 + (cc - CA) * 16, width = of_a ? Np : Kp;
+    in[i] = col < width;
+    const int at = in[i] ? col : 0;
+    src[i] = (of_a ? g.dy : g.x) + at;
+    scl[i] = (of_a ? g.dys : g.xs) + at / 128;
+    ld[i] = width;
+    sld[i] = of_a ? sn : sk;
+    to[i] = of_a ? row[i] * SA + cc * 32 : STEP * SA + row[i] * SB + (cc - CA) * 32;
+  }
+  uint4 code[LOADS];
+  unsigned scale[LOADS];
+  auto fetch = [&](long long p) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const long long r = p + row[i], at = r < p1 ? r : p1 - 1;
+      code[i] = *reinterpret_cast<const uint4 *>(src[i] + at * ld[i]);
+      scale[i] = scl[i][at * sld[i]];
+      if (!in[i] || r >= p1) code[i] = make_uint4(0, 0, 0, 0);
+    }
+  };
+  auto put = [&](unsigned char *stage) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const float s = power_of((int)scale[i]);
+      *reinterpret_cast<bf16x8 *>(stage + to[i]) = decode8(code[i].x, code[i].y, s);
+      *reinterpret_cast<bf16x8 *>(stage + to[i] + 16) = decode8(code[i].z, code[i].w, s);
+    }
+  };
+
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int m = 0; m < TM; ++m)
+#pragma unroll
+    for (int n = 0; n < TN; ++n) acc[m][n] = f32x16{};
+  const int sub = lane & 15, right = (lane >> 4 & 1) * 16 + (sub & 3) * 4, down = (lane >> 5) * 8 + (sub >> 2);
+  const int fa = down * SA + (wm * 32 * TM + right) * 2, fb = STEP * SA + down * SB + (wn * 32 * TN + right) * 2;
+  if (p0 < p1) {
+    fetch(p0);
+    put(lds[0]);
+    __syncthreads();
+    int cur = 0;
+    for (long long p = p0; p < p1; p += STEP, cur ^= 1) {
+      const bool more = p + STEP < p1;
+      if (more) fetch(p + STEP);
+      unsigned char *st = lds[cur];
+#pragma unroll
+      for (int s = 0; s < STEP / 16; ++s) {
+        bf16x8 a[TM], b[TN];
+#pragma unroll
+        for (int m = 0; m < TM; ++m) {
+          unsigned char *at = st + fa + s * 16 * SA + m * 64;
+          a[m] = __builtin_shufflevector(__builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(at)),
+                                         __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(at + 4 * SA)), 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+#pragma unroll
+        for (int n = 0; n < TN; ++n) {
+          unsigned char *at = st + fb + s * 16 * SB + n * 64;
+          b[n] = __builtin_shufflevector(__builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(at)),
+                                         __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(at + 4 * SB)), 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+#pragma unroll
+        for (int m = 0; m < TM; ++m)
+#pragma unroll
+          for (int n = 0; n < TN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[m], b[n], acc[m][n], 0, 0, 0);
+      }
+      if (more) put(lds[cur ^ 1]);
+      __syncthreads();
+    }
+  }
+  float *out = g.out + (long long)blockIdx.y * g.N * g.K;
+  const int j = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int m = 0; m < TM; ++m)
+#pragma unroll
+    for (int n = 0; n < TN; ++n) {
+      const int col = k0 + wn * 32 * TN + 32 * n + j;
+      if (col >= g.K) continue;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = n0 + wm * 32 * TM + 32 * m + i / 4 * 8 + h * 4 + i % 4;
+        if (r < g.N) out[(long long)r * g.K + col] = acc[m][n][i];
+      }
+    }
+}
+
+// out[i] = the splits' sums added in order: 64 elements x 4 lanes over the splits
+__global__ __launch_bounds__(256) void fp8_wgrad_join_kernel(const float *__restrict__ part, int splits, long long n,
+                                                             float *__restrict__ out) {
+  __shared__ float lds[4][64];
+  const int i = (int)threadIdx.x & 63, q = (int)threadIdx.x >> 6;
+  const long long e = (long long)blockIdx.x * 64 + i;
+  float s = 0;
+  if (e < n)
+    for (int k = q; k < splits; k += 4) s += part[(long long)k * n + e];
+  lds[q][i] = s;
+  __syncthreads();
+  if (q == 0 && e < n) out[e] = (lds[0][i] + lds[1][i]) + (lds[2][i] + lds[3][i]);
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+
+template <typename T, int TM, int TN, int WM, int WN>
+static int launch_tiles(GemmArgs8 g, hipStream_t st) {
+  constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
+  g.tiles_n = (g.N + BN - 1) / BN;
+  g.tiles = (g.P + BM - 1) / BM * g.tiles_n;
+  if (g.tiles > 0x7fffffffll) return GB_ERANGE;
+  fp8_gemm_kernel<T, TM, TN, WM, WN><<<(unsigned)g.tiles, 64 * WM * WN, 0, st>>>(g);
+  return check_launch("gb_fp8_gemm");
+}
+
+static long long tiles_of(long long P, int N, int b) { return ((P + b - 1) / b) * ((N + b - 1) / b); }
+
+static bool fp8_dims_bad(long long P, int N, int K) { return P < 0 || N <= 0 || K <= 0; }
+static bool fp8_dims_large(long long P, int N, int K) {   // int tile offsets: 256 rows of Kp bytes; 65535 blocks a grid axis
+  return N > (1 << 22) || K > (1 << 22) || P > (1ll << 40);
+}
+
+static int rows_per_chunk(long long P, bool sum) {
+  if (!sum) return 64;
+  const long long per = (P + 511) / 512;
+  return (int)(per < 64 ? 64 : (per + 15) / 16 * 16);
+}
+
+struct WgradPlan8 {
+  bool big;
+  int tiles_n, tiles_k, splits;
+  long long rows;
+};
+// 256 x 256 outputs per workgroup where both sides fill them, else 128 x 128; the rows are cut until there are ~512
+// workgroups, into ranges of 512 rows at least (a range writes its outputs once more and has them read once more).
+static WgradPlan8 wgrad_plan(long long P, int N, int K) {
+  WgradPlan8 p;
+  p.big = N > 192 && K > 192;
+  const int b = p.big ? 256 : 128;
+  p.tiles_n = (N + b - 1) / b;
+  p.tiles_k = (K + b - 1) / b;
+  const long long tiles = (long long)p.tiles_n * p.tiles_k, want = (512 + tiles - 1) / tiles, most = (P + 511) / 512;
+  long long splits = want < most ? want : most;
+  if (splits < 1) splits = 1;
+  p.rows = ((P + splits - 1) / splits + 31) / 32 * 32;
+  p.splits = p.rows ? (int)((P + p.rows - 1) / p.rows) : 0;
+  return p;
+}
+
+}  // namespace gb
+
+using namespace gb;
+
+extern "C" int gb_fp8_quant_rows(const void *x, int dtype, long long P, int K, void *codes, void *scales, float *colsum, void *ws,
+                                 long long ws_bytes, void *stream) {
+  if (fp8_dims_bad(P, 1, K) || !known_type(dtype)) return GB_EINVAL;
+  if (fp8_dims_large(P, 1, K)) return GB_ERANGE;
+  const int per = rows_per_chunk(P, colsum != nullptr);
+  const long long chunks = (P + per - 1) / per;
+  if (chunks > 0x7fffffffll || blocks128(K) > 65535) return GB_ERANGE;
+  if (P == 0 && !colsum) return GB_OK;
+  if (P > 0 && (!x || !codes || !scales || (reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) % 16)) return GB_EINVAL;
+  if (colsum && chunks > 0 && (!ws || ws_bytes < chunks * K * 4 || reinterpret_cast<uintptr_t>(ws) % 16)) return GB_EINVAL;
+  hipStream_t st = as_stream(stream);
+  return with_type(dtype, [&](auto z) {
+    typedef decltype(z) T;
+    const dim3 grid((unsigned)chunks, (unsigned)blocks128(K));
+    if (colsum) {
+      if (P > 0)
+        fp8_rows_kernel<T, true><<<grid, 256, 0, st>>>((const T *)x, P, K, (unsigned char *)codes, (unsigned char *)scales, per, (float *)ws);
+      fp8_colsum_kernel<<<(K + 31) / 32, 256, 0, st>>>((const float *)ws, (int)chunks, K, colsum);
+    } else {
+      fp8_rows_kernel<T, false><<<grid, 256, 0, st>>>((const T *)x, P, K, (unsigned char *)codes, (unsigned char *)scales, per, nullptr);
+    }
+    return check_launch("gb_fp8_quant_rows");
+  });
+}
+
+extern "C" int gb_fp8_quant_weight(const void *w, int dtype, int N, int K, void *codes, void *codes_t, void *scales, void *stream) {
+  if (fp8_dims_bad(0, N, K) || !known_type(dtype)) return GB_EINVAL;
+  if (fp8_dims_large(0, N, K)) return GB_ERANGE;
+  if (!w || !codes || !scales || (reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(codes_t)) % 16) return GB_EINVAL;
+  return with_type(dtype, [&](auto z) {
+    typedef decltype(z) T;
+    fp8_weight_kernel<T><<<dim3((unsigned)blocks128(K), (unsigned)blocks128(N)), 256, 0, as_stream(stream)>>>(
+        (const T *)w, N, K, (unsigned char *)codes, (unsigned char *)codes_t, (unsigned char *)scales);
+    return check_launch("gb_fp8_quant_weight");
+  });
+}
+
+static int fp8_args_bad(const void *b, const void *b_scales, const void *y) {
+  return !b || !b_scales || !y || reinterpret_cast<uintptr_t>(b) % 16;
+}
+
+extern "C" int gb_fp8_gemm(const void *a, const void *a_scales, const void *b, const void *b_scales, int transposed, const float *bias,
+                           void *y, int dtype, long long P, int N, int K, void *stream) {
+  if (fp8_dims_bad(P, N, K) || !known_type(dtype)) return GB_EINVAL;
+  if (fp8_dims_large(P, N, K)) return GB_ERANGE;
+  if (P == 0) return GB_OK;
+  if (fp8_args_bad(b, b_scales, y) || !a || !a_scales || (reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(a_scales)) % 16)
+    return GB_EINVAL;
+  GemmArgs8 g = {};
+  g.a = (const unsigned char *)a;
+  g.a_scales = (const unsigned char *)a_scales;
+  g.b = (const unsigned char *)b;
+  g.b_scales = (const unsigned char *)b_scales;
+  g.bias = bias;
+  g.y = y;
+  g.P = P;
+  g.N = N;
+  g.Kb = blocks128(K);
+  g.a_stride = scale_stride(K);
+  g.bs_n = transposed ? 1 : g.Kb;
+  g.bs_k = transposed ? blocks128(N) : 1;
+  hipStream_t st = as_stream(stream);
+  return with_type(dtype, [&](auto z) {
+    typedef decltype(z) T;
+    if (P <= FP8_FEW_ROWS) {
+      const unsigned grid = (unsigned)((N + 15) / 16);
+      if (P <= 16)
+        fp8_few_kernel<T, 1, false><<<grid, 256, 0, st>>>(g, nullptr, K);
+      else if (P <= 32)
+        fp8_few_kernel<T, 2, false><<<grid, 256, 0, st>>>(g, nullptr, K);
+      else
+        fp8_few_kernel<T, 4, false><<<grid, 256, 0, st>>>(g, nullptr, K);
+      return check_launch("gb_fp8_gemm");
+    }
+    // the largest tile that still gives every CU one
+    if (tiles_of(P, N, 256) >= 256) return launch_tiles<T, 4, 2, 2, 4>(g, st);
+    if (tiles_of(P, N, 128) >= 256) return launch_tiles<T, 2, 2, 2, 2>(g, st);
+    return launch_tiles<T, 1, 2, 2, 1>(g, st);
+  });
+}
+
+extern "C" int gb_fp8_linear_few(const void *x, const void *b, const void *b_scales, const float *bias, void *y, int dtype, int P, int N,
+                                 int K, void *stream) {
+  if (fp8_dims_bad(P, N, K) || !known_type(dtype)) return GB_EINVAL;
+  if (fp8_dims_large(P, N, K) || P > FP8_FUSED_ROWS || (long long)P * blocks128(K) * 128 > FP8_FUSED_CODES) return GB_ERANGE;
+  if (P == 0) return GB_OK;
+  if (fp8_args_bad(b, b_scales, y) || !x) return GB_EINVAL;
+  GemmArgs8 g = {};
+  g.b = (const unsigned char *)b;
+  g.b_scales = (const unsigned char *)b_scales;
+  g.bias = bias;
+  g.y = y;
+  g.P = P;
+  g.N = N;
+  g.Kb = blocks128(K);
+  g.bs_n = g.Kb;
+  g.bs_k = 1;
+  const size_t lds = ((size_t)P * g.Kb * 129 + 15) / 16 * 16;
+  return with_type(dtype, [&](auto z) {
+    typedef decltype(z) T;
+    fp8_few_kernel<T, 1, true><<<(unsigned)((N + 15) / 16), 256, lds, as_stream(stream)>>>(g, (const T *)x, K);
+    return check_launch("gb_fp8_linear_few");
+  });
+}
+
+extern "C" int gb_fp8_workspace(int what, long long P, int N, int K, long long *bytes) {
+  if (fp8_dims_bad(P, N, K) || !bytes || (what != GB_FP8_WS_COLSUM && what != GB_FP8_WS_WGRAD)) return GB_EINVAL;
+  if (fp8_dims_large(P, N, K)) return GB_ERANGE;
+  if (what == GB_FP8_WS_COLSUM) {
+    const int per = rows_per_chunk(P, true);
+    *bytes = (P + per - 1) / per * N * 4;
+  } else {
+    const WgradPlan8 p = wgrad_plan(P, N, K);
+    *bytes = p.splits > 1 ? (long long)p.splits * N * K * 4 : 0;
+  }
+  return GB_OK;
+}
+
+extern "C" int gb_fp8_wgrad(const void *dy, const void *dy_scales, const void *x, const void *x_scales, float *dw, long long P, int N, int K,
+                            void *ws, long long ws_bytes, void *stream) {
+  if (fp8_dims_bad(P, N, K)) return GB_EINVAL;
+  if (fp8_dims_large(P, N, K)) return GB_ERANGE;
+  if (!dw || (P > 0 && (!dy || !dy_scales || !x || !x_scales || (reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(x)) % 16)))
+    return GB_EINVAL;
+  const WgradPlan8 p = wgrad_plan(P, N, K);
+  const long long n = (long long)N * K;
+  if (p.splits > 1 && (!ws || ws_bytes < p.splits * n * 4 || reinterpret_cast<uintptr_t>(ws) % 16)) return GB_EINVAL;
+  if ((long long)p.tiles_n * p.tiles_k > 0x7fffffffll || (n + 63) / 64 > 0x7fffffffll) return GB_ERANGE;
+  hipStream_t st = as_stream(stream);
+  WgradArgs8 g = {};
+  g.dy = (const unsigned char *)dy;
+  g.dys = (const unsigned char *)dy_scales;
+  g.x = (const unsigned char *)x;
+  g.xs = (const unsigned char *)x_scales;
+  g.out = p.splits > 1 ? (float *)ws : dw;
+  g.P = P;
+  g.rows = p.rows;
+  g.N = N;
+  g.K = K;
+  g.tiles_k = p.tiles_k;
+  const dim3 grid((unsigned)(p.tiles_n * p.tiles_k), (unsigned)p.splits);
+  if (p.splits > 0) {
+    if (p.big)
+      fp8_wgrad_kernel<4, 2, 2, 4><<<grid, 512, 0, st>>>(g);
+    else
+      fp8_wgrad_kernel<2, 2, 2, 2><<<grid, 256, 0, st>>>(g);
+  }
+  if (p.splits != 1) fp8_wgrad_join_kernel<<<(unsigned)((n + 63) / 64), 256, 0, st>>>((const float *)ws, p.splits, n, dw);
+  return check_launch("gb_fp8_wgrad");
+}

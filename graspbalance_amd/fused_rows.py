@@ -1,5 +1,5 @@
 """Channel-last row operators beside the BatchNorm stacks of fused_mlp (no reference counterpart): group norm with an
-activation, dropout from a counter-based generator.
+activation, dropout from a counter-based generator, products in 8-bit floats with a scale for each block of 128.
 
 Rows are (..., C) tensors in fp32, bf16 or fp16 with the channels last, as everywhere on the fused path.  Kernels run on the
 current stream of the tensors' device; workspaces come from torch's allocator inside the call, so that every captured graph
@@ -230,3 +230,163 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
     return _GroupNormAct.apply(x.contiguous(), _channel_vector(what, "weight", weight, C, x),
                                _channel_vector(what, "bias", bias, C, x), residual, offsets, samples, groups, float(eps),
                                _lib.ACTIVATIONS[act], float(negative_slope), q, rng)
+
+
+# ---- products in 8-bit floats -----------------------------------------------------------------------------------------
+
+_FEW_ROWS, _FEW_CODES = 16, 16384     # gb_fp8_linear_few
+
+
+def _up(n, m):
+    return (n + m - 1) // m * m
+
+
+def _quantise_rows(x2, colsum=False):
+    """(codes, scales, column sums | None) of rows (P, K)."""
+    P, K = x2.shape
+    dev = x2.device
+    codes = torch.empty((P, _up(K, 128)), dtype=torch.uint8, device=dev)
+    scales = torch.empty((P, _up(_up(K, 128) // 128, 4)), dtype=torch.uint8, device=dev)
+    sums = ws = None
+    size = 0
+    if colsum:
+        sums = torch.empty(K, dtype=torch.float32, device=dev)
+        ws, size = _fp8_workspace(0, P, K, 1, dev)
+    _call("gb_fp8_quant_rows", dev, _lib.ptr(x2), _TYPES[x2.dtype], P, K, _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(sums),
+          _lib.ptr(ws), size, _s(x2))
+    return codes, scales, sums
+
+
+def _fp8_workspace(what, P, N, K, dev):
+    size = ctypes.c_longlong()
+    _lib.check(_lib.lib().gb_fp8_workspace(what, P, N, K, ctypes.byref(size)), "fp8_linear")
+    return (torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None), size.value
+
+
+def _quantise_weight(w, transposed):
+    """(codes, codes_t | None, scales) of a weight (N, K)."""
+    N, K = w.shape
+    dev = w.device
+    codes = torch.empty((N, _up(K, 128)), dtype=torch.uint8, device=dev)
+    codes_t = torch.empty((K, _up(N, 128)), dtype=torch.uint8, device=dev) if transposed else None
+    scales = torch.empty((_up(N, 128) // 128, _up(K, 128) // 128), dtype=torch.uint8, device=dev)
+    _call("gb_fp8_quant_weight", dev, _lib.ptr(w), _TYPES[w.dtype], N, K, _lib.ptr(codes), _lib.ptr(codes_t), _lib.ptr(scales),
+          _s(w))
+    return codes, codes_t, scales
+
+
+class Fp8Weight:
+    """A weight (out_features, in_features) held in 8 bits for fp8_linear: ``codes`` (out_features, in_features up to whole
+    blocks of 128, zeros behind) as torch.float8_e4m3fn, ``scales`` one biased exponent (1 .. 254; scale 2^(byte - 127)) per
+    block of 128 x 128 as uint8, and for gradients of the input ``codes_t`` (in_features, out_features up to whole blocks).
+    Make one from a float weight with ``Fp8Weight.quantize``."""
+
+    def __init__(self, codes, scales, in_features, codes_t=None):
+        what = "Fp8Weight"
+        N, K = codes.shape[0], int(in_features)
+        for name, t, shape, types in (
+                ("codes", codes, (N, _up(K, 128)), (torch.float8_e4m3fn, torch.uint8)),
+                ("scales", scales, (_up(N, 128) // 128, _up(K, 128) // 128), (torch.uint8,)),
+                ("codes_t", codes_t, (K, _up(N, 128)), (torch.float8_e4m3fn, torch.uint8))):
+            if t is None and name == "codes_t":
+                continue
+            if not t.is_cuda:
+                _refuse(what, "CPU not supported (%s)" % name)
+            if N <= 0 or K <= 0 or t.shape != shape or t.dtype not in types or t.device != codes.device \
+                    or not t.is_contiguous() or (name != "scales" and t.data_ptr() % 16):
+                _refuse(what, "%s must be a contiguous, 16-byte aligned %s tensor of %s" % (name, types[0], shape))
+        self.codes, self.scales, self.codes_t = codes, scales, codes_t
+        self.in_features, self.out_features = K, N
+
+    @classmethod
+    def quantize(cls, weight, input_gradients=False):
+        """From a float weight (out_features, in_features); input_gradients: also what fp8_linear's backward pass needs."""
+        w = _fp8_weight_tensor("Fp8Weight", weight.detach()).contiguous()
+        codes, codes_t, scales = _quantise_weight(w, input_gradients)
+        view = lambda t: None if t is None else t.view(torch.float8_e4m3fn)   # noqa: E731
+        return cls(view(codes), scales, w.shape[1], view(codes_t))
+
+
+def _fp8_weight_tensor(what, w):
+    _rows_tensor(what, "weight", w)
+    if w.dim() < 2 or w.numel() == 0 or any(n != 1 for n in w.shape[2:]):
+        _refuse(what, "weight must be (out_features, in_features) or that of a 1x1 convolution")
+    return w.view(w.shape[0], w.shape[1]) if w.dim() > 2 else w
+
+
+class _Fp8Linear(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, held):
+        dev, st = x.device, _s(x)
+        P, K = x.shape
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        if held is None:
+            weight = weight.contiguous()
+            N = weight.shape[0]
+            codes, codes_t, scales = _quantise_weight(weight, need_x)
+        else:
+            N, codes, codes_t, scales = held.out_features, held.codes, held.codes_t, held.scales
+            if need_x and codes_t is None:
+                _refuse("fp8_linear", "gradients of the input need Fp8Weight.quantize(weight, input_gradients=True)")
+        y = torch.empty((P, N), dtype=x.dtype, device=dev)
+        xq = xs = None
+        if P <= _FEW_ROWS and P * codes.shape[1] <= _FEW_CODES and not need_w:
+            _call("gb_fp8_linear_few", dev, _lib.ptr(x), _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(bias), _lib.ptr(y),
+                  _TYPES[x.dtype], P, N, K, st)
+        else:
+            xq, xs, _ = _quantise_rows(x)
+            _call("gb_fp8_gemm", dev, _lib.ptr(xq), _lib.ptr(xs), _lib.ptr(codes), _lib.ptr(scales), 0, _lib.ptr(bias),
+                  _lib.ptr(y), _TYPES[x.dtype], P, N, K, st)
+        # one byte per element of x stays for the backward pass
+        ctx.save_for_backward(*((xq, xs) if need_w else (None, None)), *((codes_t, scales) if need_x else (None, None)))
+        ctx.dims = (P, N, K, None if held is not None else weight.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        xq, xs, codes_t, scales = ctx.saved_tensors
+        P, N, K, wtype = ctx.dims
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dy = dy.contiguous()
+        dev, st = dy.device, _s(dy)
+        dx = dw = None
+        dq, ds, db = _quantise_rows(dy, colsum=need_b)
+        if need_x:
+            dx = torch.empty((P, K), dtype=dy.dtype, device=dev)
+            _call("gb_fp8_gemm", dev, _lib.ptr(dq), _lib.ptr(ds), _lib.ptr(codes_t), _lib.ptr(scales), 1, None, _lib.ptr(dx),
+                  _TYPES[dy.dtype], P, K, N, st)
+        if need_w:
+            dw = torch.empty((N, K), dtype=torch.float32, device=dev)
+            ws, size = _fp8_workspace(1, P, N, K, dev)
+            _call("gb_fp8_wgrad", dev, _lib.ptr(dq), _lib.ptr(ds), _lib.ptr(xq), _lib.ptr(xs), _lib.ptr(dw), P, N, K,
+                  _lib.ptr(ws), size, st)
+            dw = dw.to(wtype)
+        return dx, dw, db, None
+
+
+def fp8_linear(x, weight, bias=None):
+    """x weight^T + bias with both operands in 8-bit floats (e4m3) under power-of-two scales: x (..., in_features) has one
+    per 128 elements of a row, weight one per 128 x 128.  weight: (out_features, in_features) - a parameter, or that of a
+    1x1 convolution - quantised in the call, or an Fp8Weight that is kept.  -> (..., out_features) like x; sums in fp32.
+
+    Gradients are those of the products with the quantisers passed straight through: the incoming gradient is quantised
+    like x, dx and dweight are products of the 8-bit operands, dbias sums the gradient as it came.  An element of x or
+    weight that is not finite makes every output it takes part in NaN.  16-bit x runs on the 8-bit matrix instructions
+    (about 14 bits of the largest product kept within a step of 64 or 128), fp32 x on the bf16 ones (exact operands)."""
+    what = "fp8_linear"
+    _rows_tensor(what, "x", x)
+    held = weight if isinstance(weight, Fp8Weight) else None
+    if held is None:
+        weight = _fp8_weight_tensor(what, weight)
+        N, K = weight.shape
+        where = weight.device
+    else:
+        N, K, where = held.out_features, held.in_features, held.codes.device
+    if where != x.device:
+        _refuse(what, "weight must be on the input's device")
+    if x.dim() < 1 or x.shape[-1] != K:
+        _refuse(what, "x must be (..., %d)" % K)
+    bias = _channel_vector(what, "bias", bias, N, x)
+    y = _Fp8Linear.apply(x.reshape(-1, K).contiguous(), None if held is not None else weight, bias, held)
+    return y.view(x.shape[:-1] + (N,))

@@ -747,6 +747,36 @@ int gb_group_norm_fwd(const GbGroupNorm *n, void *y, void *ws, long long ws_byte
 int gb_group_norm_bwd(const GbGroupNorm *n, const void *dy, void *dx, void *dresidual, float *dweight, float *dbias,
                       void *ws, long long ws_bytes, void *stream);
 
+/* Products in 8-bit floats.  A matrix (R, C) is held as e4m3 codes (R, Cp), Cp = C rounded up to 128, rows padded with zeros,
+ * and biased exponents (scale 2^(byte - 127)):
+ *   by rows   (activations, their gradients): one per 128 elements of a row, (R, S), S = Cp / 128 rounded up to 4;
+ *   by blocks (weights): one per 128 x 128 block, (ceil(R / 128), Cp / 128).
+ * The exponent of a block is the least e >= -126 with max|x| <= 448 * 2^e over its finite values (0 for a block of zeros),
+ * its codes are e4m3(x * 2^-e), to nearest, ties to even; infinities and NaN become NaN.  Codes are 16-byte aligned, row
+ * scales 16, block scales any.  P <= 2^40 rows, N, K <= 2^22, else GB_ERANGE.
+ * gb_fp8_quant_rows: x (P, K) -> codes, scales; colsum: NULL, or (K) fp32 = the columns' sums of x (ws: gb_fp8_workspace
+ *   COLSUM with N = K).
+ * gb_fp8_quant_weight: w (N, K) -> codes (N, Kp), block scales, and codes_t (K, Np) = the transposed codes unless NULL.
+ * gb_fp8_gemm: y (P, N) = deq(a) deq(b)^T + bias, a (P, K) by rows, b (N, K) by blocks; transposed != 0: b is the codes_t of a
+ *   weight (K, N) whose scales are given as they are.  fp32 y: codes multiplied as bf16 with fp32 sums (values below 2^-126
+ *   count as zero); 16-bit y: 8-bit matrix instructions, whose steps add 64 or 128 products with about 14 bits below the
+ *   largest before the fp32 sum.
+ * gb_fp8_linear_few: the same from x itself for P <= 16 rows and P * Kp <= 16384 (else GB_ERANGE), in one launch.
+ * gb_fp8_wgrad: dw (N, K) fp32 = deq(dy)^T deq(x), dy (P, N) and x (P, K) by rows (ws: gb_fp8_workspace WGRAD); bf16 products
+ *   with fp32 sums in a fixed order.                                                                                    */
+#define GB_FP8_WS_COLSUM 0
+#define GB_FP8_WS_WGRAD 1
+int gb_fp8_workspace(int what, long long P, int N, int K, long long *bytes);
+int gb_fp8_quant_rows(const void *x, int dtype, long long P, int K, void *codes, void *scales, float *colsum, void *ws,
+                      long long ws_bytes, void *stream);
+int gb_fp8_quant_weight(const void *w, int dtype, int N, int K, void *codes, void *codes_t, void *scales, void *stream);
+int gb_fp8_gemm(const void *a, const void *a_scales, const void *b, const void *b_scales, int transposed, const float *bias,
+                void *y, int dtype, long long P, int N, int K, void *stream);
+int gb_fp8_linear_few(const void *x, const void *b, const void *b_scales, const float *bias, void *y, int dtype, int P, int N,
+                      int K, void *stream);
+int gb_fp8_wgrad(const void *dy, const void *dy_scales, const void *x, const void *x_scales, float *dw, long long P, int N, int K,
+                 void *ws, long long ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

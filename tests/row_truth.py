@@ -92,3 +92,18 @@ def group_norm(x, groups, weight, bias, eps, name, slope, residual, cuts, factor
         ab += g.abs().sum(0)
     out.update(dw=dw, db=db, aw=aw, ab=ab)
     return out
+
+
+def in_8_bits(x, block_rows):
+    """x (double) rounded to e4m3 under one power of two per block of block_rows x 128: the values."""
+    rows, cols = x.shape
+    out = torch.zeros(-(-rows // block_rows) * block_rows, -(-cols // 128) * 128, dtype=torch.float64)
+    out[:rows, :cols] = x
+    b = out.view(-1, block_rows, out.shape[1] // 128, 128)
+    top = b.abs().amax((1, 3), keepdim=True).numpy()
+    m, e = np.frexp(top)                                   # top = m 2^e, 0.5 <= m < 1; 448 = 0.875 * 2^9
+    e = np.maximum(np.where(m <= 0.875, e - 9, e - 8), -126)
+    scale = torch.from_numpy(np.where(top == 0, 1.0, np.ldexp(1.0, e)))
+    v = (b / scale).numpy()
+    place = np.ldexp(1.0, np.maximum(np.frexp(v)[1] - 1, -6) - 3)      # the last of four significant bits, >= 2^-9
+    return (torch.from_numpy(np.rint(v / place) * place) * scale).reshape(out.shape)[:rows, :cols].clone()

@@ -91,3 +91,60 @@ def test_dropout_refuses_on_the_host():
         args[at] = bad
         assert L.gb_dropout(*args) == -1, (at, bad)
     assert L.gb_dropout(None, None, None, 0, 0, 100, None, 1, 2, None, None) == 0
+
+
+def test_fp8_cpu_tensors_raise():
+    from graspbalance_amd import fused_rows
+    with pytest.raises(RuntimeError, match="CPU not supported"):
+        fused_rows.fp8_linear(torch.randn(4, 16), torch.randn(8, 16))
+    with pytest.raises(RuntimeError, match="CPU not supported"):
+        fused_rows.Fp8Weight.quantize(torch.randn(8, 16))
+
+
+def test_fp8_refuses_on_the_host():
+    from graspbalance_amd import _lib
+    L = _lib.lib()
+    size = ctypes.c_longlong(-5)
+
+    def refused(fn, ok, bad):
+        for at, value, rc in bad:
+            args = list(ok)
+            args[at] = value
+            assert fn(*args) == rc, (fn.__name__, at, value)
+    refused(L.gb_fp8_workspace, [1, 8, 8, 8, ctypes.byref(size)],
+            [(0, 2, -1), (0, -1, -1), (1, -1, -1), (2, 0, -1), (3, 0, -1), (4, None, -1), (1, 1 << 41, -3), (2, 1 << 23, -3)])
+    assert size.value == -5
+    refused(L.gb_fp8_quant_rows, [64, 0, 8, 8, 64, 64, None, None, 0, None],
+            [(0, None, -1), (1, 3, -1), (2, -1, -1), (3, 0, -1), (4, None, -1), (4, 72, -1), (5, None, -1), (5, 68, -1),
+             (3, 1 << 23, -3), (2, 1 << 41, -3), (6, 64, -1)])
+    refused(L.gb_fp8_quant_weight, [64, 0, 8, 8, 64, 64, 64, None],
+            [(0, None, -1), (1, 9, -1), (2, 0, -1), (3, -2, -1), (4, None, -1), (4, 65, -1), (5, 72, -1), (6, None, -1),
+             (2, 1 << 23, -3)])
+    refused(L.gb_fp8_gemm, [64, 64, 64, 64, 0, None, 64, 0, 8, 8, 8, None],
+            [(0, None, -1), (0, 72, -1), (1, None, -1), (1, 72, -1), (2, None, -1), (2, 72, -1), (3, None, -1), (6, None, -1),
+             (7, 5, -1), (8, -1, -1), (9, 0, -1), (10, 0, -1), (9, 1 << 23, -3), (10, 1 << 23, -3), (8, 1 << 41, -3)])
+    refused(L.gb_fp8_linear_few, [64, 64, 64, None, 64, 0, 8, 8, 8, None],
+            [(0, None, -1), (1, None, -1), (1, 72, -1), (2, None, -1), (4, None, -1), (5, 7, -1), (6, -1, -1), (7, 0, -1),
+             (8, 0, -1), (6, 17, -3), (8, 2049, -3)])
+    refused(L.gb_fp8_wgrad, [64, 64, 64, 64, 64, 8, 8, 8, None, 0, None],
+            [(0, None, -1), (0, 72, -1), (1, None, -1), (2, None, -1), (2, 72, -1), (3, None, -1), (4, None, -1), (5, -1, -1),
+             (6, 0, -1), (7, 0, -1), (7, 1 << 23, -3), (5, 100000, -1)])
+    assert L.gb_fp8_gemm(None, None, None, None, 0, None, None, 0, 0, 8, 8, None) == 0
+    assert L.gb_fp8_workspace(0, 100, 30, 1, ctypes.byref(size)) == 0 and size.value == 2 * 30 * 4
+
+
+def test_the_oracle_of_8_bits_agrees_with_torchs_cast():
+    """Codes of the oracle against torch's own float8_e4m3fn on values inside its range."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(64, 256, generator=g) * torch.exp(3 * torch.randn(64, 256, generator=g))
+    got = row_truth.in_8_bits(x.double(), 1)
+    blocks = x.view(64, 2, 128)
+    scale = got.new_ones(64, 2, 1)
+    for i in range(64):
+        for j in range(2):
+            e = -126
+            while blocks[i, j].abs().max().item() > 448 * 2.0 ** e:
+                e += 1
+            scale[i, j] = 2.0 ** e
+    want = (blocks / scale.float()).to(torch.float8_e4m3fn).double() * scale
+    assert torch.equal(got, want.view(64, 256))
