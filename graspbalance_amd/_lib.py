@@ -123,8 +123,7 @@ SIGNATURES = {
     "gb_fp8_workspace": [_I, _L, _I, _I, _P],
     "gb_fp8_quant_rows": [_P, _I, _L, _I, _P, _P, _P, _P, _L, _P],
     "gb_fp8_quant_weight": [_P, _I, _I, _I, _P, _P, _P, _P],
-    "gb_fp8_gemm": [_P, _P, _P, _P, _I, _P, _P, _I, _L, _I, _I, _P],
-    "gb_fp8_linear_few": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
+    "gb_fp8_linear": [_P, _I, _L, _I, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _L, _P],
     "gb_fp8_wgrad": [_P, _P, _P, _P, _P, _L, _I, _I, _P, _L, _P],
 }
 

@@ -20,6 +20,24 @@
 
 namespace gb {
 
+// the quantisers' eight elements per lane (sixteen lanes = a block of 128)
+typedef Vec<8> F8;
+template <typename T>
+__device__ __forceinline__ F8 load_upto8(const T *p, int n) {   // n <= 0: nothing is read
+  F8 f = {};
+  if (n >= 8) {
+    T v[8];
+    __builtin_memcpy(v, p, sizeof(v));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f.v[k] = (float)v[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < n) f.v[k] = (float)p[k];
+  }
+  return f;
+}
+
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -28,6 +46,8 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 
 static constexpr int FP8_FEW_ROWS = 64;          // rows up to which the products run without LDS tiles
+static constexpr long long FP8_STREAM_ROWS = 32768;   // 512 tiles: below, the two-launch way is as fast (8192 x 128 -> 512 fp32:
+                                                      // 15.4 us in two launches, 18.1 streamed; 524288 x 256 -> 128 bf16: 212, 120)
 static constexpr int FP8_FUSED_CODES = 16384;    // bytes of codes a workgroup quantises for itself
 static constexpr int FP8_FUSED_ROWS = 16;
 
@@ -66,12 +86,6 @@ __device__ __forceinline__ uint2 encode8(const F8 &f, int biased) {
   r.y = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], hi, true);
   return r;
 }
-template <typename T>
-__device__ __forceinline__ F8 load_upto8(const T *p, int n) {
-  if (n >= 8) return load8(p);
-  return load_tail(p, n);   // (n <= 0: nothing is read)
-}
-
 // Rows [r0, r0 + per) x block kb of 128 columns: sixteen lanes x eight elements a row.  SUM: also the column sums of these
 // rows, fp32 over per / 16 rows a lane, to part[chunk][K].
 template <typename T, bool SUM>
@@ -178,6 +192,94 @@ struct Exact {  // fp32 outputs take the bf16 products
   static constexpr bool value = sizeof(T) == 4;
 };
 
+// 64 codes of the reduction into TM x TN tiles: fa, fb are a lane's 32 codes of its rows, sa, sb their biased exponents
+template <bool EXACT, int TM, int TN>
+__device__ __forceinline__ void multiply64(f32x16 (&acc)[TM][TN], const i32x4 (&fa)[TM][2], const i32x4 (&fb)[TN][2], const int (&sa)[TM],
+                                           int sb) {
+  if (EXACT) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      bf16x8 db[TN];
+#pragma unroll
+      for (int n = 0; n < TN; ++n)
+        db[n] = decode8((unsigned)fb[n][q / 2][q % 2 * 2], (unsigned)fb[n][q / 2][q % 2 * 2 + 1], power_of(sb));
+#pragma unroll
+      for (int m = 0; m < TM; ++m) {
+        const bf16x8 da = decode8((unsigned)fa[m][q / 2][q % 2 * 2], (unsigned)fa[m][q / 2][q % 2 * 2 + 1], power_of(sa[m]));
+#pragma unroll
+        for (int n = 0; n < TN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(da, db[n], acc[m][n], 0, 0, 0);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int m = 0; m < TM; ++m) {
+      const i32x8 va = __builtin_shufflevector(fa[m][0], fa[m][1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int n = 0; n < TN; ++n) {
+        const i32x8 vb = __builtin_shufflevector(fb[n][0], fb[n][1], 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va, vb, acc[m][n], 0, 0, 0, sa[m], 0, sb);
+      }
+    }
+  }
+}
+
+// A wave's results to memory: lane j of a pair of tiles has columns 2 j, 2 j + 1 of 64 (from col0 of N) and, of every eight
+// rows, 4 h .. 4 h + 3.  Eight rows at a time go through the wave's own LDS cell and leave as 16 bytes per lane, whole
+// 128-byte lines: stored from where they are (4 bytes a lane) they took 75 of the 120 us of 524288 x 128 -> 256 bf16.
+// `rows` of the tile exist.  (A tile's offsets fit 32 unsigned bits: 256 rows of 2^22 fp32.)
+template <typename T>
+struct Cell {
+  static constexpr int ROW = 64 * (int)sizeof(T) + 16, BYTES = 8 * ROW;
+};
+template <typename T, int TM, int TN, bool NT>
+__device__ __forceinline__ void store_tiles(const f32x16 (&acc)[TM][TN], T *y, const float *bias, int N, int col0, int row0, int lane, int rows,
+                                            unsigned char *cell) {
+  constexpr int ROW = Cell<T>::ROW, E = 16 / (int)sizeof(T), CH = 64 / E;   // elements of an access, accesses of a row
+  const int j = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int n = 0; n < TN; n += 2) {
+    const int base = col0 + 32 * n, col = base + 2 * j;
+    if (base >= N) break;
+    const float b0 = bias && col < N ? bias[col] : 0.0f, b1 = bias && col + 1 < N ? bias[col + 1] : 0.0f;
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const T v[2] = {(T)(acc[m][n][4 * q + i] + b0), (T)(acc[m][n + 1][4 * q + i] + b1)};
+          __builtin_memcpy(cell + (4 * h + i) * ROW + 2 * j * (int)sizeof(T), v, sizeof(v));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int t = 0; t < 8 * CH / 64; ++t) {
+          const int at = t * 64 + lane, r = at / CH, c = base + at % CH * E, row = row0 + 32 * m + 8 * q + r;
+          typedef unsigned u4 __attribute__((ext_vector_type(4)));
+          const u4 w = *reinterpret_cast<const u4 *>(cell + r * ROW + at % CH * 16);
+          if (row >= rows || c >= N) continue;
+          T *to = reinterpret_cast<T *>(reinterpret_cast<unsigned char *>(y) + ((unsigned)row * (unsigned)N + (unsigned)c) * (unsigned)sizeof(T));
+          if (c + E <= N) {
+            if (NT)
+              __builtin_nontemporal_store((u32x4_any)w, reinterpret_cast<u32x4_any *>(to));
+            else
+              __builtin_memcpy(to, &w, 16);
+          } else {
+            T v[E];
+            __builtin_memcpy(v, &w, 16);
+#pragma unroll
+            for (int k = 0; k < E; ++k)
+              if (c + k < N) to[k] = v[k];
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      }
+  }
+}
+
 // ---- tiles ----------------------------------------------------------------------------------------------------------
 // A workgroup of WM x WN waves, each with TM x TN tiles of 32 x 32, steps through the reduction 128 codes (one scale block)
 // at a time: two LDS stages filled by LDS-DMA, the next one in flight while this one is multiplied.  An LDS row is 128
@@ -200,12 +302,12 @@ __device__ __forceinline__ void dma16(const unsigned char *src, unsigned char *l
                                    16, 0, 0);
 }
 
-template <typename T, int TM, int TN, int WM, int WN>
+template <typename T, int TM, int TN, int WM, int WN, bool NT>
 __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(GemmArgs8 g) {
   constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, WAVES = WM * WN, ROWS = BM + BN, LOADS = ROWS / (8 * WAVES);
   constexpr bool EXACT = Exact<T>::value;
   static_assert(TN % 2 == 0 && ROWS % (8 * WAVES) == 0 && (32 * TN) <= 128, "tile");
-  __shared__ __attribute__((aligned(128))) unsigned char lds[2][ROWS * 128];
+  extern __shared__ __attribute__((aligned(128))) unsigned char stages[];   // one, or two where there is a second step
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave / WN, wn = wave % WN, j = lane & 31, h = lane >> 5;
   // neighbouring tiles on one XCD (workgroups go to the eight XCDs in turn): its L2 then holds their common rows
   const long long per = g.tiles >> 3, extra = g.tiles & 7, x = blockIdx.x & 7;
@@ -238,7 +340,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(GemmArgs8 g) {
 #pragma unroll
     for (int n = 0; n < TN; ++n) acc[m][n] = f32x16{};
   const unsigned char *as[TM];
-  unsigned sa[TM];
+  unsigned sa[TM], sa_next[TM];
 #pragma unroll
   for (int m = 0; m < TM; ++m) {
     const int r = wm * 32 * TM + 32 * m + j;
@@ -247,16 +349,28 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(GemmArgs8 g) {
   const int nb = (n0 + wn * 32 * TN) / 128, nbs = nb < (g.N + 127) / 128 ? nb : (g.N + 127) / 128 - 1;
   const unsigned char *bs = g.b_scales + (long long)nbs * g.bs_n;
 
-  request(0, lds[0]);
-  for (int kb = 0; kb < g.Kb; ++kb) {
-    if ((kb & 3) == 0)
+  request(0, stages);
 #pragma unroll
-      for (int m = 0; m < TM; ++m) sa[m] = *reinterpret_cast<const unsigned *>(as[m] + kb);
-    const unsigned sb = bs[(long long)kb * g.bs_k];
+  for (int m = 0; m < TM; ++m) sa_next[m] = *reinterpret_cast<const unsigned *>(as[m]);
+  unsigned sb_next = bs[0];
+  for (int kb = 0; kb < g.Kb; ++kb) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();   // this stage is complete, and nobody reads the other one any more
-    if (kb + 1 < g.Kb) request(kb + 1, lds[(kb + 1) & 1]);
-    const unsigned char *st = lds[kb & 1];
+    const unsigned sb = sb_next;
+    if ((kb & 3) == 0)
+#pragma unroll
+      for (int m = 0; m < TM; ++m) sa[m] = sa_next[m];
+    if (kb + 1 < g.Kb) {   // the next step's codes and exponents travel while this one is multiplied
+      request(kb + 1, stages + ((kb + 1) & 1) * (ROWS * 128));
+      sb_next = bs[(long long)(kb + 1) * g.bs_k];
+      if ((kb & 3) == 3)
+#pragma unroll
+        for (int m = 0; m < TM; ++m) sa_next[m] = *reinterpret_cast<const unsigned *>(as[m] + kb + 1);
+    }
+    const unsigned char *st = stages + (kb & 1) * (ROWS * 128);
+    int s8[TM];
+#pragma unroll
+    for (int m = 0; m < TM; ++m) s8[m] = (int)(sa[m] >> (8 * (kb & 3)) & 0xff);
     const unsigned char *la = st + (wm * 32 * TM + j) * 128, *lb = st + (BM + wn * 32 * TN + 2 * j) * 128;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {   // 64 codes: lane half h holds 32 of them
@@ -274,65 +388,188 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(GemmArgs8 g) {
         fa[m][0] = *reinterpret_cast<const i32x4 *>(r + c0);
         fa[m][1] = *reinterpret_cast<const i32x4 *>(r + c1);
       }
-      if (EXACT) {
+      multiply64<EXACT, TM, TN>(acc, fa, fb, s8, (int)sb);
+    }
+  }
+  __syncthreads();   // (the stages become the waves' cells)
+  store_tiles<T, TM, TN, NT>(acc, (T *)g.y + p0 * g.N, g.bias, g.N, n0 + wn * 32 * TN, wm * 32 * TM, lane, last_a + 1,
+                             stages + wave * Cell<T>::BYTES);
+}
+
+// ---- streamed rows --------------------------------------------------------------------------------------------------
+// Many rows and a weight that fits LDS (64 KB: 512 x 128, 128 x 512, ...): bound by reading X and writing Y.  A workgroup
+// keeps the weight and walks over tiles of 64 rows, 128 columns of X at a step: the next step's rows travel in registers
+// while this one is multiplied, are quantised into the other LDS buffer, and go to memory as codes only where the backward
+// pass wants them.  Against a quantising kernel and the tiles above: X's codes are not read back and there is one launch
+// (524288 x 128 -> 256 bf16: 123 us in two launches).  SUM: also the column sums of X, one LDS cell per lane.
+struct StreamArgs8 {
+  const void *x;
+  const unsigned char *w, *w_scales;
+  const float *bias;
+  void *y;
+  unsigned char *codes, *scales;
+  float *part;         // (workgroups, K)
+  long long P, tiles;
+  int N, K, bs_n, bs_k;
+};
+template <typename T>
+struct Eight {
+  T v[8];
+};
+
+template <typename T, int TM, int TN, int WM, int WN, bool SUM, bool NT>
+__global__ __launch_bounds__(256, 2) void fp8_stream_kernel(StreamArgs8 g) {
+  constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, SLOTS = BM / 16;
+  constexpr bool EXACT = Exact<T>::value;
+  static_assert(WM * WN == 4 && BM == 64 && TN % 2 == 0 && 32 * TN <= 128, "tile");
+  extern __shared__ __attribute__((aligned(128))) unsigned char smem[];
+  const int Kb = blocks128(g.K), Kp = Kb * 128, ss = scale_stride(g.K);
+  unsigned char *ws = smem, *xs = ws + Kb * BN * 128, *es = xs + 2 * BM * 128;
+  float *sums = reinterpret_cast<float *>(es + 2 * BM + 4 * Cell<T>::BYTES);   // SUM: [16][Kp]
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave / WN, wn = wave % WN, j = lane & 31, h = lane >> 5;
+  const int cl = (int)threadIdx.x & 15, rl = (int)threadIdx.x >> 4;
+  const T *x = (const T *)g.x;
+
+  for (int i = wave * 8; i < Kb * BN; i += 32) {   // the weight: eight rows of 128 codes per access (see above for the order)
+    const int kb = i / BN, r = i - kb * BN + (lane >> 3), n = r < g.N ? r : g.N - 1;
+    dma16(g.w + (long long)n * Kp + kb * 128 + ((lane & 7) ^ (r >> 1 & 7)) * 16, ws + i * 128);
+  }
+  if (SUM)
+    for (int i = 0; i < Kp / 128; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          bf16x8 db[TN];
+      for (int k = 0; k < 8; ++k) sums[rl * Kp + i * 128 + cl * 8 + k] = 0;
+
+  Eight<T> raw[SLOTS];
+  auto fetch = [&](long long tile, int kb) {
+    const int col = kb * 128 + cl * 8, n = g.K - col, rows = (int)(g.P - tile * BM < BM ? g.P - tile * BM : BM);
+    const T *base = x + tile * BM * g.K;
 #pragma unroll
-          for (int n = 0; n < TN; ++n)
-            db[n] = decode8((unsigned)fb[n][q / 2][q % 2 * 2], (unsigned)fb[n][q / 2][q % 2 * 2 + 1], power_of((int)sb));
+    for (int s = 0; s < SLOTS; ++s) {
+      const T *p = base + (unsigned)((s * 16 + rl) * g.K + col);
 #pragma unroll
-          for (int m = 0; m < TM; ++m) {
-            const bf16x8 da = decode8((unsigned)fa[m][q / 2][q % 2 * 2], (unsigned)fa[m][q / 2][q % 2 * 2 + 1],
-                                      power_of((int)(sa[m] >> (8 * (kb & 3)) & 0xff)));
+      for (int k = 0; k < 8; ++k) raw[s].v[k] = (T)0.0f;
+      if (s * 16 + rl < rows) {
+        if (n >= 8) {
+          if (NT) {
+            typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(1)));
+            u4 v[sizeof(raw[s]) / 16];
 #pragma unroll
-            for (int n = 0; n < TN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(da, db[n], acc[m][n], 0, 0, 0);
+            for (int i = 0; i < (int)(sizeof(raw[s]) / 16); ++i) v[i] = __builtin_nontemporal_load(reinterpret_cast<const u4 *>(p) + i);
+            __builtin_memcpy(&raw[s], v, sizeof(raw[s]));
+          } else {
+            __builtin_memcpy(&raw[s], p, sizeof(raw[s]));
           }
-        }
-      } else {
+        } else {
 #pragma unroll
-        for (int m = 0; m < TM; ++m) {
-          const i32x8 va = __builtin_shufflevector(fa[m][0], fa[m][1], 0, 1, 2, 3, 4, 5, 6, 7);
-          const int s8 = (int)(sa[m] >> (8 * (kb & 3)) & 0xff);
-#pragma unroll
-          for (int n = 0; n < TN; ++n) {
-            const i32x8 vb = __builtin_shufflevector(fb[n][0], fb[n][1], 0, 1, 2, 3, 4, 5, 6, 7);
-            acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va, vb, acc[m][n], 0, 0, 0, s8, 0, (int)sb);
-          }
+          for (int k = 0; k < 8; ++k)
+            if (k < n) raw[s].v[k] = p[k];
         }
       }
     }
-  }
-
-  T *y = (T *)g.y + p0 * g.N;
+  };
+  auto put = [&](long long tile, int kb, int buf) {
+    F8 sum = {};
+    const int rows = (int)(g.P - tile * BM < BM ? g.P - tile * BM : BM);
+    unsigned char *codes = g.codes + tile * BM * Kp + kb * 128, *scales = g.scales + tile * BM * ss + kb;
 #pragma unroll
-  for (int n = 0; n < TN; n += 2) {
-    const int col = n0 + wn * 32 * TN + 32 * n + 2 * j;
-    const bool two = col + 1 < g.N;
-    if (col >= g.N) continue;
-    const float b0 = g.bias ? g.bias[col] : 0.0f, b1 = g.bias && two ? g.bias[col + 1] : 0.0f;
+    for (int s = 0; s < SLOTS; ++s) {
+      F8 f;
 #pragma unroll
-    for (int m = 0; m < TM; ++m)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int r = wm * 32 * TM + 32 * m + i / 4 * 8 + h * 4 + i % 4;
-        if (r > last_a) continue;
-        const T v[2] = {(T)(acc[m][n][i] + b0), (T)(acc[m][n + 1][i] + b1)};
-        T *to = y + (long long)r * g.N + col;
-        if (two)
-          __builtin_memcpy(to, v, sizeof(v));
-        else
-          *to = v[0];
+      for (int k = 0; k < 8; ++k) f.v[k] = (float)raw[s].v[k];
+      const int row = s * 16 + rl, e = block_exponent(row_max_f32(top8(f)));
+      const uint2 c = encode8(f, e);
+      *reinterpret_cast<uint2 *>(xs + (buf * BM + row) * 128 + ((cl >> 1) ^ (row & 7)) * 16 + (cl & 1) * 8) = c;
+      if (cl == 0) es[buf * BM + row] = (unsigned char)e;
+      if (g.codes && row < rows) {
+        *reinterpret_cast<uint2 *>(codes + (unsigned)(row * Kp + cl * 8)) = c;
+        if (cl == 0) scales[(unsigned)(row * ss)] = (unsigned char)e;
       }
+      if (SUM)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum.v[k] += f.v[k];
+    }
+    if (SUM)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sums[rl * Kp + kb * 128 + cl * 8 + k] += sum.v[k];
+  };
+
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int m = 0; m < TM; ++m)
+#pragma unroll
+    for (int n = 0; n < TN; ++n) acc[m][n] = f32x16{};
+  const int nb = wn * 32 * TN / 128, last_nb = (g.N - 1) / 128;
+  const unsigned char *bs = g.w_scales + (long long)(nb < last_nb ? nb : last_nb) * g.bs_n;
+
+  long long tile = blockIdx.x;
+  int kb = 0, buf = 0;
+  if (tile < g.tiles) {
+    fetch(tile, 0);
+    put(tile, 0, 0);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  while (tile < g.tiles) {
+    const bool last = kb + 1 == Kb;
+    const long long next = last ? tile + gridDim.x : tile;
+    const int next_kb = last ? 0 : kb + 1;
+    if (next < g.tiles) fetch(next, next_kb);
+    const unsigned char *la = xs + (buf * BM + wm * 32 * TM + j) * 128, *lb = ws + (kb * BN + wn * 32 * TN + 2 * j) * 128;
+    const int sb = bs[(long long)kb * g.bs_k];
+    int sa[TM];
+#pragma unroll
+    for (int m = 0; m < TM; ++m) sa[m] = es[buf * BM + wm * 32 * TM + 32 * m + j];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int c0 = ((4 * s + 2 * h) ^ (j & 7)) * 16, c1 = ((4 * s + 2 * h + 1) ^ (j & 7)) * 16;
+      i32x4 fa[TM][2], fb[TN][2];
+#pragma unroll
+      for (int n = 0; n < TN; ++n) {
+        const unsigned char *r = lb + (n / 2 * 64 + n % 2) * 128;
+        fb[n][0] = *reinterpret_cast<const i32x4 *>(r + c0);
+        fb[n][1] = *reinterpret_cast<const i32x4 *>(r + c1);
+      }
+#pragma unroll
+      for (int m = 0; m < TM; ++m) {
+        const unsigned char *r = la + 32 * m * 128;
+        fa[m][0] = *reinterpret_cast<const i32x4 *>(r + c0);
+        fa[m][1] = *reinterpret_cast<const i32x4 *>(r + c1);
+      }
+      multiply64<EXACT, TM, TN>(acc, fa, fb, sa, sb);
+    }
+    if (last) {
+      T *y = (T *)g.y + tile * BM * g.N;
+      const int rows = (int)(g.P - tile * BM < BM ? g.P - tile * BM : BM);
+      int ll = lane;   // (opaque: the offsets of the stores are the same for every tile and would live in registers)
+      asm volatile("" : "+v"(ll));
+      store_tiles<T, TM, TN, NT>(acc, y, g.bias, g.N, wn * 32 * TN, wm * 32 * TM, ll, rows, es + 2 * BM + wave * Cell<T>::BYTES);
+#pragma unroll
+      for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int n = 0; n < TN; ++n) acc[m][n] = f32x16{};
+    }
+    if (next < g.tiles) put(next, next_kb, buf ^ 1);
+    __syncthreads();
+    tile = next;
+    kb = next_kb;
+    buf ^= 1;
+  }
+  if (SUM)
+    for (int c = (int)threadIdx.x; c < g.K; c += 256) {
+      float s = 0;
+      for (int i = 0; i < 16; ++i) s += sums[i * Kp + c];
+      g.part[(long long)blockIdx.x * g.K + c] = s;
+    }
 }
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
 // Up to 64 rows: bound by reading W once.  A workgroup takes 16 outputs; its waves take the blocks of 128 in turn, a lane
 // reads 32 codes of W straight into the operand of a 16-row step (the four lanes of a row read one 128-byte line), and the
-// waves' sums meet in LDS.  FUSED: every workgroup quantises the few rows of X for itself (one launch instead of two).
+// waves' sums meet in LDS.  FUSED: every workgroup quantises the few rows of X for itself (one launch instead of two); the
+// first one stores the codes where somebody wants them.
 template <typename T, int PT, bool FUSED>
-__global__ __launch_bounds__(256) void fp8_few_kernel(GemmArgs8 g, const T *__restrict__ x, int K) {
+__global__ __launch_bounds__(256) void fp8_few_kernel(GemmArgs8 g, const T *__restrict__ x, int K, unsigned char *__restrict__ codes_out,
+                                                      unsigned char *__restrict__ scales_out) {
   constexpr bool EXACT = Exact<T>::value;
   __shared__ float sums[4][PT][64][4];
   extern __shared__ __attribute__((aligned(16))) unsigned char codes[];   // FUSED: P x Kp codes, P x Kb exponents
@@ -345,8 +582,13 @@ __global__ __launch_bounds__(256) void fp8_few_kernel(GemmArgs8 g, const T *__re
       const int r = i / g.Kb, kb = i - r * g.Kb, col = kb * 128 + cl * 8;
       const F8 f = load_upto8(x + (long long)r * K + col, K - col);
       const int e = block_exponent(row_max_f32(top8(f)));
-      *reinterpret_cast<uint2 *>(codes + r * Kp + col) = encode8(f, e);
+      const uint2 c = encode8(f, e);
+      *reinterpret_cast<uint2 *>(codes + r * Kp + col) = c;
       if (cl == 0) codes[P * Kp + r * g.Kb + kb] = (unsigned char)e;
+      if (codes_out && blockIdx.x == 0) {
+        *reinterpret_cast<uint2 *>(codes_out + r * Kp + col) = c;
+        if (cl == 0) scales_out[r * scale_stride(K) + kb] = (unsigned char)e;
+      }
     }
     __syncthreads();
   }
@@ -442,29 +684,35 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_wgrad_kernel(WgradArgs8 g) {
     const int col = of_a ? n0 + cc * 16 : k0 + (cc - CA) * 16, width = of_a ? Np : Kp;
     in[i] = col < width;
     const int at = in[i] ? col : 0;
-    src[i] = (of_a ? g.dy : g.x) + at;
-    scl[i] = (of_a ? g.dys : g.xs) + at / 128;
     ld[i] = width;
     sld[i] = of_a ? sn : sk;
+    src[i] = (of_a ? g.dy : g.x) + (p0 + row[i]) * width + at;
+    scl[i] = (of_a ? g.dys : g.xs) + (p0 + row[i]) * sld[i] + at / 128;
     to[i] = of_a ? row[i] * SA + cc * 32 : STEP * SA + row[i] * SB + (cc - CA) * 32;
   }
-  uint4 code[LOADS];
-  unsigned scale[LOADS];
-  auto fetch = [&](long long p) {
+  struct Codes {
+    uint4 code[LOADS];
+    unsigned scale[LOADS];
+  };
+  auto fetch = [&](long long p, Codes &f) {   // (called for p0, p0 + STEP, ... in turn)
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const long long r = p + row[i], at = r < p1 ? r : p1 - 1;
-      code[i] = *reinterpret_cast<const uint4 *>(src[i] + at * ld[i]);
-      scale[i] = scl[i][at * sld[i]];
-      if (!in[i] || r >= p1) code[i] = make_uint4(0, 0, 0, 0);
+      f.code[i] = make_uint4(0, 0, 0, 0);
+      f.scale[i] = 127;
+      if (in[i] && p + row[i] < p1) {
+        f.code[i] = *reinterpret_cast<const uint4 *>(src[i]);
+        f.scale[i] = *scl[i];
+      }
+      src[i] += (long long)STEP * ld[i];
+      scl[i] += STEP * sld[i];
     }
   };
-  auto put = [&](unsigned char *stage) {
+  auto put = [&](unsigned char *stage, const Codes &f) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const float s = power_of((int)scale[i]);
-      *reinterpret_cast<bf16x8 *>(stage + to[i]) = decode8(code[i].x, code[i].y, s);
-      *reinterpret_cast<bf16x8 *>(stage + to[i] + 16) = decode8(code[i].z, code[i].w, s);
+      const float s = power_of((int)f.scale[i]);
+      *reinterpret_cast<bf16x8 *>(stage + to[i]) = decode8(f.code[i].x, f.code[i].y, s);
+      *reinterpret_cast<bf16x8 *>(stage + to[i] + 16) = decode8(f.code[i].z, f.code[i].w, s);
     }
   };
 
@@ -475,36 +723,47 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_wgrad_kernel(WgradArgs8 g) {
     for (int n = 0; n < TN; ++n) acc[m][n] = f32x16{};
   const int sub = lane & 15, right = (lane >> 4 & 1) * 16 + (sub & 3) * 4, down = (lane >> 5) * 8 + (sub >> 2);
   const int fa = down * SA + (wm * 32 * TM + right) * 2, fb = STEP * SA + down * SB + (wn * 32 * TN + right) * 2;
-  if (p0 < p1) {
-    fetch(p0);
-    put(lds[0]);
-    __syncthreads();
-    int cur = 0;
-    for (long long p = p0; p < p1; p += STEP, cur ^= 1) {
-      const bool more = p + STEP < p1;
-      if (more) fetch(p + STEP);
-      unsigned char *st = lds[cur];
+  auto multiply = [&](unsigned char *st) {
 #pragma unroll
-      for (int s = 0; s < STEP / 16; ++s) {
-        bf16x8 a[TM], b[TN];
+    for (int s = 0; s < STEP / 16; ++s) {
+      bf16x8 a[TM], b[TN];
 #pragma unroll
-        for (int m = 0; m < TM; ++m) {
-          unsigned char *at = st + fa + s * 16 * SA + m * 64;
-          a[m] = __builtin_shufflevector(__builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(at)),
-                                         __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(at + 4 * SA)), 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-#pragma unroll
-        for (int n = 0; n < TN; ++n) {
-          unsigned char *at = st + fb + s * 16 * SB + n * 64;
-          b[n] = __builtin_shufflevector(__builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(at)),
-                                         __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(at + 4 * SB)), 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-#pragma unroll
-        for (int m = 0; m < TM; ++m)
-#pragma unroll
-          for (int n = 0; n < TN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[m], b[n], acc[m][n], 0, 0, 0);
+      for (int m = 0; m < TM; ++m) {
+        unsigned char *at = st + fa + s * 16 * SA + m * 64;
+        a[m] = __builtin_shufflevector(__builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(at)),
+                                       __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(at + 4 * SA)), 0, 1, 2, 3, 4, 5, 6, 7);
       }
-      if (more) put(lds[cur ^ 1]);
+#pragma unroll
+      for (int n = 0; n < TN; ++n) {
+        unsigned char *at = st + fb + s * 16 * SB + n * 64;
+        b[n] = __builtin_shufflevector(__builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(at)),
+                                       __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(at + 4 * SB)), 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+#pragma unroll
+      for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int n = 0; n < TN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[m], b[n], acc[m][n], 0, 0, 0);
+    }
+  };
+  // A step's codes are requested two steps before they are needed: one step multiplies for ~1000 cycles, less than the
+  // memory takes to answer.  Behind the range there are zeros.
+  if (p0 < p1) {
+    Codes even, odd;
+    fetch(p0, even);
+    put(lds[0], even);
+    fetch(p0 + STEP, odd);
+    fetch(p0 + 2 * STEP, even);
+    __syncthreads();
+    for (long long p = p0; p < p1; p += 2 * STEP) {
+      multiply(lds[0]);
+      __builtin_amdgcn_sched_barrier(0);
+      put(lds[1], odd);
+      fetch(p + 3 * STEP, odd);
+      __syncthreads();
+      multiply(lds[1]);   // (zeros where the range ends with an odd step)
+      __builtin_amdgcn_sched_barrier(0);
+      put(lds[0], even);
+      fetch(p + 4 * STEP, even);
       __syncthreads();
     }
   }
@@ -524,33 +783,106 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_wgrad_kernel(WgradArgs8 g) {
     }
 }
 
-// out[i] = the splits' sums added in order: 64 elements x 4 lanes over the splits
+// out[i] = the splits' sums added in order: 32 elements x 8 lanes over the splits
 __global__ __launch_bounds__(256) void fp8_wgrad_join_kernel(const float *__restrict__ part, int splits, long long n,
                                                              float *__restrict__ out) {
-  __shared__ float lds[4][64];
-  const int i = (int)threadIdx.x & 63, q = (int)threadIdx.x >> 6;
-  const long long e = (long long)blockIdx.x * 64 + i;
+  __shared__ float lds[8][32];
+  const int i = (int)threadIdx.x & 31, q = (int)threadIdx.x >> 5;
+  const long long e = (long long)blockIdx.x * 32 + i;
   float s = 0;
   if (e < n)
-    for (int k = q; k < splits; k += 4) s += part[(long long)k * n + e];
+#pragma unroll 8
+    for (int k = q; k < splits; k += 8) s += part[(long long)k * n + e];
   lds[q][i] = s;
   __syncthreads();
-  if (q == 0 && e < n) out[e] = (lds[0][i] + lds[1][i]) + (lds[2][i] + lds[3][i]);
+  if (q == 0 && e < n) {
+    for (int j = 1; j < 8; ++j) s += lds[j][i];
+    out[e] = s;
+  }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
 
-template <typename T, int TM, int TN, int WM, int WN>
-static int launch_tiles(GemmArgs8 g, hipStream_t st) {
-  constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
+template <typename T, int TM, int TN, int WM, int WN, bool NT>
+static int launch_tiles_nt(GemmArgs8 g, hipStream_t st) {
+  constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, STAGE = (BM + BN) * 128;
   g.tiles_n = (g.N + BN - 1) / BN;
   g.tiles = (g.P + BM - 1) / BM * g.tiles_n;
   if (g.tiles > 0x7fffffffll) return GB_ERANGE;
-  fp8_gemm_kernel<T, TM, TN, WM, WN><<<(unsigned)g.tiles, 64 * WM * WN, 0, st>>>(g);
-  return check_launch("gb_fp8_gemm");
+  if (2 * STAGE > 65536) {
+    static std::atomic<unsigned long long> done{0};
+    allow_dynamic_lds(fp8_gemm_kernel<T, TM, TN, WM, WN, NT>, 2 * STAGE, done);
+  }
+  fp8_gemm_kernel<T, TM, TN, WM, WN, NT><<<(unsigned)g.tiles, 64 * WM * WN, (g.Kb > 1 ? 2 : 1) * STAGE, st>>>(g);
+  return check_launch("gb_fp8_linear");
+}
+template <typename T, int TM, int TN, int WM, int WN>
+static int launch_tiles(const GemmArgs8 &g, hipStream_t st) {
+  return streams(g.P * g.N * (long long)sizeof(T)) ? launch_tiles_nt<T, TM, TN, WM, WN, true>(g, st)
+                                                   : launch_tiles_nt<T, TM, TN, WM, WN, false>(g, st);
 }
 
 static long long tiles_of(long long P, int N, int b) { return ((P + b - 1) / b) * ((N + b - 1) / b); }
+// y from codes and exponents in memory
+template <typename T>
+static int multiply_codes(const GemmArgs8 &g, int K, hipStream_t st) {
+  if (g.P <= FP8_FEW_ROWS) {
+    const unsigned grid = (unsigned)((g.N + 15) / 16);
+    if (g.P <= 16)
+      fp8_few_kernel<T, 1, false><<<grid, 256, 0, st>>>(g, nullptr, K, nullptr, nullptr);
+    else if (g.P <= 32)
+      fp8_few_kernel<T, 2, false><<<grid, 256, 0, st>>>(g, nullptr, K, nullptr, nullptr);
+    else
+      fp8_few_kernel<T, 4, false><<<grid, 256, 0, st>>>(g, nullptr, K, nullptr, nullptr);
+    return check_launch("gb_fp8_linear");
+  }
+  // 256 x 256 where that still gives every CU a tile, the columns fill it as well as 128 do to a fifth, and there are steps
+  // enough to work through; short reductions live from several workgroups per CU, which only smaller tiles leave room for.
+  if (g.Kb >= 4 && tiles_of(g.P, g.N, 256) >= 256 && 5 * blocks128(g.N) >= 8 * ((g.N + 255) / 256)) return launch_tiles<T, 4, 2, 2, 4>(g, st);
+  if (tiles_of(g.P, g.N, 128) >= 256) return launch_tiles<T, 2, 2, 2, 2>(g, st);
+  return launch_tiles<T, 1, 2, 2, 1>(g, st);
+}
+
+// columns of the streaming kernel's variant; 0: not one of its shapes
+static int stream_columns(long long P, int N, int K) {
+  if (P < FP8_STREAM_ROWS || N > 512) return 0;
+  const int cols = N <= 128 ? 128 : N <= 256 ? 256 : 512;
+  return (long long)cols * blocks128(K) * 128 <= 65536 ? cols : 0;
+}
+struct StreamPlan8 {
+  size_t lds;
+  int grid;
+};
+static StreamPlan8 stream_plan(long long P, int cols, int K, int dtype, bool sum) {
+  StreamPlan8 p;
+  const int Kp = blocks128(K) * 128;
+  p.lds = (size_t)cols * Kp + 2 * 64 * 128 + 2 * 64 + 4 * (dtype == GB_T_F32 ? Cell<float>::BYTES : Cell<__bf16>::BYTES) + (sum ? (size_t)16 * Kp * 4 : 0);
+  const int by_lds = (int)(163840 / p.lds), by_regs = (cols == 128 ? 4 : cols == 256 ? 3 : 2) - (dtype == GB_T_F32 && cols < 512),
+             per_cu = by_lds < by_regs ? by_lds : by_regs;
+  const long long tiles = (P + 63) / 64, most = 256ll * (per_cu < 1 ? 1 : per_cu);
+  p.grid = (int)(tiles < most ? tiles : most);
+  return p;
+}
+template <typename T, int TM, int TN, int WM, int WN, bool SUM>
+static int launch_stream(const StreamArgs8 &g, const StreamPlan8 &p, hipStream_t st) {
+  const bool nt = streams(g.P * (g.N < g.K ? g.N : g.K) * (long long)sizeof(T));
+  static std::atomic<unsigned long long> done[2];
+  if (nt) {
+    allow_dynamic_lds(fp8_stream_kernel<T, TM, TN, WM, WN, SUM, true>, 163840, done[1]);
+    fp8_stream_kernel<T, TM, TN, WM, WN, SUM, true><<<(unsigned)p.grid, 256, p.lds, st>>>(g);
+  } else {
+    allow_dynamic_lds(fp8_stream_kernel<T, TM, TN, WM, WN, SUM, false>, 163840, done[0]);
+    fp8_stream_kernel<T, TM, TN, WM, WN, SUM, false><<<(unsigned)p.grid, 256, p.lds, st>>>(g);
+  }
+  return check_launch("gb_fp8_linear");
+}
+template <typename T, bool SUM>
+static int stream_rows(const StreamArgs8 &g, const StreamPlan8 &p, int cols, hipStream_t st) {
+  return cols == 128   ? launch_stream<T, 1, 2, 2, 2, SUM>(g, p, st)
+         : cols == 256 ? launch_stream<T, 2, 2, 1, 4, SUM>(g, p, st)
+                       : launch_stream<T, 2, 4, 1, 4, SUM>(g, p, st);
+}
+
 
 static bool fp8_dims_bad(long long P, int N, int K) { return P < 0 || N <= 0 || K <= 0; }
 static bool fp8_dims_large(long long P, int N, int K) {   // int tile offsets: 256 rows of Kp bytes; 65535 blocks a grid axis
@@ -568,15 +900,15 @@ struct WgradPlan8 {
   int tiles_n, tiles_k, splits;
   long long rows;
 };
-// 256 x 256 outputs per workgroup where both sides fill them, else 128 x 128; the rows are cut until there are ~512
-// workgroups, into ranges of 512 rows at least (a range writes its outputs once more and has them read once more).
+// 256 x 256 outputs per workgroup where both sides fill them, else 128 x 128; the rows are cut until there is a workgroup
+// of the large kind for every CU, or two of the small, into ranges of 512 rows at least (a range writes its outputs once more and has them read once more).
 static WgradPlan8 wgrad_plan(long long P, int N, int K) {
   WgradPlan8 p;
   p.big = N > 192 && K > 192;
   const int b = p.big ? 256 : 128;
   p.tiles_n = (N + b - 1) / b;
   p.tiles_k = (K + b - 1) / b;
-  const long long tiles = (long long)p.tiles_n * p.tiles_k, want = (512 + tiles - 1) / tiles, most = (P + 511) / 512;
+  const long long tiles = (long long)p.tiles_n * p.tiles_k, want = ((p.big ? 256 : 512) + tiles - 1) / tiles, most = (P + 511) / 512;
   long long splits = want < most ? want : most;
   if (splits < 1) splits = 1;
   p.rows = ((P + splits - 1) / splits + 31) / 32 * 32;
@@ -625,80 +957,115 @@ extern "C" int gb_fp8_quant_weight(const void *w, int dtype, int N, int K, void 
   });
 }
 
-static int fp8_args_bad(const void *b, const void *b_scales, const void *y) {
-  return !b || !b_scales || !y || reinterpret_cast<uintptr_t>(b) % 16;
+// Which way a product goes: quantised by every workgroup for itself (few), streamed, or quantised by a kernel of its own
+// before the tiles.
+enum { FP8_FEW, FP8_STREAM, FP8_TILES };
+static int linear_route(long long P, int N, int K) {
+  if (P <= FP8_FUSED_ROWS && P * blocks128(K) * 128 <= FP8_FUSED_CODES) return FP8_FEW;
+  return stream_columns(P, N, K) ? FP8_STREAM : FP8_TILES;
+}
+static long long up16(long long n) { return (n + 15) / 16 * 16; }
+// (the 16-bit plan has at least as many workgroups as the fp32 one)
+// bytes: column sums' partials, then the codes and exponents of the tiles' route where the caller keeps none
+static long long linear_workspace(long long P, int N, int K, bool keeps, bool sum) {
+  const int route = linear_route(P, N, K);
+  long long b = 0;
+  if (sum) {
+    const long long per = rows_per_chunk(P, true),
+                    chunks = route == FP8_STREAM ? stream_plan(P, stream_columns(P, N, K), K, GB_T_BF16, true).grid : (P + per - 1) / per;
+    b += up16(chunks * K * 4);
+  }
+  if ((route == FP8_TILES || (route == FP8_FEW && sum)) && !keeps) b += P * (blocks128(K) * 128ll) + up16(P * scale_stride(K));
+  return b;
 }
 
-extern "C" int gb_fp8_gemm(const void *a, const void *a_scales, const void *b, const void *b_scales, int transposed, const float *bias,
-                           void *y, int dtype, long long P, int N, int K, void *stream) {
-  if (fp8_dims_bad(P, N, K) || !known_type(dtype)) return GB_EINVAL;
+extern "C" int gb_fp8_linear(const void *x, int dtype, long long P, int K, const void *w, const void *w_scales, int transposed, int N,
+                             const float *bias, void *y, void *codes, void *scales, float *colsum, void *ws, long long ws_bytes,
+                             void *stream) {
+  if (fp8_dims_bad(P, N, K) || !known_type(dtype) || !codes != !scales) return GB_EINVAL;
   if (fp8_dims_large(P, N, K)) return GB_ERANGE;
-  if (P == 0) return GB_OK;
-  if (fp8_args_bad(b, b_scales, y) || !a || !a_scales || (reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(a_scales)) % 16)
+  if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(ws) |
+       reinterpret_cast<uintptr_t>(w)) % 16)
     return GB_EINVAL;
-  GemmArgs8 g = {};
-  g.a = (const unsigned char *)a;
-  g.a_scales = (const unsigned char *)a_scales;
-  g.b = (const unsigned char *)b;
-  g.b_scales = (const unsigned char *)b_scales;
-  g.bias = bias;
-  g.y = y;
-  g.P = P;
-  g.N = N;
-  g.Kb = blocks128(K);
-  g.a_stride = scale_stride(K);
-  g.bs_n = transposed ? 1 : g.Kb;
-  g.bs_k = transposed ? blocks128(N) : 1;
+  if (P > 0 && (!x || !y || !w || !w_scales)) return GB_EINVAL;
+  const long long need = linear_workspace(P, N, K, codes != nullptr, colsum != nullptr);
+  if (need > 0 && (!ws || ws_bytes < need)) return GB_EINVAL;
   hipStream_t st = as_stream(stream);
-  return with_type(dtype, [&](auto z) {
-    typedef decltype(z) T;
-    if (P <= FP8_FEW_ROWS) {
-      const unsigned grid = (unsigned)((N + 15) / 16);
-      if (P <= 16)
-        fp8_few_kernel<T, 1, false><<<grid, 256, 0, st>>>(g, nullptr, K);
-      else if (P <= 32)
-        fp8_few_kernel<T, 2, false><<<grid, 256, 0, st>>>(g, nullptr, K);
-      else
-        fp8_few_kernel<T, 4, false><<<grid, 256, 0, st>>>(g, nullptr, K);
-      return check_launch("gb_fp8_gemm");
-    }
-    // the largest tile that still gives every CU one
-    if (tiles_of(P, N, 256) >= 256) return launch_tiles<T, 4, 2, 2, 4>(g, st);
-    if (tiles_of(P, N, 128) >= 256) return launch_tiles<T, 2, 2, 2, 2>(g, st);
-    return launch_tiles<T, 1, 2, 2, 1>(g, st);
-  });
-}
-
-extern "C" int gb_fp8_linear_few(const void *x, const void *b, const void *b_scales, const float *bias, void *y, int dtype, int P, int N,
-                                 int K, void *stream) {
-  if (fp8_dims_bad(P, N, K) || !known_type(dtype)) return GB_EINVAL;
-  if (fp8_dims_large(P, N, K) || P > FP8_FUSED_ROWS || (long long)P * blocks128(K) * 128 > FP8_FUSED_CODES) return GB_ERANGE;
-  if (P == 0) return GB_OK;
-  if (fp8_args_bad(b, b_scales, y) || !x) return GB_EINVAL;
+  if (P == 0) {
+    if (!colsum) return GB_OK;
+    fp8_colsum_kernel<<<(K + 31) / 32, 256, 0, st>>>((const float *)ws, 0, K, colsum);
+    return check_launch("gb_fp8_linear");
+  }
+  const int route = linear_route(P, N, K), Kb = blocks128(K), bs_n = transposed ? 1 : Kb, bs_k = transposed ? blocks128(N) : 1;
+  if (route == FP8_STREAM) {
+    const int cols = stream_columns(P, N, K);
+    const StreamPlan8 p = stream_plan(P, cols, K, dtype, colsum != nullptr);
+    StreamArgs8 g = {};
+    g.x = x;
+    g.w = (const unsigned char *)w;
+    g.w_scales = (const unsigned char *)w_scales;
+    g.bias = bias;
+    g.y = y;
+    g.codes = (unsigned char *)codes;
+    g.scales = (unsigned char *)scales;
+    g.part = (float *)ws;
+    g.P = P;
+    g.tiles = (P + 63) / 64;
+    g.N = N;
+    g.K = K;
+    g.bs_n = bs_n;
+    g.bs_k = bs_k;
+    const int rc = with_type(dtype, [&](auto z) {
+      typedef decltype(z) T;
+      return colsum ? stream_rows<T, true>(g, p, cols, st) : stream_rows<T, false>(g, p, cols, st);
+    });
+    if (rc || !colsum) return rc;
+    fp8_colsum_kernel<<<(K + 31) / 32, 256, 0, st>>>((const float *)ws, p.grid, K, colsum);
+    return check_launch("gb_fp8_linear");
+  }
   GemmArgs8 g = {};
-  g.b = (const unsigned char *)b;
-  g.b_scales = (const unsigned char *)b_scales;
+  g.b = (const unsigned char *)w;
+  g.b_scales = (const unsigned char *)w_scales;
   g.bias = bias;
   g.y = y;
   g.P = P;
   g.N = N;
-  g.Kb = blocks128(K);
-  g.bs_n = g.Kb;
-  g.bs_k = 1;
-  const size_t lds = ((size_t)P * g.Kb * 129 + 15) / 16 * 16;
+  g.Kb = Kb;
+  g.a_stride = scale_stride(K);
+  g.bs_n = bs_n;
+  g.bs_k = bs_k;
+  if (route == FP8_FEW && !colsum) {
+    const size_t lds = (size_t)up16(P * Kb * 129);
+    return with_type(dtype, [&](auto z) {
+      typedef decltype(z) T;
+      fp8_few_kernel<T, 1, true><<<(unsigned)((N + 15) / 16), 256, lds, st>>>(g, (const T *)x, K, (unsigned char *)codes, (unsigned char *)scales);
+      return check_launch("gb_fp8_linear");
+    });
+  }
+  unsigned char *at = (unsigned char *)ws;
+  const long long sums = colsum ? linear_workspace(P, N, K, true, true) : 0;
+  if (!codes) {
+    codes = at + sums;
+    scales = (unsigned char *)codes + P * (Kb * 128ll);
+  }
+  const int rc = gb_fp8_quant_rows(x, dtype, P, K, codes, scales, colsum, ws, sums, stream);
+  if (rc) return rc;
+  g.a = (const unsigned char *)codes;
+  g.a_scales = (const unsigned char *)scales;
   return with_type(dtype, [&](auto z) {
     typedef decltype(z) T;
-    fp8_few_kernel<T, 1, true><<<(unsigned)((N + 15) / 16), 256, lds, as_stream(stream)>>>(g, (const T *)x, K);
-    return check_launch("gb_fp8_linear_few");
+    return multiply_codes<T>(g, K, st);
   });
 }
 
 extern "C" int gb_fp8_workspace(int what, long long P, int N, int K, long long *bytes) {
-  if (fp8_dims_bad(P, N, K) || !bytes || (what != GB_FP8_WS_COLSUM && what != GB_FP8_WS_WGRAD)) return GB_EINVAL;
+  if (fp8_dims_bad(P, N, K) || !bytes || (what != GB_FP8_WS_COLSUM && what != GB_FP8_WS_WGRAD && (what < GB_FP8_WS_LINEAR || what >= GB_FP8_WS_LINEAR + 4))) return GB_EINVAL;
   if (fp8_dims_large(P, N, K)) return GB_ERANGE;
   if (what == GB_FP8_WS_COLSUM) {
     const int per = rows_per_chunk(P, true);
     *bytes = (P + per - 1) / per * N * 4;
+  } else if (what >= GB_FP8_WS_LINEAR) {
+    *bytes = linear_workspace(P, N, K, (what - GB_FP8_WS_LINEAR) & GB_FP8_KEEP, (what - GB_FP8_WS_LINEAR) & GB_FP8_SUM);
   } else {
     const WgradPlan8 p = wgrad_plan(P, N, K);
     *bytes = p.splits > 1 ? (long long)p.splits * N * K * 4 : 0;
@@ -715,7 +1082,7 @@ extern "C" int gb_fp8_wgrad(const void *dy, const void *dy_scales, const void *x
   const WgradPlan8 p = wgrad_plan(P, N, K);
   const long long n = (long long)N * K;
   if (p.splits > 1 && (!ws || ws_bytes < p.splits * n * 4 || reinterpret_cast<uintptr_t>(ws) % 16)) return GB_EINVAL;
-  if ((long long)p.tiles_n * p.tiles_k > 0x7fffffffll || (n + 63) / 64 > 0x7fffffffll) return GB_ERANGE;
+  if ((long long)p.tiles_n * p.tiles_k > 0x7fffffffll || (n + 31) / 32 > 0x7fffffffll) return GB_ERANGE;
   hipStream_t st = as_stream(stream);
   WgradArgs8 g = {};
   g.dy = (const unsigned char *)dy;
@@ -735,6 +1102,6 @@ extern "C" int gb_fp8_wgrad(const void *dy, const void *dy_scales, const void *x
     else
       fp8_wgrad_kernel<2, 2, 2, 2><<<grid, 256, 0, st>>>(g);
   }
-  if (p.splits != 1) fp8_wgrad_join_kernel<<<(unsigned)((n + 63) / 64), 256, 0, st>>>((const float *)ws, p.splits, n, dw);
+  if (p.splits != 1) fp8_wgrad_join_kernel<<<(unsigned)((n + 31) / 32), 256, 0, st>>>((const float *)ws, p.splits, n, dw);
   return check_launch("gb_fp8_wgrad");
 }

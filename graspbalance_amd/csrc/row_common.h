@@ -1,58 +1,80 @@
-// Shared helpers of the channel-last row operators (row_norm.hip, row_dropout.hip, fp8.hip): element types, eight
-// consecutive elements per lane, the counter-based generator.
+// Shared helpers of the channel-last row operators (row_norm.hip, row_dropout.hip, fp8.hip): element types, 16
+// bytes of consecutive elements per lane, the counter-based generator.
 #pragma once
 #include "gb_common.h"
 
 namespace gb {
 
-// Eight consecutive elements as fp32.  A lane always works on eight: one 16-byte access for the 16-bit types, two for
-// fp32, and exactly the eight 16-bit numbers that one block of the generator gives.  The accesses carry no alignment
-// (tensors that start inside another one are legal; the hardware takes any byte address).
-struct F8 {
-  float v[8];
+// A lane's unit of work: the 16 bytes of one access, N = 4 fp32 or 8 16-bit elements, widened to fp32.  Neighbouring lanes
+// take neighbouring units, so that a wave's access covers whole lines (fp32 in eights per lane, two accesses of every
+// other 16 bytes, copied 268 MB at 3.8 - 5.0 TB/s; in units 5.3 - 6.1).  The accesses carry no alignment: tensors that start
+// inside another one are legal, and the hardware takes any address.
+template <typename T>
+struct Unit {
+  static constexpr int N = 16 / (int)sizeof(T);
 };
 template <typename T>
-struct Raw8 {
-  T v[8];
+struct Raw {
+  T v[Unit<T>::N];
+};
+template <int N>
+struct Vec {
+  float v[N];
 };
 template <typename T>
-__device__ __forceinline__ Raw8<T> load_raw8(const T *p) {
-  Raw8<T> r;
-  __builtin_memcpy(&r, p, sizeof(r));
+using VecOf = Vec<Unit<T>::N>;
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+
+// NT: the tensors are far larger than the caches, and a line that nobody will find there again is kept out of them (268 MB:
+// reads 5.6 -> 6.4 TB/s, copies 5.4 -> 5.9).
+template <bool NT = false, typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T *p) {
+  Raw<T> r;
+  if (NT) {
+    const u32x4_any w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p));
+    __builtin_memcpy(&r, &w, 16);
+  } else {
+    __builtin_memcpy(&r, p, 16);
+  }
   return r;
 }
 template <typename T>
-__device__ __forceinline__ F8 widen(const Raw8<T> &r) {
-  F8 f;
+__device__ __forceinline__ VecOf<T> widen(const Raw<T> &r) {
+  VecOf<T> f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) f.v[k] = (float)r.v[k];
+  for (int k = 0; k < Unit<T>::N; ++k) f.v[k] = (float)r.v[k];
   return f;
 }
-template <typename T>
-__device__ __forceinline__ F8 load8(const T *p) {
-  return widen(load_raw8(p));
+template <bool NT = false, typename T>
+__device__ __forceinline__ VecOf<T> load_unit(const T *p) {
+  return widen(load_raw<NT>(p));
 }
-template <typename T>
-__device__ __forceinline__ void store8(T *p, const F8 &f) {  // the one rounding of a result: nearest, ties to even
-  Raw8<T> r;
+template <bool NT = false, typename T>
+__device__ __forceinline__ void store_unit(T *p, const VecOf<T> &f) {  // the one rounding of a result: nearest, ties to even
+  Raw<T> r;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) r.v[k] = (T)f.v[k];
-  __builtin_memcpy(p, &r, sizeof(r));
+  for (int k = 0; k < Unit<T>::N; ++k) r.v[k] = (T)f.v[k];
+  if (NT) {
+    u32x4_any w;
+    __builtin_memcpy(&w, &r, 16);
+    __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any *>(p));
+  } else {
+    __builtin_memcpy(p, &r, 16);
+  }
 }
-
-// the first n < 8 of eight elements; the others read as zero
+// the first n of a unit's elements; the others read as zero
 template <typename T>
-__device__ __forceinline__ F8 load_tail(const T *p, int n) {
-  F8 f = {};
+__device__ __forceinline__ VecOf<T> load_part(const T *p, int n) {
+  VecOf<T> f = {};
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
+  for (int k = 0; k < Unit<T>::N; ++k)
     if (k < n) f.v[k] = (float)p[k];
   return f;
 }
 template <typename T>
-__device__ __forceinline__ void store_tail(T *p, const F8 &f, int n) {
+__device__ __forceinline__ void store_part(T *p, const VecOf<T> &f, int n) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
+  for (int k = 0; k < Unit<T>::N; ++k)
     if (k < n) p[k] = (T)f.v[k];
 }
 
@@ -89,16 +111,18 @@ __device__ __forceinline__ unsigned block_mask(const unsigned (&w)[4], unsigned 
     m |= ((w[k] & 0xffffu) >= q ? 1u : 0u) << (2 * k) | ((w[k] >> 16) >= q ? 1u : 0u) << (2 * k + 1);
   return m;
 }
-__device__ __forceinline__ unsigned keep8(const RowRng &g, unsigned long long i, unsigned q) {
+// the N elements from element i on
+template <int N>
+__device__ __forceinline__ unsigned keep_mask(const RowRng &g, unsigned long long i, unsigned q) {
   unsigned w[4];
   philox_block(g, i >> 3, w);
   unsigned m = block_mask(w, q);
   const int r = (int)(i & 7);
-  if (r) {  // eight elements of a packed cloud that starts inside a block: the rest of them are in the next block
+  if (r + N > 8) {  // a packed cloud that starts inside a block: the rest of the elements are in the next one
     philox_block(g, (i >> 3) + 1, w);
-    m = (m | block_mask(w, q) << 8) >> r;
+    m |= block_mask(w, q) << 8;
   }
-  return m & 0xffu;
+  return m >> r & ((1u << N) - 1);
 }
 
 // [seed, call] from the device (a captured graph's next replay sees what its owner wrote there) or by value; the pair
@@ -114,6 +138,9 @@ __device__ __forceinline__ RowRng load_rng(const long long *rng, long long seed,
 inline float keep_scale(int q) { return q < 65536 ? (float)(65536.0 / (65536 - q)) : 0.0f; }
 
 inline bool known_type(int t) { return t == GB_T_F32 || t == GB_T_BF16 || t == GB_T_F16; }
+
+// Tensors that no cache keeps until somebody reads them again (the last level holds 256 MB)
+inline bool streams(long long bytes) { return bytes >= (96ll << 20); }
 
 // f(T()) for the element type behind a GB_T_* code
 template <typename F>

@@ -6,39 +6,36 @@
 
 namespace gb {
 
-// A lane takes eight consecutive elements = one block of the generator = 16 bytes (two times 16 for fp32) per tensor.
-// `full`: blocks of eight that lie wholly inside n; the last lane takes the rest element by element.
-template <typename T, bool RES>
+// A lane takes units of 16 bytes.  For the 16-bit types that is one block of the generator; for fp32 two lanes compute the
+// same block - 40 integer products for four elements are a third of what the bytes take.
+template <typename T, bool RES, bool NT>
 __global__ __launch_bounds__(256) void dropout_kernel(const T *__restrict__ x, const T *__restrict__ res, T *__restrict__ y,
                                                       long long n, unsigned q, float scale, const long long *__restrict__ rng,
                                                       long long seed, long long call, long long *__restrict__ used) {
+  constexpr int N = Unit<T>::N;
   const RowRng g = load_rng(rng, seed, call);
   const long long t0 = (long long)blockIdx.x * 256 + threadIdx.x, stride = (long long)gridDim.x * 256;
   if (t0 == 0 && used) {
     used[0] = (long long)g.seed;
     used[1] = (long long)g.call;
   }
-  const long long full = n >> 3;
-  for (long long b = t0; b < full; b += stride) {
-    F8 f = load8(x + 8 * b);
-    F8 r;
-    if (RES) r = load8(res + 8 * b);
-    unsigned w[4];
-    philox_block(g, (unsigned long long)b, w);
-    const unsigned m = block_mask(w, q);
+  const long long full = n / N;
+  for (long long u = t0; u < full; u += stride) {
+    VecOf<T> f = load_unit<NT>(x + N * u);
+    VecOf<T> r;
+    if (RES) r = load_unit<NT>(res + N * u);
+    const unsigned m = keep_mask<N>(g, (unsigned long long)(N * u), q);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < N; ++k) {
       f.v[k] = (m >> k & 1) ? f.v[k] * scale : 0.0f;
       if (RES) f.v[k] += r.v[k];
     }
-    store8(y + 8 * b, f);
+    store_unit<NT>(y + N * u, f);
   }
-  if (t0 == 0 && (n & 7)) {
-    unsigned w[4];
-    philox_block(g, (unsigned long long)full, w);
-    const unsigned m = block_mask(w, q);
-    for (int k = 0; k < (int)(n & 7); ++k) {
-      const long long i = 8 * full + k;
+  if (t0 == 0 && n % N) {
+    const unsigned m = keep_mask<N>(g, (unsigned long long)(N * full), q);
+    for (int k = 0; k < (int)(n % N); ++k) {
+      const long long i = N * full + k;
       float f = (m >> k & 1) ? (float)x[i] * scale : 0.0f;
       if (RES) f += (float)res[i];
       y[i] = (T)f;
@@ -56,17 +53,20 @@ extern "C" int gb_dropout(const void *x, const void *residual, void *y, long lon
   if (n == 0 && !used) return GB_OK;
   if (n > 0 && (!x || !y)) return GB_EINVAL;
   if ((reinterpret_cast<uintptr_t>(rng) | reinterpret_cast<uintptr_t>(used)) % 8 != 0) return GB_EINVAL;
-  const long long blocks = ((n >> 3) + 255) / 256;
-  const int grid = (int)(blocks < 1 ? 1 : blocks > 8192 ? 8192 : blocks);
   const float scale = keep_scale(q);
   return with_type(dtype, [&](auto z) {
     typedef decltype(z) T;
+    const long long blocks = (n / Unit<T>::N + 255) / 256;
+    const int grid = (int)(blocks < 1 ? 1 : blocks > 8192 ? 8192 : blocks);
+    auto launch = [&](auto kernel) {
+      kernel<<<grid, 256, 0, as_stream(stream)>>>((const T *)x, (const T *)residual, (T *)y, n, (unsigned)q, scale,
+                                                  (const long long *)rng, seed, call, (long long *)used);
+    };
+    const bool nt = streams(n * (long long)sizeof(T));
     if (residual)
-      dropout_kernel<T, true><<<grid, 256, 0, as_stream(stream)>>>(
-          (const T *)x, (const T *)residual, (T *)y, n, (unsigned)q, scale, (const long long *)rng, seed, call, (long long *)used);
+      nt ? launch(dropout_kernel<T, true, true>) : launch(dropout_kernel<T, true, false>);
     else
-      dropout_kernel<T, false><<<grid, 256, 0, as_stream(stream)>>>(
-          (const T *)x, nullptr, (T *)y, n, (unsigned)q, scale, (const long long *)rng, seed, call, (long long *)used);
+      nt ? launch(dropout_kernel<T, false, true>) : launch(dropout_kernel<T, false, false>);
     return check_launch("gb_dropout");
   });
 }

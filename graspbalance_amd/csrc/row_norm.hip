@@ -8,10 +8,10 @@
 // What bounds it: bytes.  The statistics stand between two uses of x, so a sample that does not fit one workgroup's
 // registers is read twice (forward 2 reads + 1 write, backward 4 + 1); one that does is read once.
 //
-// One mapping serves every pass and every channel count: a sample is ONE array of rows * C elements, a lane takes eight
-// consecutive ones, and the lanes that work step by T * 8 elements, T the largest multiple of C / gcd(C, 8) in the workgroup.
-// Then a lane meets the same eight channels at every step: its weights stay in registers, its sums need no index, loads
-// are full 16-byte accesses for odd C as well, and no lane divides.
+// One mapping serves every pass and every channel count: a sample is ONE array of rows * C elements, a lane takes units of N
+// consecutive ones (16 bytes), and the lanes that work step by T units, T the largest multiple of C / gcd(C, N) in the
+// workgroup.  Then a lane meets the same N channels at every step: its weights stay in registers, its sums need no index,
+// loads are full 16-byte accesses for odd C as well, and no lane divides.
 #include <type_traits>
 
 #include "row_common.h"
@@ -21,13 +21,14 @@
 namespace gb {
 
 static constexpr int GN_MAX_C = 4096;   // two doubles per channel in LDS while a workgroup's sums are joined
+static constexpr int GN_MIN_STEPS = 4;  // of a workgroup: with fewer, joining the sums costs what the parallelism gains
 
 struct GnShape {
   long long R;         // rows of the whole tensor
   long long rows;      // rows per sample (offs == nullptr)
   const long long *offs;
   int S, C, G, cpg;
-  int P8, T;           // lanes of one period, lanes that work (a multiple of P8)
+  int PL, T;           // lanes of one period, lanes that work (a multiple of PL)
   int ns;              // workgroups per sample
 };
 
@@ -66,13 +67,33 @@ __device__ __forceinline__ void sample_rows(const GnShape &sh, int s, long long 
 // z = x * sigmoid(x) and friends in fp32; v_exp_f32 / v_rcp_f32 are good to 1 ulp and the argument's rounding adds
 // |z| 2^-24: ~1e-7 where the value is not itself vanishing.
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
+// Phi(z) = erfc(-z / sqrt 2) / 2 and e = exp(-z^2 / 2), which the slope needs as well.  erfcx(a) = t P(t), t = 1 / (1 + 0.425 a), P of
+// degree 7 fitted for the least relative error over 0 <= a <= 9.3 (1.1e-7); negative z are taken from the tail itself, so
+// that gelu keeps its relative error there (8e-7 down to z = -5).  No branch: sixteen erff of a lane's unit twice cost spills.
+__device__ __forceinline__ float normal_cdf(float z, float &e) {
+  e = __expf(-0.5f * z * z);
+  const float t = __builtin_amdgcn_rcpf(1.0f + 0.30052038f * fabsf(z));   // 0.425 / sqrt 2
+  float p = 0.07247326f;
+  p = p * t - 0.31730647f;
+  p = p * t + 0.41477657f;
+  p = p * t - 0.10985138f;
+  p = p * t + 0.25858663f;
+  p = p * t + 0.1996421f;
+  p = p * t + 0.24201177f;
+  p = p * t + 0.23966741f;
+  const float tail = 0.5f * (p * t) * e;
+  return z < 0.0f ? tail : 1.0f - tail;
+}
 template <int ACT>
 __device__ __forceinline__ float act_value(float z, float slope) {
   switch (ACT) {
     case GB_ACT_RELU: return z > 0.0f ? z : z != z ? z : 0.0f;
     case GB_ACT_LEAKY_RELU: return z > 0.0f ? z : slope * z;
     case GB_ACT_SILU: return z * sigmoid(z);
-    case GB_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+    case GB_ACT_GELU: {
+      float e;
+      return z * normal_cdf(z, e);
+    }
     default: return z;
   }
 }
@@ -85,12 +106,16 @@ __device__ __forceinline__ float act_slope(float z, float slope) {
       const float s = sigmoid(z);
       return s * (1.0f + z * (1.0f - s));
     }
-    case GB_ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * __expf(-0.5f * z * z) * 0.39894228f;
+    case GB_ACT_GELU: {
+      float e;
+      const float c = normal_cdf(z, e);
+      return c + z * e * 0.39894228f;
+    }
     default: return 1.0f;
   }
 }
 
-// The lane's place in the period: eight channels (8 p + k) mod C.
+// The lane's place in the period: N channels (N p + k) mod C.
 struct Lane {
   int p, r;       // place in the period, row of lanes
   bool on;
@@ -98,34 +123,37 @@ struct Lane {
 __device__ __forceinline__ Lane lane_place(const GnShape &sh) {
   Lane l;
   const int t = (int)threadIdx.x;
-  l.r = t / sh.P8;
-  l.p = t - l.r * sh.P8;
+  l.r = t / sh.PL;
+  l.p = t - l.r * sh.PL;
   l.on = t < sh.T;
   return l;
 }
-__device__ __forceinline__ int channel0(const GnShape &sh, int p) { return (int)((8ll * p) % sh.C); }
+template <int N>
+__device__ __forceinline__ int channel0(const GnShape &sh, int p) {
+  return (N * p) % sh.C;
+}
 __device__ __forceinline__ int next_channel(const GnShape &sh, int c) { return c + 1 == sh.C ? 0 : c + 1; }
 
-// Joins (v0, v1)[K] of the T working lanes per channel (K = 8) or per eight (K = 1) into out0 / out1, in a fixed order.
-// buf: half of the lanes' values; out0, out1: C (K = 8) or P8 (K = 1) entries.  The lanes of one column are added as a
-// tree; then the eight elements of a lane go to their channels one after another - at each of the eight steps every lane
-// has another channel - because with C not a multiple of 8 a channel appears at several places of the period.
+// Joins (v0, v1)[K] of the T working lanes per channel (K = N) or per unit (K = 1) into out0 / out1, in a fixed order.
+// buf: half of the lanes' values; out0, out1: C (K = N) or PL (K = 1) entries.  The lanes of one column are added as a
+// tree; then the N elements of a lane go to their channels one after another - at each of these steps every lane has
+// another channel - because with C not a multiple of N a channel appears at several places of the period.
 template <int K, typename A>
 __device__ __forceinline__ void join_columns(const GnShape &sh, const Lane &l, A (&v0)[K], A (&v1)[K], A *buf, A *out0,
                                              A *out1) {
-  const int RL = sh.T / sh.P8;
+  const int RL = sh.T / sh.PL;
   int h = 1;
   while (2 * h < RL) h *= 2;
   if (RL > 1)
     for (; h >= 1; h >>= 1) {
       if (l.on && l.r >= h && l.r < 2 * h) {
-        A *to = buf + (long long)((l.r - h) * sh.P8 + l.p) * 2 * K;
+        A *to = buf + ((l.r - h) * sh.PL + l.p) * 2 * K;
 #pragma unroll
         for (int k = 0; k < K; ++k) to[2 * k] = v0[k], to[2 * k + 1] = v1[k];
       }
       __syncthreads();
       if (l.on && l.r < h && l.r + h < RL) {
-        const A *from = buf + (long long)(l.r * sh.P8 + l.p) * 2 * K;
+        const A *from = buf + (l.r * sh.PL + l.p) * 2 * K;
 #pragma unroll
         for (int k = 0; k < K; ++k) v0[k] += from[2 * k], v1[k] += from[2 * k + 1];
       }
@@ -137,12 +165,12 @@ __device__ __forceinline__ void join_columns(const GnShape &sh, const Lane &l, A
   } else {
     for (int c = (int)threadIdx.x; c < sh.C; c += (int)blockDim.x) out0[c] = 0, out1[c] = 0;
     __syncthreads();
-    int c = channel0(sh, l.p);
+    int c = channel0<K>(sh, l.p);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (l.on && l.r == 0) out0[c] += v0[k], out1[c] += v1[k];
       c = next_channel(sh, c);
-      if (sh.C & 7) __syncthreads();
+      if (sh.C % K) __syncthreads();
     }
   }
   __syncthreads();
@@ -170,20 +198,21 @@ __device__ __forceinline__ void for_group_sums(const A *a, const A *b, int G, in
   }
 }
 
-// Running count, mean and sum of squared deviations of a lane's eight columns (Chan, Golub, LeVeque: "Algorithms for
-// computing the sample variance", 1983): four rows at a time, so that an offset of the data costs no bits.
+// Running count, mean and sum of squared deviations of a lane's N columns (Chan, Golub, LeVeque: "Algorithms for computing
+// the sample variance", 1983): four rows at a time, so that an offset of the data costs no bits.
+template <int N>
 struct Moments {
   float n;
-  float mean[8], m2[8];
+  float mean[N], m2[N];
   __device__ void clear() {
     n = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) mean[k] = m2[k] = 0;
+    for (int k = 0; k < N; ++k) mean[k] = m2[k] = 0;
   }
-  __device__ void add4(const F8 &a, const F8 &b, const F8 &c, const F8 &d) {
+  __device__ void add4(const Vec<N> &a, const Vec<N> &b, const Vec<N> &c, const Vec<N> &d) {
     const float f = 4.0f / (n + 4.0f), e = n * f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < N; ++k) {
       const float m = 0.25f * ((a.v[k] + b.v[k]) + (c.v[k] + d.v[k]));
       const float da = a.v[k] - m, db = b.v[k] - m, dc = c.v[k] - m, dd = d.v[k] - m, del = m - mean[k];
       mean[k] += del * f;
@@ -191,10 +220,10 @@ struct Moments {
     }
     n += 4.0f;
   }
-  __device__ void add1(const F8 &a) {
+  __device__ void add1(const Vec<N> &a) {
     const float f = 1.0f / (n + 1.0f);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < N; ++k) {
       const float del = a.v[k] - mean[k];
       mean[k] += del * f;
       m2[k] += del * (a.v[k] - mean[k]);
@@ -203,69 +232,91 @@ struct Moments {
   }
 };
 
-// eights [j0, j1) * T of the sample for workgroup `chunk` of ns
-__device__ __forceinline__ void chunk_range(const GnShape &sh, long long L, int chunk, long long &j0, long long &j1) {
-  const long long J = ((L >> 3) + sh.T - 1) / sh.T, per = (J + sh.ns - 1) / sh.ns;
-  j0 = per * chunk < J ? per * chunk : J;
-  j1 = j0 + per < J ? j0 + per : J;
+// Steps of T units [j0, j1) of a sample for workgroup `chunk`: at most ns ranges, of at least GN_MIN_STEPS steps - a short
+// packed sample is not spread over the workgroups that the longest possible one would get.  ranges: those that are not
+// empty; the first one always counts (it also has the sample's last elements).
+__device__ __forceinline__ int chunk_ranges(const GnShape &sh, long long L, int N, long long &per) {
+  const long long J = (L / N + sh.T - 1) / sh.T, even = (J + sh.ns - 1) / sh.ns;
+  per = even < GN_MIN_STEPS ? GN_MIN_STEPS : even;
+  return J <= per ? 1 : (int)((J + per - 1) / per);
 }
 
 // Sums of x and x^2 per group from the lanes' columns and `tail`, single elements of them (zeros elsewhere); f as in
 // for_group_sums.
-template <typename F>
-__device__ __forceinline__ void reduce_groups(const GnShape &sh, const Lane &l, const Moments &m, const F8 &tail, double *lds,
+template <int N, typename F>
+__device__ __forceinline__ void reduce_groups(const GnShape &sh, const Lane &l, const Moments<N> &m, const Vec<N> &tail, double *lds,
                                               F f) {
-  if ((sh.cpg & 7) == 0) {  // a lane's eight channels are one group's (and a sample has no tail)
+  if (sh.cpg % N == 0) {  // a lane's channels are one group's (and a sample has no tail)
     double s1[1] = {0}, s2[1] = {0};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < N; ++k) {
       const double t = (double)m.n * m.mean[k];
       s1[0] += t;
       s2[0] += (double)m.m2[k] + t * m.mean[k];
     }
-    join_columns<1, double>(sh, l, s1, s2, lds, lds, lds + sh.P8);
-    for_group_sums(lds, lds + sh.P8, sh.G, sh.cpg >> 3, f);
+    join_columns<1, double>(sh, l, s1, s2, lds, lds, lds + sh.PL);
+    for_group_sums(lds, lds + sh.PL, sh.G, sh.cpg / N, f);
   } else {
-    double s1[8], s2[8];
+    double s1[N], s2[N];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < N; ++k) {
       const double t = (double)m.n * m.mean[k], e = tail.v[k];
       s1[k] = t + e;
       s2[k] = (double)m.m2[k] + t * m.mean[k] + e * e;
     }
-    join_columns<8, double>(sh, l, s1, s2, lds, lds, lds + sh.C);
+    join_columns<N, double>(sh, l, s1, s2, lds, lds, lds + sh.C);
     for_group_sums(lds, lds + sh.C, sh.G, sh.cpg, f);
   }
 }
 
 extern __shared__ __attribute__((aligned(16))) unsigned char gn_lds[];
 
-template <typename T>
+// the units of a workgroup: [first, end) in steps of T, and whether this lane has the sample's last L mod N elements
+struct Range {
+  long long base, v, end, last;
+  int tail;
+  bool none;
+};
+template <int N>
+__device__ __forceinline__ Range range_of(const GnShape &sh, int s, int chunk) {
+  Range g;
+  long long lo, hi, per;
+  sample_rows(sh, s, lo, hi);
+  const long long L = (hi - lo) * sh.C;
+  g.none = chunk >= chunk_ranges(sh, L, N, per);
+  g.base = lo * sh.C;
+  g.last = L / N;
+  g.v = per * chunk * sh.T + threadIdx.x;
+  g.end = per * (chunk + 1) * sh.T < g.last ? per * (chunk + 1) * sh.T : g.last;
+  g.tail = chunk == 0 && (int)threadIdx.x == (int)(g.last % sh.T) ? (int)(L % N) : 0;
+  return g;
+}
+
+template <typename T, bool NT>
 __global__ __launch_bounds__(1024) void gn_stats_kernel(GnArgs a) {
+  constexpr int N = Unit<T>::N;
   const GnShape &sh = a.sh;
   const int s = (int)blockIdx.y, chunk = (int)blockIdx.x;
   const Lane l = lane_place(sh);
-  long long lo, hi, j0, j1;
-  sample_rows(sh, s, lo, hi);
-  const long long L = (hi - lo) * sh.C, NV = L >> 3;
-  chunk_range(sh, L, chunk, j0, j1);
-  const T *x = (const T *)a.x + lo * sh.C;
-  Moments m;
+  const Range g = range_of<N>(sh, s, chunk);
+  if (g.none) return;
+  const T *x = (const T *)a.x + g.base;
+  Moments<N> m;
   m.clear();
+  VecOf<T> tail = {};
   if (l.on) {
-    long long v = j0 * sh.T + threadIdx.x;
-    const long long end = j1 * sh.T < NV ? j1 * sh.T : NV, step = sh.T;
-    for (; v + 3 * step < end; v += 4 * step) {
-      const Raw8<T> r0 = load_raw8(x + 8 * v), r1 = load_raw8(x + 8 * (v + step)), r2 = load_raw8(x + 8 * (v + 2 * step)),
-                    r3 = load_raw8(x + 8 * (v + 3 * step));
+    long long v = g.v;
+    const long long step = sh.T;
+    for (; v + 3 * step < g.end; v += 4 * step) {
+      const Raw<T> r0 = load_raw<NT>(x + N * v), r1 = load_raw<NT>(x + N * (v + step)), r2 = load_raw<NT>(x + N * (v + 2 * step)),
+                   r3 = load_raw<NT>(x + N * (v + 3 * step));
       m.add4(widen(r0), widen(r1), widen(r2), widen(r3));
     }
-    for (; v < end; v += step) m.add1(load8(x + 8 * v));
+    for (; v < g.end; v += step) m.add1(load_unit(x + N * v));
+    if (g.tail) tail = load_part(x + N * g.last, g.tail);
   }
-  F8 tail = {};  // the sample's last L mod 8 elements
-  if (chunk == 0 && (L & 7) && l.on && (int)threadIdx.x == (int)(NV % sh.T)) tail = load_tail(x + 8 * NV, (int)(L & 7));
   double *out = a.gpart + ((long long)s * sh.ns + chunk) * sh.G * 2;
-  reduce_groups(sh, l, m, tail, reinterpret_cast<double *>(gn_lds), [&](int g, double t1, double t2) {
+  reduce_groups<N>(sh, l, m, tail, reinterpret_cast<double *>(gn_lds), [&](int g, double t1, double t2) {
     out[2 * g] = t1;
     out[2 * g + 1] = t2;
   });
@@ -280,11 +331,16 @@ __device__ __forceinline__ void finish_group(double t1, double t2, double n, flo
 }
 
 // one wave per (sample, group)
+template <int N>
 __global__ __launch_bounds__(64) void gn_finish_kernel(GnArgs a) {
   const GnShape &sh = a.sh;
   const int g = (int)blockIdx.x, s = (int)blockIdx.y, lane = (int)threadIdx.x;
+  long long lo, hi, per;
+  sample_rows(sh, s, lo, hi);
+  const int ranges = chunk_ranges(sh, (hi - lo) * sh.C, N, per);
   double t1 = 0, t2 = 0;
-  for (int c = lane; c < sh.ns; c += 64) {
+#pragma unroll 4
+  for (int c = lane; c < ranges; c += 64) {
     const double *p = a.gpart + (((long long)s * sh.ns + c) * sh.G + g) * 2;
     t1 += p[0];
     t2 += p[1];
@@ -292,8 +348,6 @@ __global__ __launch_bounds__(64) void gn_finish_kernel(GnArgs a) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) t1 += __shfl_xor(t1, o), t2 += __shfl_xor(t2, o);
   if (lane == 0) {
-    long long lo, hi;
-    sample_rows(sh, s, lo, hi);
     float mean = 0, rstd = 0;
     if (hi > lo) finish_group(t1, t2, (double)(hi - lo) * sh.cpg, a.eps, mean, rstd);
     a.mean[(long long)s * sh.G + g] = mean;
@@ -301,16 +355,17 @@ __global__ __launch_bounds__(64) void gn_finish_kernel(GnArgs a) {
   }
 }
 
-// Eight elements from flat index i (of the whole tensor) through norm, activation and dropout; res: zeros where there is
-// no residual.
-struct Coef {  // of a lane's eight channels; a = rstd * w
-  float mean[8], rstd[8], a[8], b[8];
+// A unit from flat index i (of the whole tensor) through norm, activation and dropout; res: zeros where there is no residual.
+template <int N>
+struct Coef {  // of a lane's channels; a = rstd * w
+  float mean[N], rstd[N], a[N], b[N];
 };
+template <int N>
 __device__ __forceinline__ void load_coef(const GnShape &sh, const float *w, const float *b, int p, const float *mean,
-                                          const float *rstd, Coef &co) {
-  int c = channel0(sh, p);
+                                          const float *rstd, Coef<N> &co) {
+  int c = channel0<N>(sh, p);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < N; ++k) {
     const int g = c / sh.cpg;
     co.mean[k] = mean[g];
     co.rstd[k] = rstd[g];
@@ -319,32 +374,32 @@ __device__ __forceinline__ void load_coef(const GnShape &sh, const float *w, con
     c = next_channel(sh, c);
   }
 }
-template <int ACT>
-__device__ __forceinline__ F8 norm_act(const GnArgs &a, const Coef &co, const RowRng &rng, const F8 &x, const F8 &res,
-                                       long long i) {
-  F8 y;
+template <int ACT, int N>
+__device__ __forceinline__ Vec<N> norm_act(const GnArgs &a, const Coef<N> &co, const RowRng &rng, const Vec<N> &x, const Vec<N> &res,
+                                           long long i) {
+  Vec<N> y;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < N; ++k) {
     float z = (x.v[k] - co.mean[k]) * co.a[k] + co.b[k];
     z += res.v[k];
     y.v[k] = act_value<ACT>(z, a.slope);
   }
   if (a.q) {
-    const unsigned m = keep8(rng, (unsigned long long)i, a.q);
+    const unsigned m = keep_mask<N>(rng, (unsigned long long)i, a.q);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y.v[k] = (m >> k & 1) ? y.v[k] * a.scale : 0.0f;
+    for (int k = 0; k < N; ++k) y.v[k] = (m >> k & 1) ? y.v[k] * a.scale : 0.0f;
   }
   return y;
 }
 
-// g and xh of eight elements
-template <int ACT>
-__device__ __forceinline__ void grad_act(const GnArgs &a, const Coef &co, const RowRng &rng, const F8 &x, const F8 &res,
-                                         const F8 &dy, long long i, F8 &g, F8 &xh) {
-  unsigned m = 0xff;
-  if (a.q) m = keep8(rng, (unsigned long long)i, a.q);
+// g and xh of a unit
+template <int ACT, int N>
+__device__ __forceinline__ void grad_act(const GnArgs &a, const Coef<N> &co, const RowRng &rng, const Vec<N> &x, const Vec<N> &res,
+                                         const Vec<N> &dy, long long i, Vec<N> &g, Vec<N> &xh) {
+  unsigned m = (1u << N) - 1;
+  if (a.q) m = keep_mask<N>(rng, (unsigned long long)i, a.q);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < N; ++k) {
     const float d0 = x.v[k] - co.mean[k];
     xh.v[k] = d0 * co.rstd[k];
     float z = d0 * co.a[k] + co.b[k];
@@ -368,8 +423,9 @@ __device__ __forceinline__ void zero_outside(const GnShape &sh, T *y, T *y2, lon
   }
 }
 
-template <typename T, int ACT>
+template <typename T, int ACT, bool NT>
 __global__ __launch_bounds__(1024) void gn_apply_kernel(GnArgs a) {
+  constexpr int N = Unit<T>::N;
   const GnShape &sh = a.sh;
   const int s = (int)blockIdx.y, chunk = (int)blockIdx.x;
   const RowRng rng = load_rng(a.rng, a.seed, a.call);
@@ -382,43 +438,48 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(GnArgs a) {
     return;
   }
   const Lane l = lane_place(sh);
-  if (!l.on) return;
-  long long lo, hi, j0, j1;
-  sample_rows(sh, s, lo, hi);
-  const long long L = (hi - lo) * sh.C, NV = L >> 3, base = lo * sh.C;
-  chunk_range(sh, L, chunk, j0, j1);
-  const T *x = (const T *)a.x + base, *res = a.res ? (const T *)a.res + base : nullptr;
-  T *y = (T *)a.y + base;
-  Coef co;
-  load_coef(sh, a.w, a.b, l.p, a.mean + (long long)s * sh.G, a.rstd + (long long)s * sh.G, co);
-  const long long end = j1 * sh.T < NV ? j1 * sh.T : NV;
-  for (long long v = j0 * sh.T + threadIdx.x; v < end; v += sh.T) {
-    const F8 f = load8(x + 8 * v);
-    F8 r = {};
-    if (res) r = load8(res + 8 * v);
-    store8(y + 8 * v, norm_act<ACT>(a, co, rng, f, r, base + 8 * v));
+  const Range g = range_of<N>(sh, s, chunk);
+  if (g.none || !l.on) return;
+  const T *x = (const T *)a.x + g.base, *res = a.res ? (const T *)a.res + g.base : nullptr;
+  T *y = (T *)a.y + g.base;
+  Coef<N> co;
+  load_coef<N>(sh, a.w, a.b, l.p, a.mean + (long long)s * sh.G, a.rstd + (long long)s * sh.G, co);
+  const long long step = sh.T;
+  long long v = g.v;
+  for (; v + step < g.end; v += 2 * step) {   // two steps' loads in flight
+    const Raw<T> f0 = load_raw<NT>(x + N * v), f1 = load_raw<NT>(x + N * (v + step));
+    VecOf<T> r0 = {}, r1 = {};
+    if (res) r0 = load_unit<NT>(res + N * v), r1 = load_unit<NT>(res + N * (v + step));
+    store_unit<NT>(y + N * v, norm_act<ACT, N>(a, co, rng, widen(f0), r0, g.base + N * v));
+    store_unit<NT>(y + N * (v + step), norm_act<ACT, N>(a, co, rng, widen(f1), r1, g.base + N * (v + step)));
   }
-  if (chunk == 0 && (L & 7) && (int)threadIdx.x == (int)(NV % sh.T)) {  // the sample's last L mod 8 elements
-    const int n = (int)(L & 7);
-    F8 r = {};
-    if (res) r = load_tail(res + 8 * NV, n);
-    store_tail(y + 8 * NV, norm_act<ACT>(a, co, rng, load_tail(x + 8 * NV, n), r, base + 8 * NV), n);
+  if (v < g.end) {
+    VecOf<T> r = {};
+    if (res) r = load_unit(res + N * v);
+    store_unit(y + N * v, norm_act<ACT, N>(a, co, rng, load_unit(x + N * v), r, g.base + N * v));
+  }
+  if (g.tail) {
+    v = g.last;
+    VecOf<T> r = {};
+    if (res) r = load_part(res + N * v, g.tail);
+    store_part(y + N * v, norm_act<ACT, N>(a, co, rng, load_part(x + N * v, g.tail), r, g.base + N * v), g.tail);
   }
 }
 
 // ---- samples whose columns fit a workgroup's registers ----------------------------------------------------------------
 // A workgroup takes all rows of a sample and `sub` columns (whole groups: the fewest that make full 128-byte lines), keeps
-// its eights in registers between the statistics and the output, and reads them once.  The period is that of the columns:
-// place p of it is eight columns of a row, a step goes down T / P8 rows.  With C no multiple of 8 all columns are one
+// its units in registers between the statistics and the output, and reads them once.  The period is that of the columns:
+// place p of it is N columns of a row, a step goes down T / PL rows.  With C no multiple of N all columns are one
 // workgroup's, as one flat array.
 struct Sub {
-  GnShape sh;       // the columns as a tensor of their own: C, G, P8, T
+  GnShape sh;       // the columns as a tensor of their own: C, G, PL, T
   long long base;   // first element
   int c0, g0;
   int first, step;  // of a lane, in elements from base
-  int NV, tail;     // eights of the workgroup, elements behind the last of them
+  int NV, tail;     // units of the workgroup, elements behind the last of them
   double n;         // elements of a group
 };
+template <int N>
 __device__ __forceinline__ Sub sub_of(const GnArgs &a, int s, int part, const Lane &l) {
   Sub u;
   u.sh = a.sh;
@@ -431,27 +492,25 @@ __device__ __forceinline__ Sub sub_of(const GnArgs &a, int s, int part, const La
   u.sh.C = W;
   u.sh.G = W / a.sh.cpg;
   u.n = (double)rows * a.sh.cpg;
-  if (W & 7) {
-    u.NV = rows * W >> 3;
-    u.tail = rows * W & 7;
-    u.first = 8 * (int)threadIdx.x;
-    u.step = 8 * a.sh.T;
+  if (W % N) {
+    u.NV = rows * W / N;
+    u.tail = rows * W % N;
+    u.first = N * (int)threadIdx.x;
+    u.step = N * a.sh.T;
   } else {
-    u.NV = rows * a.sh.P8;
+    u.NV = rows * a.sh.PL;
     u.tail = 0;
-    u.first = l.r * a.sh.C + 8 * l.p;
-    u.step = a.sh.T / a.sh.P8 * a.sh.C;
+    u.first = l.r * a.sh.C + N * l.p;
+    u.step = a.sh.T / a.sh.PL * a.sh.C;
   }
   return u;
 }
-// Eights per lane: 32 registers of elements, what leaves 1024 lanes of 128 registers without spills.
-template <typename T>
-struct Held {
-  static constexpr int N = 16 / (int)sizeof(T);
-};
+// A lane holds 32 elements, what leaves 1024 lanes of 128 registers without spills.
+static constexpr int GN_HELD = 32;
 
 template <typename T, int ACT>
 __global__ __launch_bounds__(1024) void gn_small_kernel(GnArgs a) {
+  constexpr int N = Unit<T>::N, H = GN_HELD / N;
   const int s = (int)blockIdx.y, part = (int)blockIdx.x;
   const RowRng rng = load_rng(a.rng, a.seed, a.call);
   if (s == 0 && part == 0 && threadIdx.x == 0 && a.used) {
@@ -462,25 +521,24 @@ __global__ __launch_bounds__(1024) void gn_small_kernel(GnArgs a) {
     zero_outside<T>(a.sh, (T *)a.y, nullptr, part, gridDim.x);
     return;
   }
-  constexpr int H = Held<T>::N;
   const Lane l = lane_place(a.sh);
-  const Sub u = sub_of(a, s, part, l);
+  const Sub u = sub_of<N>(a, s, part, l);
   const T *x = (const T *)a.x + u.base, *res = a.res ? (const T *)a.res + u.base : nullptr;
   T *y = (T *)a.y + u.base;
   const bool owns_tail = u.tail && l.on && (int)threadIdx.x == u.NV % u.sh.T;
-  Raw8<T> held[H];
+  Raw<T> held[H];
 #pragma unroll
   for (int i = 0; i < H; ++i)
-    if (l.on && (int)threadIdx.x + i * u.sh.T < u.NV) held[i] = load_raw8(x + (u.first + i * u.step));
-  F8 t = {};
-  if (owns_tail) t = load_tail(x + 8 * u.NV, u.tail);
-  Moments m;
+    if (l.on && (int)threadIdx.x + i * u.sh.T < u.NV) held[i] = load_raw(x + (u.first + i * u.step));
+  VecOf<T> t = {};
+  if (owns_tail) t = load_part(x + N * u.NV, u.tail);
+  Moments<N> m;
   m.clear();
 #pragma unroll
   for (int i = 0; i < H; ++i)
     if (l.on && (int)threadIdx.x + i * u.sh.T < u.NV) m.add1(widen(held[i]));
   float *mean = a.mean + (long long)s * a.sh.G + u.g0, *rstd = a.rstd + (long long)s * a.sh.G + u.g0;
-  reduce_groups(u.sh, l, m, t, reinterpret_cast<double *>(gn_lds), [&](int g, double t1, double t2) {
+  reduce_groups<N>(u.sh, l, m, t, reinterpret_cast<double *>(gn_lds), [&](int g, double t1, double t2) {
     float mu = 0, r = 0;
     if (u.n > 0) finish_group(t1, t2, u.n, a.eps, mu, r);
     mean[g] = mu;
@@ -489,82 +547,100 @@ __global__ __launch_bounds__(1024) void gn_small_kernel(GnArgs a) {
   __threadfence_block();
   __syncthreads();
   if (!l.on) return;
-  Coef co;
-  load_coef(u.sh, a.w ? a.w + u.c0 : nullptr, a.b ? a.b + u.c0 : nullptr, l.p, mean, rstd, co);
+  Coef<N> co;
+  load_coef<N>(u.sh, a.w ? a.w + u.c0 : nullptr, a.b ? a.b + u.c0 : nullptr, l.p, mean, rstd, co);
 #pragma unroll
-  for (int i = 0; i < H; ++i)
+  for (int i = 0; i < H; ++i) {
     if ((int)threadIdx.x + i * u.sh.T < u.NV) {
       const int e = u.first + i * u.step;
-      F8 r = {};
-      if (res) r = load8(res + e);
-      store8(y + e, norm_act<ACT>(a, co, rng, widen(held[i]), r, u.base + e));
+      VecOf<T> r = {};
+      if (res) r = load_unit(res + e);
+      store_unit(y + e, norm_act<ACT, N>(a, co, rng, widen(held[i]), r, u.base + e));
     }
+    __builtin_amdgcn_sched_barrier(0);   // (one unit widened at a time)
+  }
   if (owns_tail) {
-    F8 r = {};
-    if (res) r = load_tail(res + 8 * u.NV, u.tail);
-    store_tail(y + 8 * u.NV, norm_act<ACT>(a, co, rng, t, r, u.base + 8 * u.NV), u.tail);
+    VecOf<T> r = {};
+    if (res) r = load_part(res + N * u.NV, u.tail);
+    store_part(y + N * u.NV, norm_act<ACT, N>(a, co, rng, t, r, u.base + N * u.NV), u.tail);
   }
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------
 
-template <typename T, int ACT>
+template <typename T, int ACT, bool NT>
 __global__ __launch_bounds__(1024) void gn_bwd_stats_kernel(GnArgs a) {
+  constexpr int N = Unit<T>::N;
   const GnShape &sh = a.sh;
   const int s = (int)blockIdx.y, chunk = (int)blockIdx.x;
   const RowRng rng = load_rng(a.rng, a.seed, a.call);
   const Lane l = lane_place(sh);
-  long long lo, hi, j0, j1;
-  sample_rows(sh, s, lo, hi);
-  const long long L = (hi - lo) * sh.C, NV = L >> 3, base = lo * sh.C;
-  chunk_range(sh, L, chunk, j0, j1);
-  const T *x = (const T *)a.x + base, *dy = (const T *)a.dy + base, *res = a.res ? (const T *)a.res + base : nullptr;
-  float sg[8] = {}, sx[8] = {};
+  const Range u = range_of<N>(sh, s, chunk);
+  if (u.none) return;
+  const T *x = (const T *)a.x + u.base, *dy = (const T *)a.dy + u.base, *res = a.res ? (const T *)a.res + u.base : nullptr;
+  float sg[N] = {}, sx[N] = {};
   if (l.on) {
-    Coef co;
-    load_coef(sh, a.w, a.b, l.p, a.mean + (long long)s * sh.G, a.rstd + (long long)s * sh.G, co);
-    const long long end = j1 * sh.T < NV ? j1 * sh.T : NV;
-    for (long long v = j0 * sh.T + threadIdx.x; v < end; v += sh.T) {
-      const F8 f = load8(x + 8 * v), d = load8(dy + 8 * v);
-      F8 r = {}, g, xh;
-      if (res) r = load8(res + 8 * v);
-      grad_act<ACT>(a, co, rng, f, r, d, base + 8 * v, g, xh);
+    Coef<N> co;
+    load_coef<N>(sh, a.w, a.b, l.p, a.mean + (long long)s * sh.G, a.rstd + (long long)s * sh.G, co);
+    auto add = [&](const VecOf<T> &f, const VecOf<T> &r, const VecOf<T> &d, long long v) {
+      VecOf<T> g, xh;
+      grad_act<ACT, N>(a, co, rng, f, r, d, u.base + N * v, g, xh);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sg[k] += g.v[k], sx[k] += g.v[k] * xh.v[k];
+      for (int k = 0; k < N; ++k) sg[k] += g.v[k], sx[k] += g.v[k] * xh.v[k];
+    };
+    const long long step = sh.T;
+    long long v = u.v;
+    for (; v + step < u.end; v += 2 * step) {
+      const Raw<T> f0 = load_raw<NT>(x + N * v), f1 = load_raw<NT>(x + N * (v + step)), d0 = load_raw<NT>(dy + N * v),
+                   d1 = load_raw<NT>(dy + N * (v + step));
+      VecOf<T> r0 = {}, r1 = {};
+      if (res) r0 = load_unit<NT>(res + N * v), r1 = load_unit<NT>(res + N * (v + step));
+      add(widen(f0), r0, widen(d0), v);
+      add(widen(f1), r1, widen(d1), v + step);
     }
-    if (chunk == 0 && (L & 7) && (int)threadIdx.x == (int)(NV % sh.T)) {
-      const int n = (int)(L & 7);
-      F8 r = {}, g, xh;
-      if (res) r = load_tail(res + 8 * NV, n);
-      grad_act<ACT>(a, co, rng, load_tail(x + 8 * NV, n), r, load_tail(dy + 8 * NV, n), base + 8 * NV, g, xh);
+    if (v < u.end) {
+      VecOf<T> r = {};
+      if (res) r = load_unit(res + N * v);
+      add(load_unit(x + N * v), r, load_unit(dy + N * v), v);
+    }
+    if (u.tail) {
+      v = u.last;
+      VecOf<T> r = {}, g, xh;
+      if (res) r = load_part(res + N * v, u.tail);
+      grad_act<ACT, N>(a, co, rng, load_part(x + N * v, u.tail), r, load_part(dy + N * v, u.tail), u.base + N * v, g, xh);
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k < n) sg[k] += g.v[k], sx[k] += g.v[k] * xh.v[k];
+      for (int k = 0; k < N; ++k)
+        if (k < u.tail) sg[k] += g.v[k], sx[k] += g.v[k] * xh.v[k];
     }
   }
   float *lds = reinterpret_cast<float *>(gn_lds);
-  join_columns<8, float>(sh, l, sg, sx, lds, lds, lds + sh.C);
+  join_columns<N, float>(sh, l, sg, sx, lds, lds, lds + sh.C);
   float2 *out = reinterpret_cast<float2 *>(a.cpart) + ((long long)s * sh.ns + chunk) * sh.C;
   for (int c = (int)threadIdx.x; c < sh.C; c += (int)blockDim.x) out[c] = make_float2(lds[c], lds[sh.C + c]);
 }
 
-// The workgroups' sums of a sample, joined: 32 channels x 8 lanes over the workgroups, in 64 bits.
+// The workgroups' sums of a sample, joined: 8 channels x 32 lanes over the workgroups, in 64 bits.
+template <int N>
 __global__ __launch_bounds__(256) void gn_bwd_join_kernel(GnArgs a) {
-  __shared__ double part[2][8][32];
+  __shared__ double part[32][8][2];
   const GnShape &sh = a.sh;
-  const int s = (int)blockIdx.y, c = (int)blockIdx.x * 32 + ((int)threadIdx.x & 31), q = (int)threadIdx.x >> 5;
+  long long lo, hi, per;
+  sample_rows(sh, (int)blockIdx.y, lo, hi);
+  const int ranges = chunk_ranges(sh, (hi - lo) * sh.C, N, per);
+  const int s = (int)blockIdx.y, i = (int)threadIdx.x & 7, c = (int)blockIdx.x * 8 + i, q = (int)threadIdx.x >> 3;
   double s0 = 0, s1 = 0;
   if (c < sh.C)
-    for (int i = q; i < sh.ns; i += 8) {
-      const float2 f = reinterpret_cast<const float2 *>(a.cpart)[((long long)s * sh.ns + i) * sh.C + c];
+#pragma unroll 4
+    for (int k = q; k < ranges; k += 32) {
+      const float2 f = reinterpret_cast<const float2 *>(a.cpart)[((long long)s * sh.ns + k) * sh.C + c];
       s0 += f.x;
       s1 += f.y;
     }
-  part[0][q][threadIdx.x & 31] = s0;
-  part[1][q][threadIdx.x & 31] = s1;
+  part[q][i][0] = s0;
+  part[q][i][1] = s1;
   __syncthreads();
   if (q == 0 && c < sh.C) {
-    for (int i = 1; i < 8; ++i) s0 += part[0][i][threadIdx.x], s1 += part[1][i][threadIdx.x];
+    for (int k = 1; k < 32; ++k) s0 += part[k][i][0], s1 += part[k][i][1];
     reinterpret_cast<float2 *>(a.csum)[(long long)s * sh.C + c] = make_float2((float)s0, (float)s1);
   }
 }
@@ -611,15 +687,18 @@ __device__ __forceinline__ void group_terms(const GnArgs &a, float *v0, float *v
   __syncthreads();
 }
 
-__device__ __forceinline__ F8 grad_x(const Coef &co, const F8 &g, const F8 &xh, const float (&c1)[8], const float (&c2)[8]) {
-  F8 o;
+template <int N>
+__device__ __forceinline__ Vec<N> grad_x(const Coef<N> &co, const Vec<N> &g, const Vec<N> &xh, const float (&c1)[N],
+                                         const float (&c2)[N]) {
+  Vec<N> o;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) o.v[k] = co.a[k] * g.v[k] - c1[k] - xh.v[k] * c2[k];
+  for (int k = 0; k < N; ++k) o.v[k] = co.a[k] * g.v[k] - c1[k] - xh.v[k] * c2[k];
   return o;
 }
 
-template <typename T, int ACT>
+template <typename T, int ACT, bool NT>
 __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnArgs a) {
+  constexpr int N = Unit<T>::N;
   const GnShape &sh = a.sh;
   const int s = (int)blockIdx.y, chunk = (int)blockIdx.x;
   if (s == sh.S) {
@@ -629,11 +708,11 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnArgs a) {
   }
   const RowRng rng = load_rng(a.rng, a.seed, a.call);
   const Lane l = lane_place(sh);
-  long long lo, hi, j0, j1;
+  const Range u = range_of<N>(sh, s, chunk);
+  if (u.none) return;
+  long long lo, hi;
   sample_rows(sh, s, lo, hi);
-  const long long L = (hi - lo) * sh.C, NV = L >> 3, base = lo * sh.C;
-  chunk_range(sh, L, chunk, j0, j1);
-  if (L == 0) return;
+  if (hi == lo) return;
   float *v0 = reinterpret_cast<float *>(gn_lds), *v1 = v0 + sh.C, *k1 = v1 + sh.C, *k2 = k1 + sh.G;
   for (int c = (int)threadIdx.x; c < sh.C; c += (int)blockDim.x) {
     const float2 f = reinterpret_cast<const float2 *>(a.csum)[(long long)s * sh.C + c];
@@ -642,96 +721,118 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnArgs a) {
   }
   group_terms(a, v0, v1, k1, k2, (double)(hi - lo) * sh.cpg);
   if (!l.on) return;
-  Coef co;
-  load_coef(sh, a.w, a.b, l.p, a.mean + (long long)s * sh.G, a.rstd + (long long)s * sh.G, co);
-  float c1[8], c2[8];
-  int c = channel0(sh, l.p);
+  Coef<N> co;
+  load_coef<N>(sh, a.w, a.b, l.p, a.mean + (long long)s * sh.G, a.rstd + (long long)s * sh.G, co);
+  float c1[N], c2[N];
+  int c = channel0<N>(sh, l.p);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < N; ++k) {
     c1[k] = co.rstd[k] * k1[c / sh.cpg];
     c2[k] = co.rstd[k] * k2[c / sh.cpg];
     c = next_channel(sh, c);
   }
-  const T *x = (const T *)a.x + base, *dy = (const T *)a.dy + base, *res = a.res ? (const T *)a.res + base : nullptr;
-  T *dx = (T *)a.dx + base, *dres = a.dres ? (T *)a.dres + base : nullptr;
-  const long long end = j1 * sh.T < NV ? j1 * sh.T : NV;
-  for (long long v = j0 * sh.T + threadIdx.x; v < end; v += sh.T) {
-    const F8 f = load8(x + 8 * v), d = load8(dy + 8 * v);
-    F8 r = {}, g, xh;
-    if (res) r = load8(res + 8 * v);
-    grad_act<ACT>(a, co, rng, f, r, d, base + 8 * v, g, xh);
-    store8(dx + 8 * v, grad_x(co, g, xh, c1, c2));
-    if (dres) store8(dres + 8 * v, g);
+  const T *x = (const T *)a.x + u.base, *dy = (const T *)a.dy + u.base, *res = a.res ? (const T *)a.res + u.base : nullptr;
+  T *dx = (T *)a.dx + u.base, *dres = a.dres ? (T *)a.dres + u.base : nullptr;
+  auto put = [&](const VecOf<T> &f, const VecOf<T> &r, const VecOf<T> &d, long long v) {
+    VecOf<T> g, xh;
+    grad_act<ACT, N>(a, co, rng, f, r, d, u.base + N * v, g, xh);
+    store_unit<NT>(dx + N * v, grad_x<N>(co, g, xh, c1, c2));
+    if (dres) store_unit<NT>(dres + N * v, g);
+  };
+  const long long step = sh.T;
+  long long v = u.v;
+  for (; v + step < u.end; v += 2 * step) {
+    const Raw<T> f0 = load_raw<NT>(x + N * v), f1 = load_raw<NT>(x + N * (v + step)), d0 = load_raw<NT>(dy + N * v),
+                 d1 = load_raw<NT>(dy + N * (v + step));
+    VecOf<T> r0 = {}, r1 = {};
+    if (res) r0 = load_unit<NT>(res + N * v), r1 = load_unit<NT>(res + N * (v + step));
+    put(widen(f0), r0, widen(d0), v);
+    put(widen(f1), r1, widen(d1), v + step);
   }
-  if (chunk == 0 && (L & 7) && (int)threadIdx.x == (int)(NV % sh.T)) {
-    const int n = (int)(L & 7);
-    F8 r = {}, g, xh;
-    if (res) r = load_tail(res + 8 * NV, n);
-    grad_act<ACT>(a, co, rng, load_tail(x + 8 * NV, n), r, load_tail(dy + 8 * NV, n), base + 8 * NV, g, xh);
-    store_tail(dx + 8 * NV, grad_x(co, g, xh, c1, c2), n);
-    if (dres) store_tail(dres + 8 * NV, g, n);
+  if (v < u.end) {
+    VecOf<T> r = {};
+    if (res) r = load_unit(res + N * v);
+    put(load_unit(x + N * v), r, load_unit(dy + N * v), v);
+  }
+  if (u.tail) {
+    v = u.last;
+    VecOf<T> r = {}, g, xh;
+    if (res) r = load_part(res + N * v, u.tail);
+    grad_act<ACT, N>(a, co, rng, load_part(x + N * v, u.tail), r, load_part(dy + N * v, u.tail), u.base + N * v, g, xh);
+    store_part(dx + N * v, grad_x<N>(co, g, xh, c1, c2), u.tail);
+    if (dres) store_part(dres + N * v, g, u.tail);
   }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
 
-static int gcd8(int c) { return c % 8 == 0 ? 8 : c % 4 == 0 ? 4 : c % 2 == 0 ? 2 : 1; }
+static int unit_of(int dtype) { return dtype == GB_T_F32 ? 4 : 8; }
+static int period(int c, int unit) {   // lanes: c / gcd(c, unit)
+  while (unit > 1 && c % unit) unit /= 2;
+  return c / unit;
+}
 
 struct GnPlan {
-  int block, P8, T, ns;
+  int block, PL, T;
+  int ns;    // workgroups per sample
   int sub;   // columns per workgroup of the one-pass kernel; 0: the sample is read twice
   size_t lds, ws;
 };
 
-static int lds_tree(int T, int P8) {  // join_columns: most lanes that give theirs away at a step (RL - h first, then h / 2, ...)
-  const int RL = T / P8;
+static int lds_tree(int T, int PL) {  // join_columns: most lanes that give theirs away at a step (RL - h first, then h / 2, ...)
+  const int RL = T / PL;
   int h = 1;
   while (2 * h < RL) h *= 2;
-  return RL > 1 ? (RL - h > h / 2 ? RL - h : h / 2) * P8 : 0;
+  return RL > 1 ? (RL - h > h / 2 ? RL - h : h / 2) * PL : 0;
+}
+
+// Workgroups per sample: as many as are resident at once (waves per SIMD by the kernel's registers), so that there is no
+// last round of a few (4 x 131072 x 128 fp32 statistics: 68 us with 2048 workgroups where 1536 fit, 45 with 2048 where 2048
+// do and streamed loads).  Packed samples may be of very different lengths and are cut twice as fine.
+static int spread(const GbGroupNorm *n, long long steps, long long resident) {
+  const long long most = resident * (n->offsets ? 2 : 1) / n->samples, want = (steps + GN_MIN_STEPS - 1) / GN_MIN_STEPS;
+  const long long ns = want < most ? want : most;
+  return (int)(ns < 1 ? 1 : ns);
 }
 
 static GnPlan gn_plan(const GbGroupNorm *n, bool backward) {
   GnPlan p;
   const long long longest = n->offsets ? n->rows : n->rows / n->samples;
-  const int C = n->channels, cpg = C / n->groups, size = n->dtype == GB_T_F32 ? 4 : 2;
+  const int C = n->channels, cpg = C / n->groups, N = unit_of(n->dtype), size = 16 / N;
   p.sub = 0;
   if (!backward) {
     // The one-pass kernel wherever a sample's columns fit: no second read and one launch instead of three.  Columns: all
-    // of them when C is no multiple of 8, else the fewest whole groups that divide C into full 128-byte lines of eights.
+    // of them when C is no multiple of N, else the fewest whole groups that divide C into full 128-byte lines of units.
     int sub = C;
-    if (C % 8 == 0)
+    if (C % N == 0)
       for (int gs = 1; gs <= n->groups; ++gs)
-        if (n->groups % gs == 0 && gs * cpg % 8 == 0 && gs * cpg * size >= 128) {
+        if (n->groups % gs == 0 && gs * cpg % N == 0 && gs * cpg * size >= 128) {
           sub = gs * cpg;
           break;
         }
-    const int P8 = sub / gcd8(sub), T = P8 <= 1024 ? 1024 / P8 * P8 : 0;
-    if (T && longest * sub / 8 < (long long)T * (16 / size)) {
+    const int PL = period(sub, N), T = PL <= 1024 ? 1024 / PL * PL : 0;
+    if (T && longest * sub / N < (long long)T * (GN_HELD / N)) {
       p.sub = sub;
-      p.P8 = P8;
-      // (lanes for one eight each, in whole waves: latency counts more than what a lane could hold)
-      const long long eights = (longest * sub + 7) / 8;
-      p.block = P8 <= 256 && eights <= 256 ? 256 : P8 <= 512 && eights <= 512 ? 512 : 1024;
+      p.PL = PL;
+      // (lanes for one unit each, in whole waves: latency counts more than what a lane could hold)
+      const long long units = (longest * sub + N - 1) / N;
+      p.block = PL <= 256 && units <= 256 ? 256 : PL <= 512 && units <= 512 ? 512 : 1024;
       p.ns = C / sub;
     }
   }
   if (!p.sub) {
-    // Lanes: 256 where a period fits (more workgroups per CU to change between), else 512 or 1024.  A sample is spread
-    // over enough workgroups that a lane meets ~16 eights (64 KB of fp32 per workgroup keep the joining of the sums below
-    // 2 % of the pass) but the device has ~2048 in all; packed samples may be of very different lengths and are cut finer.
-    p.P8 = C / gcd8(C);
-    p.block = p.P8 <= 256 ? 256 : p.P8 <= 512 ? 512 : 1024;
-    const int T = p.block / p.P8 * p.P8;
-    const long long eights = (longest * C + 7) / 8, steps = (eights + T - 1) / T;
-    long long ns = (steps + 15) / 16;
-    const long long fill = n->offsets ? 8192 : 2048, most = (fill + n->samples - 1) / n->samples;
-    if (ns > most) ns = most;
-    p.ns = (int)(ns < 1 ? 1 : ns);
+    // Lanes: 256 where a period fits (more workgroups per CU to change between), else 512 or 1024.
+    p.PL = period(C, N);
+    p.block = p.PL <= 256 ? 256 : p.PL <= 512 ? 512 : 1024;
+    const int T = p.block / p.PL * p.PL;
+    const long long units = (longest * C + N - 1) / N, steps = (units + T - 1) / T;
+    const int waves = N == 4 ? (backward ? 5 : 8) : (backward ? 4 : 6);   // per SIMD, by the kernels' registers
+    p.ns = spread(n, steps, 256ll * 4 * waves * 64 / p.block);
   }
-  p.T = p.block / p.P8 * p.P8;
+  p.T = p.block / p.PL * p.PL;
   const size_t cell = backward ? sizeof(float) : sizeof(double);
-  const int K = !backward && cpg % 8 == 0 ? 1 : 8;
-  const size_t tree = (size_t)lds_tree(p.T, p.P8) * 2 * K * cell, flat = (size_t)(K == 1 ? p.P8 : p.sub ? p.sub : C) * 2 * cell;
+  const int K = !backward && cpg % N == 0 ? 1 : N;
+  const size_t tree = (size_t)lds_tree(p.T, p.PL) * 2 * K * cell, flat = (size_t)(K == 1 ? p.PL : p.sub ? p.sub : C) * 2 * cell;
   p.lds = tree > flat ? tree : flat;
   if (backward) {
     const size_t apply = (size_t)(C + n->groups) * 2 * sizeof(float);
@@ -749,7 +850,7 @@ static int gn_bad(const GbGroupNorm *n) {
   if (!n || n->rows < 0 || n->samples <= 0 || n->channels <= 0 || n->groups <= 0 || n->channels % n->groups) return GB_EINVAL;
   if (!known_type(n->dtype) || n->act < 0 || n->act > GB_ACT_GELU || n->q < 0 || n->q > 65536 || !(n->eps >= 0)) return GB_EINVAL;
   if (!n->offsets && n->rows % n->samples) return GB_EINVAL;
-  if (n->channels > GN_MAX_C || n->channels / gcd8(n->channels) > 1024 || n->samples > 65534) return GB_ERANGE;
+  if (n->channels > GN_MAX_C || period(n->channels, unit_of(n->dtype)) > 1024 || n->samples > 65534) return GB_ERANGE;
   if (n->rows > (1ll << 62) / n->channels) return GB_ERANGE;
   if ((reinterpret_cast<uintptr_t>(n->offsets) | reinterpret_cast<uintptr_t>(n->rng) | reinterpret_cast<uintptr_t>(n->used)) % 8)
     return GB_EINVAL;
@@ -778,7 +879,7 @@ static GnArgs gn_args(const GbGroupNorm *n, const GnPlan &p) {
   a.sh.C = n->channels;
   a.sh.G = n->groups;
   a.sh.cpg = n->channels / n->groups;
-  a.sh.P8 = p.P8;
+  a.sh.PL = p.PL;
   a.sh.T = p.T;
   a.sh.ns = p.ns;
   a.sub = p.sub;
@@ -821,6 +922,7 @@ extern "C" int gb_group_norm_fwd(const GbGroupNorm *n, void *y, void *ws, long l
   a.y = y;
   a.gpart = (double *)ws;
   hipStream_t st = as_stream(stream);
+  const bool nt = streams(n->rows * n->channels * (16 / unit_of(n->dtype)));
   const dim3 all((unsigned)p.ns, (unsigned)(n->samples + (n->offsets ? 1 : 0)));
   return with_type_and_act(n, [&](auto z, auto act) {
     typedef decltype(z) T;
@@ -828,9 +930,16 @@ extern "C" int gb_group_norm_fwd(const GbGroupNorm *n, void *y, void *ws, long l
     if (p.sub) {
       gn_small_kernel<T, ACT><<<all, p.block, p.lds, st>>>(a);
     } else {
-      gn_stats_kernel<T><<<dim3((unsigned)p.ns, (unsigned)n->samples), p.block, p.lds, st>>>(a);
-      gn_finish_kernel<<<dim3((unsigned)n->groups, (unsigned)n->samples), 64, 0, st>>>(a);
-      gn_apply_kernel<T, ACT><<<all, p.block, 0, st>>>(a);
+      const dim3 grid((unsigned)p.ns, (unsigned)n->samples);
+      if (nt)
+        gn_stats_kernel<T, true><<<grid, p.block, p.lds, st>>>(a);
+      else
+        gn_stats_kernel<T, false><<<grid, p.block, p.lds, st>>>(a);
+      gn_finish_kernel<Unit<T>::N><<<dim3((unsigned)n->groups, (unsigned)n->samples), 64, 0, st>>>(a);
+      if (nt)
+        gn_apply_kernel<T, ACT, true><<<all, p.block, 0, st>>>(a);
+      else
+        gn_apply_kernel<T, ACT, false><<<all, p.block, 0, st>>>(a);
     }
     return check_launch("gb_group_norm_fwd");
   });
@@ -853,12 +962,20 @@ extern "C" int gb_group_norm_bwd(const GbGroupNorm *n, const void *dy, void *dx,
   a.cpart = (float *)ws;
   a.csum = a.cpart + (size_t)n->samples * p.ns * n->channels * 2;
   hipStream_t st = as_stream(stream);
+  const bool nt = streams(n->rows * n->channels * (16 / unit_of(n->dtype)));
   return with_type_and_act(n, [&](auto z, auto act) {
     typedef decltype(z) T;
     constexpr int ACT = decltype(act)::value;
-    gn_bwd_stats_kernel<T, ACT><<<dim3((unsigned)p.ns, (unsigned)n->samples), p.block, p.lds, st>>>(a);
-    gn_bwd_join_kernel<<<dim3((unsigned)((n->channels + 31) / 32), (unsigned)n->samples), 256, 0, st>>>(a);
-    gn_bwd_apply_kernel<T, ACT><<<dim3((unsigned)p.ns, (unsigned)n->samples + 1), p.block, p.lds, st>>>(a);
+    const dim3 grid((unsigned)p.ns, (unsigned)n->samples), all((unsigned)p.ns, (unsigned)n->samples + 1);
+    if (nt)
+      gn_bwd_stats_kernel<T, ACT, true><<<grid, p.block, p.lds, st>>>(a);
+    else
+      gn_bwd_stats_kernel<T, ACT, false><<<grid, p.block, p.lds, st>>>(a);
+    gn_bwd_join_kernel<Unit<T>::N><<<dim3((unsigned)((n->channels + 7) / 8), (unsigned)n->samples), 256, 0, st>>>(a);
+    if (nt)
+      gn_bwd_apply_kernel<T, ACT, true><<<all, p.block, p.lds, st>>>(a);
+    else
+      gn_bwd_apply_kernel<T, ACT, false><<<all, p.block, p.lds, st>>>(a);
     return check_launch("gb_group_norm_bwd");
   });
 }

@@ -234,27 +234,44 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
 
 # ---- products in 8-bit floats -----------------------------------------------------------------------------------------
 
-_FEW_ROWS, _FEW_CODES = 16, 16384     # gb_fp8_linear_few
+_WS_COLSUM, _WS_WGRAD, _WS_LINEAR, _KEEP, _SUM = 0, 1, 4, 1, 2     # GB_FP8_*
 
 
 def _up(n, m):
     return (n + m - 1) // m * m
 
 
+def _code_buffers(P, K, dev):
+    """Uninitialised (codes, scales) of rows (P, K), in one allocation."""
+    Kp, S = _up(K, 128), _up(_up(K, 128) // 128, 4)
+    both = torch.empty(P * (Kp + S) + 16, dtype=torch.uint8, device=dev)
+    at = _up(P * Kp, 16)
+    return both[:P * Kp].view(P, Kp), both[at:at + P * S].view(P, S)
+
+
 def _quantise_rows(x2, colsum=False):
     """(codes, scales, column sums | None) of rows (P, K)."""
     P, K = x2.shape
     dev = x2.device
-    codes = torch.empty((P, _up(K, 128)), dtype=torch.uint8, device=dev)
-    scales = torch.empty((P, _up(_up(K, 128) // 128, 4)), dtype=torch.uint8, device=dev)
-    sums = ws = None
-    size = 0
-    if colsum:
-        sums = torch.empty(K, dtype=torch.float32, device=dev)
-        ws, size = _fp8_workspace(0, P, K, 1, dev)
+    codes, scales = _code_buffers(P, K, dev)
+    sums = torch.empty(K, dtype=torch.float32, device=dev) if colsum else None
+    ws, size = _fp8_workspace(_WS_COLSUM, P, K, 1, dev) if colsum else (None, 0)
     _call("gb_fp8_quant_rows", dev, _lib.ptr(x2), _TYPES[x2.dtype], P, K, _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(sums),
           _lib.ptr(ws), size, _s(x2))
     return codes, scales, sums
+
+
+def _fp8_product(x2, w, w_scales, transposed, N, bias, keep, colsum):
+    """(y (P, N), codes, scales, column sums) of rows x2 and a weight's codes; what is not asked for is None."""
+    P, K = x2.shape
+    dev = x2.device
+    y = torch.empty((P, N), dtype=x2.dtype, device=dev)
+    codes, scales = _code_buffers(P, K, dev) if keep else (None, None)
+    sums = torch.empty(K, dtype=torch.float32, device=dev) if colsum else None
+    ws, size = _fp8_workspace(_WS_LINEAR + _KEEP * keep + _SUM * colsum, P, N, K, dev)
+    _call("gb_fp8_linear", dev, _lib.ptr(x2), _TYPES[x2.dtype], P, K, _lib.ptr(w), _lib.ptr(w_scales), transposed, N,
+          _lib.ptr(bias), _lib.ptr(y), _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(sums), _lib.ptr(ws), size, _s(x2))
+    return y, codes, scales, sums
 
 
 def _fp8_workspace(what, P, N, K, dev):
@@ -317,8 +334,6 @@ def _fp8_weight_tensor(what, w):
 class _Fp8Linear(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, held):
-        dev, st = x.device, _s(x)
-        P, K = x.shape
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         if held is None:
             weight = weight.contiguous()
@@ -328,40 +343,31 @@ class _Fp8Linear(Function):
             N, codes, codes_t, scales = held.out_features, held.codes, held.codes_t, held.scales
             if need_x and codes_t is None:
                 _refuse("fp8_linear", "gradients of the input need Fp8Weight.quantize(weight, input_gradients=True)")
-        y = torch.empty((P, N), dtype=x.dtype, device=dev)
-        xq = xs = None
-        if P <= _FEW_ROWS and P * codes.shape[1] <= _FEW_CODES and not need_w:
-            _call("gb_fp8_linear_few", dev, _lib.ptr(x), _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(bias), _lib.ptr(y),
-                  _TYPES[x.dtype], P, N, K, st)
-        else:
-            xq, xs, _ = _quantise_rows(x)
-            _call("gb_fp8_gemm", dev, _lib.ptr(xq), _lib.ptr(xs), _lib.ptr(codes), _lib.ptr(scales), 0, _lib.ptr(bias),
-                  _lib.ptr(y), _TYPES[x.dtype], P, N, K, st)
+        y, xq, xs, _ = _fp8_product(x, codes, scales, 0, N, bias, need_w, False)
         # one byte per element of x stays for the backward pass
-        ctx.save_for_backward(*((xq, xs) if need_w else (None, None)), *((codes_t, scales) if need_x else (None, None)))
-        ctx.dims = (P, N, K, None if held is not None else weight.dtype)
+        ctx.save_for_backward(xq, xs, *((codes_t, scales) if need_x else (None, None)))
+        ctx.dims = (N, x.shape[1], None if held is not None else weight.dtype)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         xq, xs, codes_t, scales = ctx.saved_tensors
-        P, N, K, wtype = ctx.dims
+        N, K, wtype = ctx.dims
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dy = dy.contiguous()
-        dev, st = dy.device, _s(dy)
         dx = dw = None
-        dq, ds, db = _quantise_rows(dy, colsum=need_b)
         if need_x:
-            dx = torch.empty((P, K), dtype=dy.dtype, device=dev)
-            _call("gb_fp8_gemm", dev, _lib.ptr(dq), _lib.ptr(ds), _lib.ptr(codes_t), _lib.ptr(scales), 1, None, _lib.ptr(dx),
-                  _TYPES[dy.dtype], P, K, N, st)
+            dx, dq, ds, db = _fp8_product(dy, codes_t, scales, 1, K, None, need_w, need_b)
+        else:
+            dq, ds, db = _quantise_rows(dy, colsum=need_b)
         if need_w:
+            dev, P = dy.device, dy.shape[0]
             dw = torch.empty((N, K), dtype=torch.float32, device=dev)
-            ws, size = _fp8_workspace(1, P, N, K, dev)
+            ws, size = _fp8_workspace(_WS_WGRAD, P, N, K, dev)
             _call("gb_fp8_wgrad", dev, _lib.ptr(dq), _lib.ptr(ds), _lib.ptr(xq), _lib.ptr(xs), _lib.ptr(dw), P, N, K,
-                  _lib.ptr(ws), size, st)
-            dw = dw.to(wtype)
+                  _lib.ptr(ws), size, _s(dy))
+            dw = dw if wtype == torch.float32 else dw.to(wtype)
         return dx, dw, db, None
 
 

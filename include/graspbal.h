@@ -726,7 +726,8 @@ int gb_dropout(const void *x, const void *residual, void *y, long long n, int dt
  *     numbers, sample s = rows [offsets[s], offsets[s+1]) - none for an empty one.  Rows outside every sample get zeros (y,
  *     dx, dresidual).  Values outside [0, rows] are brought into it.
  *   weight, bias: (channels) fp32 or NULL (1 / 0); mean, rstd: (samples, groups) fp32, written by _fwd, read by _bwd.
- *   channels: <= 4096, and channels / gcd(channels, 8) <= 1024 (odd counts up to 1024); samples <= 65534 - else GB_ERANGE.
+ *   channels: <= 4096, and channels / gcd(channels, 4 for fp32, 8 else) <= 1024 (odd counts up to 1024); samples <= 65534
+ *     - else GB_ERANGE.
  *   rng / seed / call / used: as gb_dropout; _bwd takes the pair that _fwd used (as rng or by value; `used` is not written).
  * _bwd: dx, dresidual (may be NULL) like x; dweight, dbias (channels) fp32 (either may be NULL), zeros' worth of rows give
  * zeros.  x, residual, act, q must be those of _fwd.  ws: gb_group_norm_workspace bytes, 16-byte aligned.  All sums are
@@ -757,23 +758,25 @@ int gb_group_norm_bwd(const GbGroupNorm *n, const void *dy, void *dx, void *dres
  * gb_fp8_quant_rows: x (P, K) -> codes, scales; colsum: NULL, or (K) fp32 = the columns' sums of x (ws: gb_fp8_workspace
  *   COLSUM with N = K).
  * gb_fp8_quant_weight: w (N, K) -> codes (N, Kp), block scales, and codes_t (K, Np) = the transposed codes unless NULL.
- * gb_fp8_gemm: y (P, N) = deq(a) deq(b)^T + bias, a (P, K) by rows, b (N, K) by blocks; transposed != 0: b is the codes_t of a
- *   weight (K, N) whose scales are given as they are.  fp32 y: codes multiplied as bf16 with fp32 sums (values below 2^-126
- *   count as zero); 16-bit y: 8-bit matrix instructions, whose steps add 64 or 128 products with about 14 bits below the
- *   largest before the fp32 sum.
- * gb_fp8_linear_few: the same from x itself for P <= 16 rows and P * Kp <= 16384 (else GB_ERANGE), in one launch.
+ * gb_fp8_linear: y (P, N) = deq(Q(x)) deq(w)^T + bias, x (P, K) in floats, w (N, K) by blocks; transposed != 0: w is the
+ *   codes_t of a weight (K, N) whose scales are given as they are.  fp32: codes multiplied as bf16 with fp32 sums (values
+ *   below 2^-126 count as zero); 16 bits: 8-bit matrix instructions, whose steps add 64 or 128 products with about 14 bits
+ *   below the largest before the fp32 sum.  codes, scales: NULL, or x's by rows are kept there; colsum: as above; bias:
+ *   (N) fp32 or NULL.  ws: gb_fp8_workspace LINEAR (+ KEEP with codes, + SUM with colsum), 16-byte aligned.
  * gb_fp8_wgrad: dw (N, K) fp32 = deq(dy)^T deq(x), dy (P, N) and x (P, K) by rows (ws: gb_fp8_workspace WGRAD); bf16 products
  *   with fp32 sums in a fixed order.                                                                                    */
 #define GB_FP8_WS_COLSUM 0
 #define GB_FP8_WS_WGRAD 1
+#define GB_FP8_WS_LINEAR 4
+#define GB_FP8_KEEP 1
+#define GB_FP8_SUM 2
 int gb_fp8_workspace(int what, long long P, int N, int K, long long *bytes);
 int gb_fp8_quant_rows(const void *x, int dtype, long long P, int K, void *codes, void *scales, float *colsum, void *ws,
                       long long ws_bytes, void *stream);
 int gb_fp8_quant_weight(const void *w, int dtype, int N, int K, void *codes, void *codes_t, void *scales, void *stream);
-int gb_fp8_gemm(const void *a, const void *a_scales, const void *b, const void *b_scales, int transposed, const float *bias,
-                void *y, int dtype, long long P, int N, int K, void *stream);
-int gb_fp8_linear_few(const void *x, const void *b, const void *b_scales, const float *bias, void *y, int dtype, int P, int N,
-                      int K, void *stream);
+int gb_fp8_linear(const void *x, int dtype, long long P, int K, const void *w, const void *w_scales, int transposed, int N,
+                  const float *bias, void *y, void *codes, void *scales, float *colsum, void *ws, long long ws_bytes,
+                  void *stream);
 int gb_fp8_wgrad(const void *dy, const void *dy_scales, const void *x, const void *x_scales, float *dw, long long P, int N, int K,
                  void *ws, long long ws_bytes, void *stream);
 

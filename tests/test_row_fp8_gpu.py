@@ -102,6 +102,26 @@ def test_many_rows():
         _check(dw, dq.t().contiguous(), xq.t().contiguous(), None, torch.float32, "dw", length=P)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("P,K,N", [(32768, 128, 128), (33001, 131, 100), (40003, 100, 255), (35000, 127, 470), (32770, 512, 90),
+                                   (120007, 256, 130)])
+def test_streamed_rows(P, K, N, dtype):
+    """Many rows and a weight that LDS holds: every column variant, one and several steps, odd widths, kept codes, sums."""
+    from graspbalance_amd import fused_rows
+    x, w, b, dy = (t.to("cuda:0") for t in _data(P, K, N, dtype))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = fused_rows.fp8_linear(*leaves)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    xq, wq, dq = (row_truth.in_8_bits(t.detach().cpu().double(), n) for t, n in ((x, 1), (w, 128), (dy, 1)))
+    _check(y, xq, wq, b.detach().cpu().double(), dtype, "y")
+    _check(dx, dq, wq.t().contiguous(), None, dtype, "dx")
+    _check(dw, dq.t().contiguous(), xq.t().contiguous(), None, torch.float32, "dw", length=P)
+    sums = dy.cpu().double().sum(0)
+    assert bool(((db.double().cpu() - sums).abs() <= 2.0 ** -24 * (256 * dy.cpu().double().abs().sum(0) + sums.abs())).all())
+    with torch.no_grad():      # nothing kept
+        assert torch.equal(fused_rows.fp8_linear(x, fused_rows.Fp8Weight.quantize(w), b), y)
+
+
 def _codes(x):
     from graspbalance_amd import fused_rows
     codes, scales, _ = fused_rows._quantise_rows(x)

@@ -112,7 +112,7 @@ def test_fp8_refuses_on_the_host():
             args[at] = value
             assert fn(*args) == rc, (fn.__name__, at, value)
     refused(L.gb_fp8_workspace, [1, 8, 8, 8, ctypes.byref(size)],
-            [(0, 2, -1), (0, -1, -1), (1, -1, -1), (2, 0, -1), (3, 0, -1), (4, None, -1), (1, 1 << 41, -3), (2, 1 << 23, -3)])
+            [(0, 2, -1), (0, 3, -1), (0, 8, -1), (0, -1, -1), (1, -1, -1), (2, 0, -1), (3, 0, -1), (4, None, -1), (1, 1 << 41, -3), (2, 1 << 23, -3)])
     assert size.value == -5
     refused(L.gb_fp8_quant_rows, [64, 0, 8, 8, 64, 64, None, None, 0, None],
             [(0, None, -1), (1, 3, -1), (2, -1, -1), (3, 0, -1), (4, None, -1), (4, 72, -1), (5, None, -1), (5, 68, -1),
@@ -120,16 +120,22 @@ def test_fp8_refuses_on_the_host():
     refused(L.gb_fp8_quant_weight, [64, 0, 8, 8, 64, 64, 64, None],
             [(0, None, -1), (1, 9, -1), (2, 0, -1), (3, -2, -1), (4, None, -1), (4, 65, -1), (5, 72, -1), (6, None, -1),
              (2, 1 << 23, -3)])
-    refused(L.gb_fp8_gemm, [64, 64, 64, 64, 0, None, 64, 0, 8, 8, 8, None],
-            [(0, None, -1), (0, 72, -1), (1, None, -1), (1, 72, -1), (2, None, -1), (2, 72, -1), (3, None, -1), (6, None, -1),
-             (7, 5, -1), (8, -1, -1), (9, 0, -1), (10, 0, -1), (9, 1 << 23, -3), (10, 1 << 23, -3), (8, 1 << 41, -3)])
-    refused(L.gb_fp8_linear_few, [64, 64, 64, None, 64, 0, 8, 8, 8, None],
-            [(0, None, -1), (1, None, -1), (1, 72, -1), (2, None, -1), (4, None, -1), (5, 7, -1), (6, -1, -1), (7, 0, -1),
-             (8, 0, -1), (6, 17, -3), (8, 2049, -3)])
+    ok = [64, 0, 8, 8, 64, 64, 0, 8, None, 64, None, None, None, 64, 1 << 20, None]
+    refused(L.gb_fp8_linear, ok,
+            [(0, None, -1), (1, 5, -1), (2, -1, -1), (3, 0, -1), (4, None, -1), (4, 72, -1), (5, None, -1), (7, 0, -1), (9, None, -1),
+             (10, 64, -1), (11, 64, -1), (13, 72, -1), (3, 1 << 23, -3), (7, 1 << 23, -3), (2, 1 << 41, -3)])
+    # a shape whose codes need room: none, too little, and room that is not needed where the caller keeps the codes
+    big = list(ok)
+    big[2], big[3], big[7] = 1000, 1024, 1024
+    assert L.gb_fp8_workspace(4, 1000, 1024, 1024, ctypes.byref(size)) == 0 and size.value == 1000 * (1024 + 8)
+    refused(L.gb_fp8_linear, big, [(13, None, -1), (14, size.value - 1, -1)])
+    assert L.gb_fp8_workspace(5, 1000, 1024, 1024, ctypes.byref(size)) == 0 and size.value == 0
+    big[12] = 64      # column sums
+    refused(L.gb_fp8_linear, big, [(14, 1000 * (1024 + 8) - 1, -1)])
     refused(L.gb_fp8_wgrad, [64, 64, 64, 64, 64, 8, 8, 8, None, 0, None],
             [(0, None, -1), (0, 72, -1), (1, None, -1), (2, None, -1), (2, 72, -1), (3, None, -1), (4, None, -1), (5, -1, -1),
              (6, 0, -1), (7, 0, -1), (7, 1 << 23, -3), (5, 100000, -1)])
-    assert L.gb_fp8_gemm(None, None, None, None, 0, None, None, 0, 0, 8, 8, None) == 0
+    assert L.gb_fp8_linear(None, 0, 0, 8, None, None, 0, 8, None, None, None, None, None, None, 0, None) == 0
     assert L.gb_fp8_workspace(0, 100, 30, 1, ctypes.byref(size)) == 0 and size.value == 2 * 30 * 4
 
 
