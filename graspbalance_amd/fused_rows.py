@@ -394,5 +394,7 @@ def fp8_linear(x, weight, bias=None):
     if x.dim() < 1 or x.shape[-1] != K:
         _refuse(what, "x must be (..., %d)" % K)
     bias = _channel_vector(what, "bias", bias, N, x)
+    if not torch.is_grad_enabled():   # (needs_input_grad does not know the grad mode: nothing would be kept in vain)
+        x, weight, bias = (t.detach() if isinstance(t, torch.Tensor) else t for t in (x, weight, bias))
     y = _Fp8Linear.apply(x.reshape(-1, K).contiguous(), None if held is not None else weight, bias, held)
     return y.view(x.shape[:-1] + (N,))
