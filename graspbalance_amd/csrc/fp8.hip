@@ -8,12 +8,13 @@
 // exact in bf16.
 //
 // Two inner products, chosen by the output's type:
-//   16-bit outputs: v_mfma_scale_f32_32x32x64_f8f6f4 - 4.7 PFLOP/s on this card, scales applied by the instruction.  It adds
+//   16-bit outputs: v_mfma_scale_f32_32x32x64_f8f6f4 - 4.0 PFLOP/s on this card with random codes (4.7 with zeros: the clock
+//     falls with the power), scales applied by the instruction.  It adds
 //     the products of a step with about 14 bits below the largest one (measured: 5e-5 of the result's norm for codes over
 //     the whole range, 0 where they span 2^4), then accumulates in fp32: a twentieth of bf16's half step, a quarter of
 //     fp16's.
 //   fp32 outputs: the codes are turned into bf16 (exact) in registers, scale included, and go through
-//     v_mfma_f32_32x32x16_bf16 (2.35 PFLOP/s; 8e-8 of the norm).
+//     v_mfma_f32_32x32x16_bf16 (1.76 PFLOP/s with random values; 8e-8 of the norm).
 #include "row_common.h"
 
 #pragma clang fp contract(on)
@@ -283,10 +284,10 @@ __device__ __forceinline__ void store_tiles(const f32x16 (&acc)[TM][TN], T *y, c
 // ---- tiles ----------------------------------------------------------------------------------------------------------
 // A workgroup of WM x WN waves, each with TM x TN tiles of 32 x 32, steps through the reduction 128 codes (one scale block)
 // at a time: two LDS stages filled by LDS-DMA, the next one in flight while this one is multiplied.  An LDS row is 128
-// codes, eight chunks of 16 bytes; chunk c of row r lies at place c ^ key(r) (the DMA writes lane-linearly, so the lane's
-// SOURCE is permuted), which spreads the eight rows that a group of lanes reads over all banks.  key(r) = r & 7 for rows of
-// X and (r >> 1) & 7 for rows of W: the tiles of W come in pairs and lane j of a pair takes rows 2j and 2j + 1, so that a
-// lane ends up with two neighbouring outputs.
+// codes, eight chunks of 16 bytes; chunk c of row r lies at place c ^ (r >> 1 & 7) (the DMA writes lane-linearly, so the
+// lane's SOURCE is permuted), which spreads the sixteen rows that are read in a cycle over all 64 banks.  The tiles of W come
+// in pairs, and lane j of a pair takes rows 2j and 2j + 1 of its 64, so that a lane ends up with two neighbouring outputs: in
+// LDS the even rows of each 64 come first.
 
 struct GemmArgs8 {
   const unsigned char *a, *a_scales, *b, *b_scales;  // a (P, Kp), b (N, Kp); a_scales (P, stride), b_scales by block
@@ -301,6 +302,9 @@ __device__ __forceinline__ void dma16(const unsigned char *src, unsigned char *l
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)lds,
                                    16, 0, 0);
 }
+
+// the row of W at place `at` of LDS
+__device__ __forceinline__ int weight_row(int at) { return (at & ~63) + 2 * (at & 31) + (at >> 5 & 1); }
 
 template <typename T, int TM, int TN, int WM, int WN, bool NT>
 __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(GemmArgs8 g) {
@@ -323,8 +327,8 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(GemmArgs8 g) {
   for (int i = 0; i < LOADS; ++i) {
     const int row = (i * WAVES + wave) * 8 + (lane >> 3);
     const bool of_a = row < BM;
-    const int r = of_a ? row : row - BM, key = of_a ? r & 7 : r >> 1 & 7, last = of_a ? last_a : last_b;
-    off[i] = (r < last ? r : last) * Kp + ((lane & 7) ^ key) * 16;
+    const int at = of_a ? row : row - BM, r = of_a ? at : weight_row(at), last = of_a ? last_a : last_b;
+    off[i] = (r < last ? r : last) * Kp + ((lane & 7) ^ (at >> 1 & 7)) * 16;
   }
   auto request = [&](int kb, unsigned char *stage) {
 #pragma unroll
@@ -371,14 +375,14 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(GemmArgs8 g) {
     int s8[TM];
 #pragma unroll
     for (int m = 0; m < TM; ++m) s8[m] = (int)(sa[m] >> (8 * (kb & 3)) & 0xff);
-    const unsigned char *la = st + (wm * 32 * TM + j) * 128, *lb = st + (BM + wn * 32 * TN + 2 * j) * 128;
+    const unsigned char *la = st + (wm * 32 * TM + j) * 128, *lb = st + (BM + wn * 32 * TN + j) * 128;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {   // 64 codes: lane half h holds 32 of them
-      const int c0 = ((4 * s + 2 * h) ^ (j & 7)) * 16, c1 = ((4 * s + 2 * h + 1) ^ (j & 7)) * 16;
+      const int c0 = ((4 * s + 2 * h) ^ (j >> 1 & 7)) * 16, c1 = ((4 * s + 2 * h + 1) ^ (j >> 1 & 7)) * 16;
       i32x4 fa[TM][2], fb[TN][2];
 #pragma unroll
       for (int n = 0; n < TN; ++n) {
-        const unsigned char *r = lb + (n / 2 * 64 + n % 2) * 128;
+        const unsigned char *r = lb + 32 * n * 128;
         fb[n][0] = *reinterpret_cast<const i32x4 *>(r + c0);
         fb[n][1] = *reinterpret_cast<const i32x4 *>(r + c1);
       }
@@ -431,8 +435,8 @@ __global__ __launch_bounds__(256, 2) void fp8_stream_kernel(StreamArgs8 g) {
   const T *x = (const T *)g.x;
 
   for (int i = wave * 8; i < Kb * BN; i += 32) {   // the weight: eight rows of 128 codes per access (see above for the order)
-    const int kb = i / BN, r = i - kb * BN + (lane >> 3), n = r < g.N ? r : g.N - 1;
-    dma16(g.w + (long long)n * Kp + kb * 128 + ((lane & 7) ^ (r >> 1 & 7)) * 16, ws + i * 128);
+    const int kb = i / BN, at = i - kb * BN + (lane >> 3), r = weight_row(at), n = r < g.N ? r : g.N - 1;
+    dma16(g.w + (long long)n * Kp + kb * 128 + ((lane & 7) ^ (at >> 1 & 7)) * 16, ws + i * 128);
   }
   if (SUM)
     for (int i = 0; i < Kp / 128; ++i)
@@ -478,7 +482,7 @@ __global__ __launch_bounds__(256, 2) void fp8_stream_kernel(StreamArgs8 g) {
       for (int k = 0; k < 8; ++k) f.v[k] = (float)raw[s].v[k];
       const int row = s * 16 + rl, e = block_exponent(row_max_f32(top8(f)));
       const uint2 c = encode8(f, e);
-      *reinterpret_cast<uint2 *>(xs + (buf * BM + row) * 128 + ((cl >> 1) ^ (row & 7)) * 16 + (cl & 1) * 8) = c;
+      *reinterpret_cast<uint2 *>(xs + (buf * BM + row) * 128 + ((cl >> 1) ^ (row >> 1 & 7)) * 16 + (cl & 1) * 8) = c;
       if (cl == 0) es[buf * BM + row] = (unsigned char)e;
       if (g.codes && row < rows) {
         *reinterpret_cast<uint2 *>(codes + (unsigned)(row * Kp + cl * 8)) = c;
@@ -514,18 +518,18 @@ __global__ __launch_bounds__(256, 2) void fp8_stream_kernel(StreamArgs8 g) {
     const long long next = last ? tile + gridDim.x : tile;
     const int next_kb = last ? 0 : kb + 1;
     if (next < g.tiles) fetch(next, next_kb);
-    const unsigned char *la = xs + (buf * BM + wm * 32 * TM + j) * 128, *lb = ws + (kb * BN + wn * 32 * TN + 2 * j) * 128;
+    const unsigned char *la = xs + (buf * BM + wm * 32 * TM + j) * 128, *lb = ws + (kb * BN + wn * 32 * TN + j) * 128;
     const int sb = bs[(long long)kb * g.bs_k];
     int sa[TM];
 #pragma unroll
     for (int m = 0; m < TM; ++m) sa[m] = es[buf * BM + wm * 32 * TM + 32 * m + j];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int c0 = ((4 * s + 2 * h) ^ (j & 7)) * 16, c1 = ((4 * s + 2 * h + 1) ^ (j & 7)) * 16;
+      const int c0 = ((4 * s + 2 * h) ^ (j >> 1 & 7)) * 16, c1 = ((4 * s + 2 * h + 1) ^ (j >> 1 & 7)) * 16;
       i32x4 fa[TM][2], fb[TN][2];
 #pragma unroll
       for (int n = 0; n < TN; ++n) {
-        const unsigned char *r = lb + (n / 2 * 64 + n % 2) * 128;
+        const unsigned char *r = lb + 32 * n * 128;
         fb[n][0] = *reinterpret_cast<const i32x4 *>(r + c0);
         fb[n][1] = *reinterpret_cast<const i32x4 *>(r + c1);
       }
