@@ -360,3 +360,10 @@ def device_ctx(device):
 def current_stream(device):
     import torch
     return _c.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def raw_stream(device):
+    """The current stream of `device` as a plain address: what current_stream gives, without building a Stream object
+    (0.1 us against 2, and 11 on autograd's worker thread, per launch)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device.index)

@@ -7,6 +7,7 @@ has its own.  CPU tensors raise, like every operator of this package.  Gradients
 bit (no atomics); differentiating them again is refused.
 """
 import ctypes
+import functools
 
 import torch
 import torch.nn as nn
@@ -14,9 +15,13 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .fused_mlp import _call, _s
+from .fused_mlp import _call
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # GB_T_*
+
+
+def _s(t):
+    return _lib.raw_stream(t.device)
 
 
 def _refuse(what, why):
@@ -141,30 +146,37 @@ class Dropout(nn.Module):
         return dropout(x, self.p, self.take(), residual)
 
 
+def _norm_struct(x, weight, bias, residual, offsets, stats, at, used, seed, call, cfg):
+    """GbGroupNorm of one call, in the order of its fields."""
+    samples, groups, eps, act, slope, q = cfg
+    C, at_stats = x.shape[-1], stats.data_ptr()
+    return _lib.GroupNorm(x.data_ptr(), _lib.ptr(residual), _lib.ptr(weight), _lib.ptr(bias), _lib.ptr(offsets), at_stats,
+                          at_stats + 4 * samples * groups, at, used, x.numel() // C, seed, call, samples, C, groups,
+                          _TYPES[x.dtype], act, q, eps, slope)
+
+
 class _GroupNormAct(Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, offsets, samples, groups, eps, act, slope, q, rng):
-        dev, C = x.device, x.shape[-1]
-        rows = x.numel() // C
+    def forward(ctx, x, weight, bias, residual, offsets, cfg, rng):
+        dev = x.device
+        samples, groups = cfg[:2]
         y = torch.empty_like(x)
         stats = torch.empty((2, samples, groups), dtype=torch.float32, device=dev)
         at, seed, call = _rng_args(rng)
         used = torch.empty_like(rng) if at is not None else None
-        n = _lib.GroupNorm(x=_lib.ptr(x), residual=_lib.ptr(residual), weight=_lib.ptr(weight), bias=_lib.ptr(bias),
-                           offsets=_lib.ptr(offsets), mean=stats.data_ptr(), rstd=stats[1].data_ptr(), rng=at,
-                           used=_lib.ptr(used), rows=rows, seed=seed, call=call, samples=samples, channels=C, groups=groups,
-                           dtype=_TYPES[x.dtype], act=act, q=q, eps=eps, slope=slope)
-        ws, size = _norm_workspace(n, 0, dev)
-        _call("gb_group_norm_fwd", dev, ctypes.byref(n), _lib.ptr(y), _lib.ptr(ws), size, _s(x))
+        n = _norm_struct(x, weight, bias, residual, offsets, stats, at, _lib.ptr(used), seed, call, cfg)
+        size = _norm_workspace_bytes(n.rows, samples, n.channels, groups, n.dtype, offsets is not None, 0)
+        ws = _bytes(size, dev)
+        _call("gb_group_norm_fwd", dev, ctypes.byref(n), y.data_ptr(), _lib.ptr(ws), size, _s(x))
         ctx.save_for_backward(x, weight, bias, residual, offsets, stats, used)
-        ctx.cfg = (samples, groups, eps, act, slope, q, None if used is not None else rng)
+        ctx.cfg, ctx.rng = cfg, None if used is not None else rng
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, weight, bias, residual, offsets, stats, used = ctx.saved_tensors
-        samples, groups, eps, act, slope, q, rng = ctx.cfg
+        samples, groups, _, act, _, q = cfg = ctx.cfg
         dev, C = x.device, x.shape[-1]
         dy = dy.contiguous()
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
@@ -172,24 +184,28 @@ class _GroupNormAct(Function):
         # (the residual's gradient is dy itself where nothing stands between it and y)
         plain = act == 0 and q == 0 and offsets is None
         dres = torch.empty_like(x) if need_r and not plain else None
-        grads = torch.zeros((2, C), dtype=torch.float32, device=dev) if x.numel() == 0 else \
-            torch.empty((2, C), dtype=torch.float32, device=dev)
-        at, seed, call = _rng_args(used if rng is None else rng)
-        n = _lib.GroupNorm(x=_lib.ptr(x), residual=_lib.ptr(residual), weight=_lib.ptr(weight), bias=_lib.ptr(bias),
-                           offsets=_lib.ptr(offsets), mean=stats.data_ptr(), rstd=stats[1].data_ptr(), rng=at, used=None,
-                           rows=x.numel() // C, seed=seed, call=call, samples=samples, channels=C, groups=groups,
-                           dtype=_TYPES[x.dtype], act=act, q=q, eps=eps, slope=slope)
-        ws, size = _norm_workspace(n, 1, dev)
-        _call("gb_group_norm_bwd", dev, ctypes.byref(n), _lib.ptr(dy), _lib.ptr(dx), _lib.ptr(dres), grads.data_ptr(),
-              grads[1].data_ptr(), _lib.ptr(ws), size, _s(x))
-        return (dx if need_x else None, grads[0] if need_w else None, grads[1] if need_b else None,
-                (dy if plain else dres) if need_r else None) + (None,) * 8
+        make = torch.empty if x.numel() else torch.zeros
+        dw = make(C, dtype=torch.float32, device=dev) if need_w else None
+        db = make(C, dtype=torch.float32, device=dev) if need_b else None
+        at, seed, call = _rng_args(used if ctx.rng is None else ctx.rng)
+        n = _norm_struct(x, weight, bias, residual, offsets, stats, at, None, seed, call, cfg)
+        size = _norm_workspace_bytes(n.rows, samples, C, groups, n.dtype, offsets is not None, 1)
+        ws = _bytes(size, dev)
+        _call("gb_group_norm_bwd", dev, ctypes.byref(n), dy.data_ptr(), dx.data_ptr(), _lib.ptr(dres), _lib.ptr(dw),
+              _lib.ptr(db), _lib.ptr(ws), size, _s(x))
+        return dx if need_x else None, dw, db, (dy if plain else dres) if need_r else None, None, None, None
 
 
-def _norm_workspace(n, backward, dev):
+@functools.lru_cache(maxsize=1024)
+def _norm_workspace_bytes(rows, samples, channels, groups, dtype, packed, backward):
+    n = _lib.GroupNorm(rows=rows, samples=samples, channels=channels, groups=groups, dtype=dtype, offsets=8 if packed else None)
     size = ctypes.c_longlong()
     _lib.check(_lib.lib().gb_group_norm_workspace(ctypes.byref(n), backward, ctypes.byref(size)), "group_norm_act")
-    return (torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None), size.value
+    return size.value
+
+
+def _bytes(size, dev):
+    return torch.empty(size, dtype=torch.uint8, device=dev) if size else None
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", negative_slope=0.01, residual=None,
@@ -228,8 +244,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
         residual = residual.contiguous()
     q, rng = _rate(what, dropout_p, rng, x)
     return _GroupNormAct.apply(x.contiguous(), _channel_vector(what, "weight", weight, C, x),
-                               _channel_vector(what, "bias", bias, C, x), residual, offsets, samples, groups, float(eps),
-                               _lib.ACTIVATIONS[act], float(negative_slope), q, rng)
+                               _channel_vector(what, "bias", bias, C, x), residual, offsets,
+                               (samples, groups, float(eps), _lib.ACTIVATIONS[act], float(negative_slope), q), rng)
 
 
 # ---- products in 8-bit floats -----------------------------------------------------------------------------------------
@@ -274,10 +290,16 @@ def _fp8_product(x2, w, w_scales, transposed, N, bias, keep, colsum):
     return y, codes, scales, sums
 
 
-def _fp8_workspace(what, P, N, K, dev):
+@functools.lru_cache(maxsize=1024)
+def _fp8_workspace_bytes(what, P, N, K):
     size = ctypes.c_longlong()
     _lib.check(_lib.lib().gb_fp8_workspace(what, P, N, K, ctypes.byref(size)), "fp8_linear")
-    return (torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None), size.value
+    return size.value
+
+
+def _fp8_workspace(what, P, N, K, dev):
+    size = _fp8_workspace_bytes(what, P, N, K)
+    return _bytes(size, dev), size
 
 
 def _quantise_weight(w, transposed):
