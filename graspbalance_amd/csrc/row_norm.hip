@@ -21,6 +21,9 @@
 namespace gb {
 
 static constexpr int GN_MAX_C = 4096;   // two doubles per channel in LDS while a workgroup's sums are joined
+static constexpr int GN_DIRECT = 32;    // workgroups per sample up to which every applying one adds their sums for itself:
+                                        // a launch less (4 x 1024 x 256 bf16: 40 -> 30 us of kernels and gaps a pass)
+static constexpr int GN_DIRECT_GROUPS = 256;
 static constexpr int GN_MIN_STEPS = 4;  // of a workgroup: with fewer, joining the sums costs what the parallelism gains
 
 struct GnShape {
@@ -48,6 +51,7 @@ struct GnArgs {
   float eps, slope, scale;
   unsigned q;
   int sub;             // columns of a workgroup that holds them in registers
+  int direct;          // the applying kernel joins the workgroups' sums itself
 };
 
 // Rows of sample s.  Offsets come from the device and are taken as they are within [0, R]: no value of theirs leads
@@ -330,29 +334,32 @@ __device__ __forceinline__ void finish_group(double t1, double t2, double n, flo
   rstd = (float)(1.0 / sqrt(var + (double)eps));
 }
 
-// one wave per (sample, group)
+// mean and rstd of a group from the workgroups' sums, added by the lanes of a wave (lane, lanes) or by one alone (0, 1)
 template <int N>
-__global__ __launch_bounds__(64) void gn_finish_kernel(GnArgs a) {
+__device__ __forceinline__ void sample_stats(const GnArgs &a, int s, int g, int lane, int lanes, float &mean, float &rstd) {
   const GnShape &sh = a.sh;
-  const int g = (int)blockIdx.x, s = (int)blockIdx.y, lane = (int)threadIdx.x;
   long long lo, hi, per;
   sample_rows(sh, s, lo, hi);
   const int ranges = chunk_ranges(sh, (hi - lo) * sh.C, N, per);
   double t1 = 0, t2 = 0;
 #pragma unroll 4
-  for (int c = lane; c < ranges; c += 64) {
+  for (int c = lane; c < ranges; c += lanes) {
     const double *p = a.gpart + (((long long)s * sh.ns + c) * sh.G + g) * 2;
     t1 += p[0];
     t2 += p[1];
   }
-#pragma unroll
-  for (int o = 32; o; o >>= 1) t1 += __shfl_xor(t1, o), t2 += __shfl_xor(t2, o);
-  if (lane == 0) {
-    float mean = 0, rstd = 0;
-    if (hi > lo) finish_group(t1, t2, (double)(hi - lo) * sh.cpg, a.eps, mean, rstd);
-    a.mean[(long long)s * sh.G + g] = mean;
-    a.rstd[(long long)s * sh.G + g] = rstd;
-  }
+  for (int o = lanes >> 1; o; o >>= 1) t1 += __shfl_xor(t1, o), t2 += __shfl_xor(t2, o);
+  mean = rstd = 0;
+  if (hi > lo) finish_group(t1, t2, (double)(hi - lo) * sh.cpg, a.eps, mean, rstd);
+}
+
+// one wave per (sample, group)
+template <int N>
+__global__ __launch_bounds__(64) void gn_finish_kernel(GnArgs a) {
+  const long long at = (long long)blockIdx.y * a.sh.G + blockIdx.x;
+  float mean, rstd;
+  sample_stats<N>(a, (int)blockIdx.y, (int)blockIdx.x, (int)threadIdx.x, 64, mean, rstd);
+  if (threadIdx.x == 0) a.mean[at] = mean, a.rstd[at] = rstd;
 }
 
 // A unit from flat index i (of the whole tensor) through norm, activation and dropout; res: zeros where there is no residual.
@@ -439,11 +446,26 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(GnArgs a) {
   }
   const Lane l = lane_place(sh);
   const Range g = range_of<N>(sh, s, chunk);
-  if (g.none || !l.on) return;
+  if (g.none) return;
+  const float *mean = a.mean + (long long)s * sh.G, *rstd = a.rstd + (long long)s * sh.G;
+  __shared__ float stats[2][GN_DIRECT_GROUPS];
+  if (a.direct) {
+    for (int i = (int)threadIdx.x; i < sh.G; i += (int)blockDim.x) {
+      sample_stats<N>(a, s, i, 0, 1, stats[0][i], stats[1][i]);
+      if (chunk == 0) {
+        a.mean[(long long)s * sh.G + i] = stats[0][i];
+        a.rstd[(long long)s * sh.G + i] = stats[1][i];
+      }
+    }
+    __syncthreads();
+    mean = stats[0];
+    rstd = stats[1];
+  }
+  if (!l.on) return;
   const T *x = (const T *)a.x + g.base, *res = a.res ? (const T *)a.res + g.base : nullptr;
   T *y = (T *)a.y + g.base;
   Coef<N> co;
-  load_coef<N>(sh, a.w, a.b, l.p, a.mean + (long long)s * sh.G, a.rstd + (long long)s * sh.G, co);
+  load_coef<N>(sh, a.w, a.b, l.p, mean, rstd, co);
   const long long step = sh.T;
   long long v = g.v;
   for (; v + step < g.end; v += 2 * step) {   // two steps' loads in flight
@@ -645,7 +667,29 @@ __global__ __launch_bounds__(256) void gn_bwd_join_kernel(GnArgs a) {
   }
 }
 
+// the sums of a channel over a sample, as the joining kernel left them or from the workgroups'
+template <int N>
+__device__ __forceinline__ void channel_sums(const GnArgs &a, int s, int c, double &s0, double &s1) {
+  const GnShape &sh = a.sh;
+  if (!a.direct) {
+    const float2 f = reinterpret_cast<const float2 *>(a.csum)[(long long)s * sh.C + c];
+    s0 += f.x;
+    s1 += f.y;
+    return;
+  }
+  long long lo, hi, per;
+  sample_rows(sh, s, lo, hi);
+  const int ranges = chunk_ranges(sh, (hi - lo) * sh.C, N, per);
+#pragma unroll 8
+  for (int k = 0; k < ranges; ++k) {
+    const float2 f = reinterpret_cast<const float2 *>(a.cpart)[((long long)s * sh.ns + k) * sh.C + c];
+    s0 += f.x;
+    s1 += f.y;
+  }
+}
+
 // dw, db = the samples' sums added, by workgroup `part` of `parts`: 32 channels x blockDim / 32 lanes over the samples
+template <int N>
 __device__ __forceinline__ void channel_gradients(const GnArgs &a, int part, int parts) {
   const GnShape &sh = a.sh;
   double *lds = reinterpret_cast<double *>(gn_lds);
@@ -654,11 +698,7 @@ __device__ __forceinline__ void channel_gradients(const GnArgs &a, int part, int
     const int c = c0 + i;
     double s0 = 0, s1 = 0;
     if (c < sh.C)
-      for (int s = q; s < sh.S; s += Q) {
-        const float2 f = reinterpret_cast<const float2 *>(a.csum)[(long long)s * sh.C + c];
-        s0 += f.x;
-        s1 += f.y;
-      }
+      for (int s = q; s < sh.S; s += Q) channel_sums<N>(a, s, c, s0, s1);
     lds[2 * threadIdx.x] = s0;
     lds[2 * threadIdx.x + 1] = s1;
     __syncthreads();
@@ -702,7 +742,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnArgs a) {
   const GnShape &sh = a.sh;
   const int s = (int)blockIdx.y, chunk = (int)blockIdx.x;
   if (s == sh.S) {
-    channel_gradients(a, chunk, sh.ns);
+    channel_gradients<N>(a, chunk, sh.ns);
     if (sh.offs) zero_outside<T>(sh, (T *)a.dx, (T *)a.dres, chunk, sh.ns);
     return;
   }
@@ -715,9 +755,10 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnArgs a) {
   if (hi == lo) return;
   float *v0 = reinterpret_cast<float *>(gn_lds), *v1 = v0 + sh.C, *k1 = v1 + sh.C, *k2 = k1 + sh.G;
   for (int c = (int)threadIdx.x; c < sh.C; c += (int)blockDim.x) {
-    const float2 f = reinterpret_cast<const float2 *>(a.csum)[(long long)s * sh.C + c];
-    v0[c] = f.x;
-    v1[c] = f.y;
+    double s0 = 0, s1 = 0;
+    channel_sums<N>(a, s, c, s0, s1);
+    v0[c] = (float)s0;
+    v1[c] = (float)s1;
   }
   group_terms(a, v0, v1, k1, k2, (double)(hi - lo) * sh.cpg);
   if (!l.on) return;
@@ -775,6 +816,7 @@ static int period(int c, int unit) {   // lanes: c / gcd(c, unit)
 struct GnPlan {
   int block, PL, T;
   int ns;    // workgroups per sample
+  int direct;
   int sub;   // columns per workgroup of the one-pass kernel; 0: the sample is read twice
   size_t lds, ws;
 };
@@ -802,22 +844,25 @@ static GnPlan gn_plan(const GbGroupNorm *n, bool backward) {
   p.sub = 0;
   if (!backward) {
     // The one-pass kernel wherever a sample's columns fit: no second read and one launch instead of three.  Columns: all
-    // of them when C is no multiple of N, else the fewest whole groups that divide C into full 128-byte lines of units.
-    int sub = C;
-    if (C % N == 0)
-      for (int gs = 1; gs <= n->groups; ++gs)
-        if (n->groups % gs == 0 && gs * cpg % N == 0 && gs * cpg * size >= 128) {
-          sub = gs * cpg;
-          break;
-        }
-    const int PL = period(sub, N), T = PL <= 1024 ? 1024 / PL * PL : 0;
-    if (T && longest * sub / N < (long long)T * (GN_HELD / N)) {
-      p.sub = sub;
-      p.PL = PL;
-      // (lanes for one unit each, in whole waves: latency counts more than what a lane could hold)
-      const long long units = (longest * sub + N - 1) / N;
-      p.block = PL <= 256 && units <= 256 ? 256 : PL <= 512 && units <= 512 ? 512 : 1024;
-      p.ns = C / sub;
+    // of them when C is no multiple of N, else the fewest whole groups that divide C into full 128-byte lines of units, or
+    // halves or quarters of lines where only those fit (the other parts' workgroups find the line in L2).
+    for (int line = 128; line >= 32 && !p.sub; line /= 2) {
+      int sub = C;
+      if (C % N == 0)
+        for (int gs = 1; gs <= n->groups; ++gs)
+          if (n->groups % gs == 0 && gs * cpg % N == 0 && gs * cpg * size >= line) {
+            sub = gs * cpg;
+            break;
+          }
+      const int PL = period(sub, N), T = PL <= 1024 ? 1024 / PL * PL : 0;
+      if (T && longest * sub / N < (long long)T * (GN_HELD / N)) {
+        p.sub = sub;
+        p.PL = PL;
+        // (lanes for one unit each, in whole waves: latency counts more than what a lane could hold)
+        const long long units = (longest * sub + N - 1) / N;
+        p.block = PL <= 256 && units <= 256 ? 256 : PL <= 512 && units <= 512 ? 512 : 1024;
+        p.ns = C / sub;
+      }
     }
   }
   if (!p.sub) {
@@ -828,7 +873,10 @@ static GnPlan gn_plan(const GbGroupNorm *n, bool backward) {
     const long long units = (longest * C + N - 1) / N, steps = (units + T - 1) / T;
     const int waves = N == 4 ? (backward ? 5 : 8) : (backward ? 4 : 6);   // per SIMD, by the kernels' registers
     p.ns = spread(n, steps, 256ll * 4 * waves * 64 / p.block);
+    // a few more steps each rather than a launch more
+    if (p.ns > GN_DIRECT && p.ns <= 2 * GN_DIRECT) p.ns = GN_DIRECT;
   }
+  p.direct = !p.sub && p.ns <= GN_DIRECT && (backward || n->groups <= GN_DIRECT_GROUPS);
   p.T = p.block / p.PL * p.PL;
   const size_t cell = backward ? sizeof(float) : sizeof(double);
   const int K = !backward && cpg % N == 0 ? 1 : N;
@@ -883,6 +931,7 @@ static GnArgs gn_args(const GbGroupNorm *n, const GnPlan &p) {
   a.sh.T = p.T;
   a.sh.ns = p.ns;
   a.sub = p.sub;
+  a.direct = p.direct;
   a.x = n->x;
   a.res = n->residual;
   a.w = n->weight;
@@ -935,7 +984,7 @@ extern "C" int gb_group_norm_fwd(const GbGroupNorm *n, void *y, void *ws, long l
         gn_stats_kernel<T, true><<<grid, p.block, p.lds, st>>>(a);
       else
         gn_stats_kernel<T, false><<<grid, p.block, p.lds, st>>>(a);
-      gn_finish_kernel<Unit<T>::N><<<dim3((unsigned)n->groups, (unsigned)n->samples), 64, 0, st>>>(a);
+      if (!p.direct) gn_finish_kernel<Unit<T>::N><<<dim3((unsigned)n->groups, (unsigned)n->samples), 64, 0, st>>>(a);
       if (nt)
         gn_apply_kernel<T, ACT, true><<<all, p.block, 0, st>>>(a);
       else
@@ -971,7 +1020,7 @@ extern "C" int gb_group_norm_bwd(const GbGroupNorm *n, const void *dy, void *dx,
       gn_bwd_stats_kernel<T, ACT, true><<<grid, p.block, p.lds, st>>>(a);
     else
       gn_bwd_stats_kernel<T, ACT, false><<<grid, p.block, p.lds, st>>>(a);
-    gn_bwd_join_kernel<Unit<T>::N><<<dim3((unsigned)((n->channels + 7) / 8), (unsigned)n->samples), 256, 0, st>>>(a);
+    if (!p.direct) gn_bwd_join_kernel<Unit<T>::N><<<dim3((unsigned)((n->channels + 7) / 8), (unsigned)n->samples), 256, 0, st>>>(a);
     if (nt)
       gn_bwd_apply_kernel<T, ACT, true><<<all, p.block, p.lds, st>>>(a);
     else
