@@ -47,7 +47,7 @@ def _channel_vector(what, name, t, n, x):
         return None
     if t.shape != (n,) or t.device != x.device or not t.is_floating_point():
         _refuse(what, "%s must be a float tensor of %d elements on the input's device" % (name, n))
-    return t.float().contiguous()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
 def _rate(what, p, rng, x):
@@ -74,15 +74,26 @@ def _rng_args(rng):
     return (_lib.ptr(rng), 0, 0) if isinstance(rng, torch.Tensor) else (None, rng[0], rng[1])
 
 
+def _grads(*tensors):
+    """Whether a call has to be recorded for a backward pass."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _dropout(x, residual, q, rng, keep):
+    """(y, the pair that was used | None)"""
+    y = torch.empty_like(x)
+    at, seed, call = _rng_args(rng)
+    # the numbers' key is kept as it was used: the owner may write the next call's into rng before the backward pass
+    used = torch.empty_like(rng) if keep and at is not None else None
+    _call("gb_dropout", x.device, x.data_ptr(), _lib.ptr(residual), y.data_ptr(), x.numel(), _TYPES[x.dtype], q, at, seed, call,
+          _lib.ptr(used), _s(x))
+    return y, used
+
+
 class _Dropout(Function):
     @staticmethod
     def forward(ctx, x, residual, q, rng):
-        y = torch.empty_like(x)
-        at, seed, call = _rng_args(rng)
-        # the numbers' key is kept as it was used: the owner may write the next call's into rng before the backward pass
-        used = torch.empty_like(rng) if at is not None else None
-        _call("gb_dropout", x.device, _lib.ptr(x), _lib.ptr(residual), _lib.ptr(y), x.numel(), _TYPES[x.dtype], q, at, seed,
-              call, _lib.ptr(used), _s(x))
+        y, used = _dropout(x, residual, q, rng, True)
         ctx.q, ctx.rng, ctx.has_residual = q, None if used is not None else rng, residual is not None
         ctx.save_for_backward(*(() if used is None else (used,)))
         return y
@@ -92,11 +103,7 @@ class _Dropout(Function):
     def backward(ctx, dy):
         dx = None
         if ctx.needs_input_grad[0]:
-            dy = dy.contiguous()
-            dx = torch.empty_like(dy)
-            at, seed, call = _rng_args(ctx.saved_tensors[0] if ctx.rng is None else ctx.rng)
-            _call("gb_dropout", dy.device, _lib.ptr(dy), None, _lib.ptr(dx), dy.numel(), _TYPES[dy.dtype], ctx.q, at, seed,
-                  call, None, _s(dy))
+            dx, _ = _dropout(dy.contiguous(), None, ctx.q, ctx.saved_tensors[0] if ctx.rng is None else ctx.rng, False)
         return dx, dy if ctx.has_residual and ctx.needs_input_grad[1] else None, None, None
 
 
@@ -112,7 +119,10 @@ def dropout(x, p, rng, residual=None):
         _like("dropout", "residual", residual, x)
     if q == 0:
         return x if residual is None else x + residual
-    return _Dropout.apply(x.contiguous(), None if residual is None else residual.contiguous(), q, rng)
+    x, residual = x.contiguous(), None if residual is None else residual.contiguous()
+    if not _grads(x, residual):
+        return _dropout(x, residual, q, rng, False)[0]
+    return _Dropout.apply(x, residual, q, rng)
 
 
 class Dropout(nn.Module):
@@ -155,19 +165,25 @@ def _norm_struct(x, weight, bias, residual, offsets, stats, at, used, seed, call
                           _TYPES[x.dtype], act, q, eps, slope)
 
 
+def _norm(x, weight, bias, residual, offsets, cfg, rng, keep):
+    """(y, statistics, the pair that was used | None)"""
+    dev = x.device
+    samples, groups = cfg[:2]
+    y = torch.empty_like(x)
+    stats = torch.empty((2, samples, groups), dtype=torch.float32, device=dev)
+    at, seed, call = _rng_args(rng)
+    used = torch.empty_like(rng) if keep and at is not None else None
+    n = _norm_struct(x, weight, bias, residual, offsets, stats, at, _lib.ptr(used), seed, call, cfg)
+    size = _norm_workspace_bytes(n.rows, samples, n.channels, groups, n.dtype, offsets is not None, 0)
+    ws = _bytes(size, dev)
+    _call("gb_group_norm_fwd", dev, ctypes.byref(n), y.data_ptr(), _lib.ptr(ws), size, _s(x))
+    return y, stats, used
+
+
 class _GroupNormAct(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, offsets, cfg, rng):
-        dev = x.device
-        samples, groups = cfg[:2]
-        y = torch.empty_like(x)
-        stats = torch.empty((2, samples, groups), dtype=torch.float32, device=dev)
-        at, seed, call = _rng_args(rng)
-        used = torch.empty_like(rng) if at is not None else None
-        n = _norm_struct(x, weight, bias, residual, offsets, stats, at, _lib.ptr(used), seed, call, cfg)
-        size = _norm_workspace_bytes(n.rows, samples, n.channels, groups, n.dtype, offsets is not None, 0)
-        ws = _bytes(size, dev)
-        _call("gb_group_norm_fwd", dev, ctypes.byref(n), y.data_ptr(), _lib.ptr(ws), size, _s(x))
+        y, stats, used = _norm(x, weight, bias, residual, offsets, cfg, rng, True)
         ctx.save_for_backward(x, weight, bias, residual, offsets, stats, used)
         ctx.cfg, ctx.rng = cfg, None if used is not None else rng
         return y
@@ -243,9 +259,12 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
         _like(what, "residual", residual, x)
         residual = residual.contiguous()
     q, rng = _rate(what, dropout_p, rng, x)
-    return _GroupNormAct.apply(x.contiguous(), _channel_vector(what, "weight", weight, C, x),
-                               _channel_vector(what, "bias", bias, C, x), residual, offsets,
-                               (samples, groups, float(eps), _lib.ACTIVATIONS[act], float(negative_slope), q), rng)
+    x = x.contiguous()
+    weight, bias = _channel_vector(what, "weight", weight, C, x), _channel_vector(what, "bias", bias, C, x)
+    cfg = (samples, groups, float(eps), _lib.ACTIVATIONS[act], float(negative_slope), q)
+    if not _grads(x, weight, bias, residual):
+        return _norm(x, weight, bias, residual, offsets, cfg, rng, False)[0]
+    return _GroupNormAct.apply(x, weight, bias, residual, offsets, cfg, rng)
 
 
 # ---- products in 8-bit floats -----------------------------------------------------------------------------------------
@@ -416,7 +435,11 @@ def fp8_linear(x, weight, bias=None):
     if x.dim() < 1 or x.shape[-1] != K:
         _refuse(what, "x must be (..., %d)" % K)
     bias = _channel_vector(what, "bias", bias, N, x)
-    if not torch.is_grad_enabled():   # (needs_input_grad does not know the grad mode: nothing would be kept in vain)
-        x, weight, bias = (t.detach() if isinstance(t, torch.Tensor) else t for t in (x, weight, bias))
-    y = _Fp8Linear.apply(x.reshape(-1, K).contiguous(), None if held is not None else weight, bias, held)
-    return y.view(x.shape[:-1] + (N,))
+    weight = None if held is not None else weight
+    rows = (x if x.dim() == 2 else x.reshape(-1, K)).contiguous()
+    if _grads(x, weight, bias):
+        y = _Fp8Linear.apply(rows, weight, bias, held)
+    else:
+        codes, scales = (held.codes, held.scales) if held is not None else _quantise_weight(weight.contiguous(), False)[::2]
+        y = _fp8_product(rows, codes, scales, 0, N, bias, False, False)[0]
+    return y if x.dim() == 2 else y.view(x.shape[:-1] + (N,))
