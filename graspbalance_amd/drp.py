@@ -11,7 +11,7 @@ import torch.nn as nn
 from .backbone import break_up_pc, make_sa
 from .modified_net_tools.activation import CHANNEL_MAP, create_act
 from .modified_net_tools.conv import create_convblock1d, create_convblock2d
-from . import fused_mlp
+from . import fused_mlp, fused_rows
 from . import pytorch_utils as pt_utils
 from .modified_net_tools.group import QueryAndGroup, ball_query, create_grouper, get_aggregation_feautres
 from .pointnet2_modules import PointnetFPModule
@@ -63,13 +63,18 @@ def _pointwise(channels, norm_args, act_args, conv_args, less_act):
 
 
 class InvResMLP(nn.Module):
-    """LocalAggregation(C->C) -> pointwise C->expansion*C->C -> residual add -> act."""
+    """LocalAggregation(C->C) -> pointwise C->expansion*C->C -> residual add -> act.
+
+    Beyond the reference: norm_args={'norm': 'gn', 'num_groups': g} takes group norm for BatchNorm (channel-last on the GPU
+    like the BatchNorm path); dropout > 0 drops the expanded features between the pointwise convolutions
+    (fused_rows.Dropout, key ``dropout``); fp8 runs the three products in 8-bit floats (group norm only)."""
 
     def __init__(self, in_channels, norm_args=None, act_args=None,
                  aggr_args={'feature_type': 'dp_fj', "reduction": 'max'}, group_args={'NAME': 'ballquery'},
-                 conv_args=None, expansion=1, use_res=True, num_posconvs=2, less_act=False, **kwargs):
+                 conv_args=None, expansion=1, use_res=True, num_posconvs=2, less_act=False, dropout=0.0, fp8=False, **kwargs):
         super().__init__()
         self.use_res = use_res
+        self.fp8 = bool(fp8)
         mid_channels = int(in_channels * expansion)
         self.convs = LocalAggregation([in_channels, in_channels], norm_args=norm_args,
                                       act_args=act_args if num_posconvs > 0 else None, group_args=group_args,
@@ -82,12 +87,35 @@ class InvResMLP(nn.Module):
             channels = [in_channels, mid_channels, in_channels]
         self.pwconv = _pointwise(channels, norm_args, act_args, conv_args, less_act)
         self.act = create_act(act_args)
+        self.dropout = None
+        if dropout:
+            if len(self.pwconv) != 2:
+                raise ValueError("dropout stands between the two pointwise convolutions: num_posconvs must be 2")
+            self.dropout = fused_rows.Dropout(dropout)
+        if self.fp8 and not self.fusable_gn():
+            raise ValueError("fp8 needs group norm, a max over ball-query neighbours and the standard conv-norm-act blocks")
+
+    def _standard(self):
+        """dp_fj features, max reduction, plain ball-query grouper, one aggregation layer, two pointwise layers, residual."""
+        la = self.convs
+        g = la.grouper
+        return (la.feature_type == 'dp_fj' and la.reduction == 'max' and isinstance(g, QueryAndGroup)
+                and g.relative_xyz and not g.normalize_dp and not g.return_only_idx
+                and len(la.convs) == 1 and len(self.pwconv) == 2 and self.use_res)
+
+    def fusable_gn(self):
+        """conv + group norm + an activation that the row kernels have, after the aggregation, the expansion and the sum."""
+        def is_block(seq, with_act):
+            mods = list(seq.children())
+            return (len(mods) == (3 if with_act else 2) and isinstance(mods[0], (nn.Conv1d, nn.Conv2d)) and mods[0].bias is None
+                    and all(k == 1 for k in mods[0].kernel_size) and isinstance(mods[1], nn.GroupNorm)
+                    and (not with_act or fused_rows.activation_of(mods[2]) is not None))
+        return (self._standard() and is_block(self.convs.convs[0], True) and is_block(self.pwconv[0], True)
+                and is_block(self.pwconv[1], False) and fused_rows.activation_of(self.act) is not None)
 
     def fusable(self):
         """The configuration DRP builds: dp_fj features, max reduction, plain ball-query grouper,
         one conv+BN+ReLU aggregation layer, conv+BN+ReLU -> conv+BN pointwise pair, residual, ReLU."""
-        la = self.convs
-        g = la.grouper
         def is_block(seq, with_act):
             mods = list(seq.children())
             want = 3 if with_act else 2
@@ -95,11 +123,8 @@ class InvResMLP(nn.Module):
                     and isinstance(mods[1], (nn.BatchNorm1d, nn.BatchNorm2d))
                     and not (mods[1].momentum is None and mods[1].track_running_stats)
                     and (not with_act or isinstance(mods[2], nn.ReLU)))
-        return (la.feature_type == 'dp_fj' and la.reduction == 'max' and isinstance(g, QueryAndGroup)
-                and g.relative_xyz and not g.normalize_dp and not g.return_only_idx
-                and len(la.convs) == 1 and is_block(la.convs[0], True) and len(self.pwconv) == 2
-                and is_block(self.pwconv[0], True) and is_block(self.pwconv[1], False) and self.use_res
-                and isinstance(self.act, nn.ReLU))
+        return (self._standard() and is_block(self.convs.convs[0], True) and is_block(self.pwconv[0], True)
+                and is_block(self.pwconv[1], False) and isinstance(self.act, nn.ReLU))
 
     def forward_cl(self, p, f_cl, idx=None, geo=None):
         """Channel-last execution: f_cl (B,N,C) -> (B,N,C).  `idx` (B,N,ns) and the grouping summary `geo`
@@ -108,6 +133,8 @@ class InvResMLP(nn.Module):
         g = self.convs.grouper
         if idx is None:
             idx = ball_query(g.radius, g.nsample, p, p)
+        if isinstance(self.convs.convs[0][1], nn.GroupNorm):
+            return self._forward_gn(p, f_cl, idx)
         agg_conv, agg_bn = self.convs.convs[0][0], self.convs.convs[0][1]
         if fused_mlp.local_agg_supported(agg_conv.weight.shape[0], g.nsample) and fused_mlp.local_agg_enabled():
             # the 1x1 conv commutes with the gather: no grouped (B*N*ns, 3+C) tensor at all
@@ -117,19 +144,43 @@ class InvResMLP(nn.Module):
         else:
             x0 = fused_mlp.group_concat_cl(p, p, idx, f_cl, mode=0)               # [dp, fj] rows
             agg = fused_mlp.conv_bn_act(x0, agg_conv, agg_bn, relu=True, pool_ns=g.nsample)   # (B*N, C)
+        if self.dropout is not None and self.training:   # (the pair in two, the expanded features dropped in between)
+            hidden = self.dropout(fused_mlp.conv_bn_act(agg, self.pwconv[0][0], self.pwconv[0][1]))
+            out = fused_mlp.conv_bn_act(hidden, self.pwconv[1][0], self.pwconv[1][1], relu=True,
+                                        residual=f_cl.reshape(B * N, C))
+            return out.view(B, N, C)
         # C -> 4C -> C pointwise pair as one fused stack; act(bn(.) + identity) at the end
         out = fused_mlp.conv_bn_act_chain(agg, [(self.pwconv[0][0], self.pwconv[0][1]),
                                                 (self.pwconv[1][0], self.pwconv[1][1])],
                                           residual=f_cl.reshape(B * N, C), relu_last=True)
         return out.view(B, N, C)
 
+    def _forward_gn(self, p, f_cl, idx):
+        """The block with group norm: statistics per cloud, every layer on channel-last rows."""
+        B, N, C = f_cl.shape
+        agg, (pw0, pw1) = self.convs.convs[0], self.pwconv
+        x0 = fused_mlp.group_concat_cl(p, p, idx, f_cl, mode=0)                   # [dp, fj] rows, (B*N*ns, 3 + C)
+        x = fused_rows.conv_gn_act(x0.view(B, -1, x0.shape[-1]), agg[0], agg[1], fused_rows.activation_of(agg[2]), self.fp8)
+        x = x.view(B, N, -1, C).max(dim=2)[0]
+        x = fused_rows.conv_gn_act(x, pw0[0], pw0[1], fused_rows.activation_of(pw0[2]), self.fp8, dropout=self.dropout)
+        return fused_rows.conv_gn_act(x, pw1[0], pw1[1], fused_rows.activation_of(self.act), self.fp8, residual=f_cl)
+
+    def _fused_on(self, f):
+        return fused_mlp.enabled(f) and (self.fusable() or (fused_rows.supports(f) and self.fusable_gn()))
+
     def forward(self, pf):
         p, f = pf
-        if fused_mlp.enabled(f) and self.fusable():
+        if self._fused_on(f):
             out = self.forward_cl(p, f.transpose(1, 2).contiguous())
             return [p, out.transpose(1, 2)]
+        if self.fp8:
+            raise RuntimeError("InvResMLP: fp8 runs on the GPU only")
         identity = f
-        f = self.pwconv(self.convs([p, f]))
+        f = self.convs([p, f])
+        if self.dropout is not None:
+            f = self.pwconv[1](self.dropout(self.pwconv[0](f)))
+        else:
+            f = self.pwconv(f)
         if f.shape[-1] == identity.shape[-1] and self.use_res:
             f += identity
         return [p, self.act(f)]
@@ -139,7 +190,7 @@ def run_stage(blocks, p, f):
     """A Sequential of InvResMLP blocks over the same points: on the fused path the features stay
     channel-last across the blocks and the ball query (same p, same radius) is done once."""
     blocks = list(blocks)
-    if not (fused_mlp.enabled(f) and blocks and all(isinstance(b, InvResMLP) and b.fusable() for b in blocks)):
+    if not (blocks and all(isinstance(b, InvResMLP) and b._fused_on(f) for b in blocks)):
         for blk in blocks:
             p, f = blk([p, f])
         return p, f
@@ -148,7 +199,7 @@ def run_stage(blocks, p, f):
     idx = ball_query(g0.radius, g0.nsample, p, p) if same else None
     geo = None
     if same and fused_mlp.local_agg_enabled() and all(
-            fused_mlp.local_agg_supported(b.convs.convs[0][0].weight.shape[0], g0.nsample) for b in blocks):
+            b.fusable() and fused_mlp.local_agg_supported(b.convs.convs[0][0].weight.shape[0], g0.nsample) for b in blocks):
         geo = fused_mlp.LocalGeometry(p, p, idx, mode=0)
     f_cl = f.transpose(1, 2).contiguous()
     for blk in blocks:
@@ -208,11 +259,14 @@ STAGE_SPECS = ((128, 0.08, 64, 3), (256, 0.2, 32, 6), (256, 0.4, 16, 3), (256, 0
 
 
 class DRP(nn.Module):
-    def __init__(self, input_feature_dim=0):
+    """norm_args, act_args, dropout, fp8: of the InvResMLP blocks (see there); the set abstraction and feature propagation
+    keep the reference's BatchNorm + ReLU."""
+
+    def __init__(self, input_feature_dim=0, norm_args=None, act_args=None, dropout=0.0, fp8=False):
         super().__init__()
         self.aggr_args = {'feature_type': 'dp_fj', "reduction": 'max'}
-        self.norm_args = {'norm': 'bn'}
-        self.act_args = {'act': 'relu'}
+        self.norm_args = norm_args or {'norm': 'bn'}
+        self.act_args = act_args or {'act': 'relu'}
         self.conv_args = {'order': 'conv-norm-act'}
         self.use_res = True
         self.expansion = 4
@@ -221,7 +275,8 @@ class DRP(nn.Module):
             group_args = {'NAME': 'ballquery', 'radius': radius, 'nsample': nsample}
             blocks = [InvResMLP(in_channels=channels, aggr_args=self.aggr_args, norm_args=self.norm_args,
                                 act_args=self.act_args, group_args=group_args, conv_args=self.conv_args,
-                                expansion=self.expansion, use_res=self.use_res) for _ in range(depth)]
+                                expansion=self.expansion, use_res=self.use_res, dropout=dropout, fp8=fp8)
+                      for _ in range(depth)]
             setattr(self, 'InvResMLP_blocks%d' % (level + 1), nn.Sequential(*blocks))
         self.fp1 = PointnetFPModule(mlp=[256 + 256, 256, 256])
         self.fp2 = PointnetFPModule(mlp=[256 + 256, 256, 256])

@@ -15,7 +15,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .fused_mlp import _call
+from .fused_mlp import _call, linear_bias
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # GB_T_*
 
@@ -26,6 +26,11 @@ def _s(t):
 
 def _refuse(what, why):
     raise RuntimeError("%s: %s" % (what, why))
+
+
+def supports(t):
+    """Whether the operators of this module take tensor t."""
+    return t.is_cuda and t.dtype in _TYPES
 
 
 def _rows_tensor(what, name, t):
@@ -443,3 +448,34 @@ def fp8_linear(x, weight, bias=None):
         codes, scales = (held.codes, held.scales) if held is not None else _quantise_weight(weight.contiguous(), False)[::2]
         y = _fp8_product(rows, codes, scales, 0, N, bias, False, False)[0]
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (N,))
+
+
+# ---- conv + group norm blocks ------------------------------------------------------------------------------------------
+
+def activation_of(module):
+    """(name, slope) of an activation module as group_norm_act takes it (None: no activation); None for any other."""
+    if module is None or isinstance(module, nn.Identity):
+        return "none", 0.0
+    if isinstance(module, nn.ReLU):
+        return "relu", 0.0
+    if isinstance(module, nn.LeakyReLU):
+        return "leaky_relu", float(module.negative_slope)
+    if isinstance(module, nn.SiLU):
+        return "silu", 0.0
+    if isinstance(module, nn.GELU) and module.approximate == "none":
+        return "gelu", 0.0
+    return None
+
+
+def conv_gn_act(x, conv, gn, act=("none", 0.0), fp8=False, residual=None, dropout=None):
+    """A 1x1 ``conv`` without bias, ``gn`` (nn.GroupNorm), an activation (activation_of) and optionally a Dropout on
+    channel-last rows x (samples, rows, Cin) -> (samples, rows, Cout), with the modules' own parameters; residual joins
+    in front of the activation.  fp8: the product in 8-bit floats."""
+    W = conv.weight.view(conv.weight.shape[0], -1)
+    if fp8:
+        y = fp8_linear(x, W)
+    else:
+        y = linear_bias(x.reshape(-1, x.shape[-1]), conv).view(x.shape[:-1] + (W.shape[0],))
+    drop = dropout is not None and dropout.training and dropout.p > 0
+    return group_norm_act(y, gn.num_groups, gn.weight, gn.bias, gn.eps, act[0], act[1], residual,
+                          dropout_p=dropout.p if drop else 0.0, rng=dropout.take() if drop else None)

@@ -22,9 +22,9 @@ from .pointnet2_utils import three_interpolate, three_nn
 class GraspPoseStage1(nn.Module):
     """Backbone + graspable / approach-view head."""
 
-    def __init__(self, input_feature_dim=0, num_view=300, obs=False, is_training=True):
+    def __init__(self, input_feature_dim=0, num_view=300, obs=False, is_training=True, backbone_args=None):
         super().__init__()
-        self.FeatureExtraction = DRP()
+        self.FeatureExtraction = DRP(**(backbone_args or {}))
         self.GraspableClasification = GraspableDetection(num_view, 256)  # spelling = reference key name
         self.obs = obs
         self.is_training = is_training
@@ -148,10 +148,12 @@ class GraspPoseStage2_seed_features_multi_scale(nn.Module):
 class GraspBalance(nn.Module):
     def __init__(self, input_feature_dim=0, num_view=300, num_angle=12, num_depth=4, cylinder_radius=0.08,
                  hmin=-0.02, hmax_list=[0.01, 0.02, 0.03, 0.04], is_training=True, obs=False,
-                 fused_cylinder=True):
+                 fused_cylinder=True, backbone_args=None):
+        """backbone_args: keyword arguments of the DRP backbone (group norm, dropout, 8-bit products of its blocks)."""
         super().__init__()
         self.is_training = is_training
-        self.view_estimator = GraspPoseStage1(input_feature_dim, num_view, is_training=is_training, obs=obs)
+        self.view_estimator = GraspPoseStage1(input_feature_dim, num_view, is_training=is_training, obs=obs,
+                                              backbone_args=backbone_args)
         self.grasp_generator = GraspPoseStage2_seed_features_multi_scale(
             num_angle, num_depth, cylinder_radius, hmin, hmax_list, is_training, fused_cylinder=fused_cylinder)
 

@@ -37,11 +37,27 @@ class FastBatchNorm1d(nn.Module):
         raise ValueError("Non supported number of dimensions {}".format(x.dim()))
 
 
+class ChannelLastGroupNorm(nn.GroupNorm):
+    """nn.GroupNorm built from (channels, num_groups) like every norm of this factory, for (B, C, ...) tensors.  On the GPU
+    it runs on channel-last rows (fused_rows.group_norm_act), which is how this package keeps its activations: the result
+    is a channel-first view of them."""
+
+    def __init__(self, num_channels, num_groups=8, **kwargs):
+        super().__init__(num_groups, num_channels, **kwargs)
+
+    def forward(self, x):
+        from .. import fused_mlp, fused_rows
+        if not (fused_mlp.enabled(x) and fused_rows.supports(x)):
+            return super().forward(x)
+        return fused_rows.group_norm_act(x.movedim(1, -1), self.num_groups, self.weight, self.bias, self.eps).movedim(-1, 1)
+
+
 _NORM_LAYER = dict(
     bn1d=nn.BatchNorm1d, bn2d=nn.BatchNorm2d, bn=nn.BatchNorm2d, in2d=nn.InstanceNorm2d,
     in1d=nn.InstanceNorm1d, gn=nn.GroupNorm, syncbn=nn.SyncBatchNorm, ln=nn.LayerNorm,
     ln1d=LayerNorm1d, ln2d=LayerNorm2d, fastbn1d=FastBatchNorm1d, fastbn2d=FastBatchNorm1d,
     fastbn=FastBatchNorm1d,
+    gn1d=ChannelLastGroupNorm, gn2d=ChannelLastGroupNorm,   # 'gn' in a conv block (the reference's table has no such entry)
 )
 
 

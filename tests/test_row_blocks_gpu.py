@@ -1,0 +1,233 @@
+"""The row operators together, as the backbone's blocks use them: conv -> group norm + activation -> dropout, products in
+8-bit floats, residual; inside a train step of the whole network, eager and captured."""
+import copy
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from tests import f64_truth, row_truth
+from tests.seeded import fill_by_key
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _rel(a, b):
+    a, b = a.detach().double().cpu(), b.detach().double().cpu()
+    return float((a - b).norm() / (b.norm() + 1e-30))
+
+
+def _block(channels=32, norm=None, act='silu', **kw):
+    from graspbalance_amd.drp import InvResMLP
+    return InvResMLP(in_channels=channels, aggr_args={'feature_type': 'dp_fj', "reduction": 'max'},
+                     norm_args=norm or {'norm': 'gn', 'num_groups': 4}, act_args={'act': act},
+                     group_args={'NAME': 'ballquery', 'radius': 0.1, 'nsample': 16}, conv_args={'order': 'conv-norm-act'},
+                     expansion=4, use_res=True, **kw)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_group_norm_stage_fused_and_plain_vs_f64_truth(act):
+    """Two stacked blocks, forward and every gradient: at most twice as far from the fp64 truth as torch's plain
+    composition (GroupNorm and activation as modules on channel-first tensors)."""
+    from graspbalance_amd import fused_mlp
+    from graspbalance_amd.drp import run_stage
+    from graspbalance_amd.scene import make_batch
+    blocks = fill_by_key(nn.Sequential(*[_block(act=act) for _ in range(2)]), seed=4).to(DEV).train()
+    assert all(b.fusable_gn() and not b.fusable() for b in blocks)
+    p = torch.from_numpy(make_batch([0, 1], 1024)).to(DEV)
+    torch.manual_seed(4)
+    f0, w = torch.randn(2, 32, 1024, device=DEV), torch.randn(2, 32, 1024, device=DEV)
+
+    def run(mod, flag, dtype):
+        mod = copy.deepcopy(mod).to(dtype)
+        f = f0.detach().to(dtype).clone().requires_grad_(True)
+        fused_mlp.set_enabled(flag)
+        try:
+            if dtype == torch.float64:
+                with f64_truth.torch_geometry():
+                    _, out = run_stage(mod, p.to(dtype), f)
+            else:
+                _, out = run_stage(mod, p, f)
+            (out * w.to(dtype)).sum().backward()
+        finally:
+            fused_mlp.set_enabled(True)
+        return out.detach(), f.grad, torch.cat([q.grad.reshape(-1) for q in mod.parameters()])
+
+    fused, plain, truth = run(blocks, True, torch.float32), run(blocks, False, torch.float32), run(blocks, False, torch.float64)
+    assert _rel(fused[0], truth[0]) <= 1e-5
+    for i in range(3):
+        assert _rel(fused[i], truth[i]) <= 2.0 * _rel(plain[i], truth[i]) + 1e-6, (i, _rel(fused[i], truth[i]), _rel(plain[i], truth[i]))
+
+
+class _Codes(torch.autograd.Function):
+    """The 8-bit operand in 64 bits on the way forward, the gradient as it comes on the way back."""
+
+    @staticmethod
+    def forward(ctx, x, block_rows):
+        return row_truth.in_8_bits(x, block_rows)
+
+    @staticmethod
+    def backward(ctx, g):
+        return g, None
+
+
+class _CodedGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y):
+        return y.view_as(y)
+
+    @staticmethod
+    def backward(ctx, g):
+        return row_truth.in_8_bits(g, 1)
+
+
+def _layer(x, w, gn, act, fp8, residual=None, factor=None):
+    """conv -> group norm -> (+ residual) -> act -> dropout on (B, N, C) in double, by autograd."""
+    rows = x.reshape(-1, x.shape[-1])
+    y = _CodedGradient.apply(_Codes.apply(rows, 1) @ _Codes.apply(w, 128).t()) if fp8 else rows @ w.t()
+    y = y.view(x.shape[0], x.shape[1], -1).transpose(1, 2)
+    y = F.group_norm(y, gn.num_groups, gn.weight.double(), gn.bias.double(), gn.eps).transpose(1, 2)
+    if residual is not None:
+        y = y + residual
+    y = row_truth.act(y, act, 0.0)
+    return y if factor is None else y * factor
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_run_of_the_operators_together(fp8):
+    """expand (dropped out) -> contract (residual), as InvResMLP's pointwise pair: outputs and all gradients against the
+    composition in 64 bits.  In 8 bits an operand that lands within fp32 rounding (some 2^-22 of it) of the border
+    between two codes takes the other one, a step of up to 2^-3: of 2^-22 / 2^-4 of the elements, i.e. 2^-9 * 2^-3 of the
+    norm at most after three quantisers - 1e-3."""
+    from graspbalance_amd import fused_rows
+    torch.manual_seed(0)
+    B, N, C, E = 3, 217, 96, 384
+    conv0, conv1 = nn.Conv1d(C, E, 1, bias=False).to(DEV), nn.Conv1d(E, C, 1, bias=False).to(DEV)
+    gn0, gn1 = nn.GroupNorm(8, E).to(DEV), nn.GroupNorm(8, C).to(DEV)
+    for gn in (gn0, gn1):
+        nn.init.normal_(gn.weight, 1.0, 0.2)
+        nn.init.normal_(gn.bias, 0.0, 0.2)
+    drop = fused_rows.Dropout(0.2, seed=9).to(DEV)
+    x = torch.randn(B, N, C, device=DEV, requires_grad=True)
+    dy = torch.randn(B, N, C, device=DEV)
+    h = fused_rows.conv_gn_act(x, conv0, gn0, ("gelu", 0.0), fp8, dropout=drop)
+    y = fused_rows.conv_gn_act(h, conv1, gn1, ("gelu", 0.0), fp8, residual=x)
+    params = [x, conv0.weight, conv1.weight, gn0.weight, gn0.bias, gn1.weight, gn1.bias]
+    got = torch.autograd.grad(y, params, dy)
+    # the same in double on the CPU
+    keep, scale = row_truth.keep_mask(B * N * E, 0.2, 9, 0)
+    factor = keep.view(B, N, E).double() * scale
+    twin = copy.deepcopy(nn.ModuleList([conv0, conv1, gn0, gn1])).double().cpu()
+    xd = x.detach().double().cpu().requires_grad_()
+    hd = _layer(xd, twin[0].weight[:, :, 0], twin[2], "gelu", fp8, factor=factor)
+    yd = _layer(hd, twin[1].weight[:, :, 0], twin[3], "gelu", fp8, residual=xd)
+    want = torch.autograd.grad(yd, [xd, twin[0].weight, twin[1].weight, twin[2].weight, twin[2].bias, twin[3].weight, twin[3].bias],
+                               dy.double().cpu())
+    bound = 1e-3 if fp8 else 1e-5
+    assert _rel(y, yd) <= bound
+    for g, t in zip(got, want):
+        assert g.shape == t.shape and _rel(g, t) <= bound, (tuple(g.shape), _rel(g, t))
+    assert drop.rng.tolist() == [9, 1]
+
+
+def test_dropout_between_the_batch_norm_pair():
+    """norm 'bn' with dropout: the pair in two calls around the dropped features; in evaluation the block without it."""
+    from graspbalance_amd import fused_mlp, fused_rows
+    from graspbalance_amd.scene import make_batch
+    blk = fill_by_key(_block(norm={'norm': 'bn'}, act='relu', dropout=0.3), seed=2).to(DEV).train()
+    blk.dropout.rng.copy_(torch.tensor([5, 0]))
+    assert blk.fusable()
+    p = torch.from_numpy(make_batch([0], 1024)).to(DEV)
+    f = torch.randn(1, 1024, 32, device=DEV)
+    other = copy.deepcopy(blk)
+    out = blk.forward_cl(p, f)
+    assert blk.dropout.rng.tolist() == [5, 1]
+    seen = {}
+    other.dropout.forward = lambda h, residual=None: seen.setdefault("y", fused_rows.dropout(seen.setdefault("h", h), 0.3, (5, 0)))
+    again = other.forward_cl(p, f)
+    share = (seen["y"][seen["h"] != 0] == 0).double().mean().item()
+    n = int((seen["h"] != 0).sum())
+    assert abs(share - 0.3) < 6 * math.sqrt(0.21 / n) + 2.0 ** -16
+    # (the aggregation's sums are atomic: the two runs agree to rounding)
+    assert _rel(out, again) < 1e-5
+    blk.eval()
+    plain = copy.deepcopy(blk)
+    plain.dropout = None
+    assert _rel(blk.forward_cl(p, f), plain.forward_cl(p, f)) < 1e-6 and blk.dropout.rng.tolist() == [5, 1]
+
+
+def test_norm_factory_in_a_conv_block():
+    """create_convblock1d with 'gn': a channel-last result seen channel-first, values and gradients of F.group_norm."""
+    from graspbalance_amd.modified_net_tools.conv import create_convblock1d, create_convblock2d
+    torch.manual_seed(1)
+    for make, shape in ((create_convblock1d, (2, 24, 130)), (create_convblock2d, (2, 24, 10, 13))):
+        block = make(24, 48, norm_args={'norm': 'gn', 'num_groups': 6}, act_args={'act': 'gelu'}).to(DEV)
+        x = torch.randn(*shape, device=DEV, requires_grad=True)
+        y = block(x)
+        dy = torch.randn_like(y)
+        got = torch.autograd.grad(y, [x] + list(block.parameters()), dy)
+        twin = copy.deepcopy(block).double().cpu()
+        xd = x.detach().double().cpu().requires_grad_()
+        conv, norm = twin[0], twin[1]
+        yd = F.gelu(F.group_norm(conv(xd), 6, norm.weight, norm.bias, norm.eps))
+        want = torch.autograd.grad(yd, [xd] + list(twin.parameters()), dy.double().cpu())
+        assert y.shape == yd.shape and _rel(y, yd) < 1e-5
+        for g, t in zip(got, want):
+            assert _rel(g, t) < 1e-4
+
+
+def _tiny_net(**backbone_args):
+    from graspbalance_amd import backbone, graspbalance
+    saved = backbone.SA_SPECS
+    backbone.SA_SPECS = ((256, 0.08, 16, (None, 16, 16, 128)), (128, 0.15, 8, (128, 32, 32, 256)),
+                         (64, 0.3, 8, (256, 32, 32, 256)), (32, 0.5, 8, (256, 32, 32, 256)))
+    try:
+        torch.manual_seed(0)
+        return graspbalance.GraspBalance(num_view=30, backbone_args=backbone_args)
+    finally:
+        backbone.SA_SPECS = saved
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_network_trains_with_the_row_operators(fp8):
+    """A train step of the whole network whose blocks use group norm, dropout (and 8-bit products), launch by launch and as
+    captured graphs: finite losses, every parameter moves, every step draws its own numbers; then an evaluation pass."""
+    from graspbalance_amd.fused_rows import Dropout
+    from graspbalance_amd.synthetic import make_training_batch
+    from graspbalance_amd.train import Trainer
+    net = _tiny_net(norm_args={'norm': 'gn', 'num_groups': 8}, act_args={'act': 'silu'}, dropout=0.1, fp8=fp8)
+    batch = make_training_batch([0, 1], num_point=3000, num_objects=2, grasp_points_per_object=20, num_view=30, device=DEV)
+    for graph in (False, True):
+        tr = Trainer(DEV, num_view=30, model=copy.deepcopy(net), steps_per_epoch=10, max_epoch=2, graph=graph)
+        drops = [m for m in tr.net.modules() if isinstance(m, Dropout)]
+        assert len(drops) == 15 and len({int(d.rng[0]) for d in drops}) == 15
+        before = [p.detach().clone() for p in tr.net.view_estimator.FeatureExtraction.InvResMLP_blocks1.parameters()]
+        for step in range(3):
+            loss = tr.train_step(batch)
+            torch.cuda.synchronize()
+            assert bool(torch.isfinite(loss))
+            assert all(int(d.rng[1]) == step + 1 for d in drops)
+        after = list(tr.net.view_estimator.FeatureExtraction.InvResMLP_blocks1.parameters())
+        assert all(not torch.equal(a, b) and bool(torch.isfinite(b).all()) for a, b in zip(before, after))
+        tr.net.eval()
+        with torch.no_grad():
+            feats = tr.net.view_estimator.FeatureExtraction(batch['point_clouds'])[0]
+        assert bool(torch.isfinite(feats).all()) and all(int(d.rng[1]) == 3 for d in drops)
+
+
+def test_refusals_of_the_blocks():
+    with pytest.raises(ValueError):
+        _block(norm={'norm': 'bn'}, act='relu', fp8=True)
+    with pytest.raises(ValueError):
+        _block(dropout=0.1, num_posconvs=1)
+    from graspbalance_amd import fused_mlp
+    blk = _block(fp8=True).to(DEV)
+    fused_mlp.set_enabled(False)
+    try:
+        with pytest.raises(RuntimeError, match="fp8"):
+            blk([torch.randn(1, 64, 3, device=DEV), torch.randn(1, 32, 64, device=DEV)])
+    finally:
+        fused_mlp.set_enabled(True)
