@@ -47,8 +47,6 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 
 static constexpr int FP8_FEW_ROWS = 64;          // rows up to which the products run without LDS tiles
-static constexpr long long FP8_STREAM_ROWS = 32768;   // 512 tiles: below, the two-launch way is as fast (8192 x 128 -> 512 fp32:
-                                                      // 15.4 us in two launches, 18.1 streamed; 524288 x 256 -> 128 bf16: 212, 120)
 static constexpr int FP8_FUSED_CODES = 16384;    // bytes of codes a workgroup quantises for itself
 static constexpr int FP8_FUSED_ROWS = 16;
 
@@ -405,7 +403,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(GemmArgs8 g) {
 // keeps the weight and walks over tiles of 64 rows, 128 columns of X at a step: the next step's rows travel in registers
 // while this one is multiplied, are quantised into the other LDS buffer, and go to memory as codes only where the backward
 // pass wants them.  Against a quantising kernel and the tiles above: X's codes are not read back and there is one launch
-// (524288 x 128 -> 256 bf16: 123 us in two launches).  SUM: also the column sums of X, one LDS cell per lane.
+// (524288 x 128 -> 256 bf16: 123 us in two launches, 100 here: 470 MB at 4.7 TB/s, a large copy's rate).  SUM: also the column sums of X, one LDS cell per lane.
 struct StreamArgs8 {
   const void *x;
   const unsigned char *w, *w_scales;
@@ -760,12 +758,10 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_wgrad_kernel(WgradArgs8 g) {
     __syncthreads();
     for (long long p = p0; p < p1; p += 2 * STEP) {
       multiply(lds[0]);
-      __builtin_amdgcn_sched_barrier(0);
       put(lds[1], odd);
       fetch(p + 3 * STEP, odd);
       __syncthreads();
       multiply(lds[1]);   // (zeros where the range ends with an odd step)
-      __builtin_amdgcn_sched_barrier(0);
       put(lds[0], even);
       fetch(p + 4 * STEP, even);
       __syncthreads();
@@ -847,11 +843,15 @@ static int multiply_codes(const GemmArgs8 &g, int K, hipStream_t st) {
   return launch_tiles<T, 1, 2, 2, 1>(g, st);
 }
 
-// columns of the streaming kernel's variant; 0: not one of its shapes
+// Columns of the streaming kernel's variant; 0: not one of its shapes.  A weight of 128 x 128 is in LDS at once, and one
+// launch beats two from the first rows on (1024 rows fp32: 5.4 us against 6.7; 16384: 7.0, 9.4); a larger one has to be worth
+// its loading by every workgroup (8192 x 512 -> 128 bf16: 15.2 against 10.1, 16384 x 256 -> 256 fp32: 12.4 against 13.5,
+// 524288 x 256 -> 128 bf16: 120 against 212).
 static int stream_columns(long long P, int N, int K) {
-  if (P < FP8_STREAM_ROWS || N > 512) return 0;
+  if (P <= FP8_FEW_ROWS || N > 512) return 0;
   const int cols = N <= 128 ? 128 : N <= 256 ? 256 : 512;
-  return (long long)cols * blocks128(K) * 128 <= 65536 ? cols : 0;
+  const long long bytes = (long long)cols * blocks128(K) * 128;
+  return bytes <= 16384 || (bytes <= 65536 && P >= 16384) ? cols : 0;
 }
 struct StreamPlan8 {
   size_t lds;

@@ -189,7 +189,8 @@ class _GroupNormAct(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, offsets, cfg, rng):
         y, stats, used = _norm(x, weight, bias, residual, offsets, cfg, rng, True)
-        ctx.save_for_backward(x, weight, bias, residual, offsets, stats, used)
+        # (without an activation the gradient does not depend on the residual)
+        ctx.save_for_backward(x, weight, bias, residual if cfg[3] else None, offsets, stats, used)
         ctx.cfg, ctx.rng = cfg, None if used is not None else rng
         return y
 

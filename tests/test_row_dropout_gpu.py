@@ -54,6 +54,21 @@ def test_numbers_past_32_bits_of_elements():
     assert torch.equal(tail, torch.from_numpy(h >= 32768))
 
 
+def test_fp32_past_the_caches():
+    """Over 96 MB of fp32: the streamed form keeps the places and values of the others."""
+    from graspbalance_amd import fused_rows
+    n = (96 << 18) + 4099
+    x, res = torch.randn(n, device="cuda:0"), torch.randn(n, device="cuda:0")
+    for r in (None, res):
+        y = fused_rows.dropout(x, 0.4, (3, 7), residual=r)
+        cut = 1 << 20
+        head = fused_rows.dropout(x[:cut], 0.4, (3, 7), residual=None if r is None else r[:cut])
+        assert torch.equal(y[:cut], head)
+        keep, scale = row_truth.keep_mask(n, 0.4, 3, 7)
+        want = torch.where(keep.to("cuda:0"), x * scale, 0.0) + (0 if r is None else r)
+        assert bool(((y - want).abs() <= 4 * 2.0 ** -24 * (x.abs() * scale + want.abs())).all())
+
+
 def test_rates_and_independence():
     """The share of kept elements and of places kept by two calls: within 6 sigma of p and p^2."""
     from graspbalance_amd import fused_rows

@@ -122,6 +122,32 @@ def test_streamed_rows(P, K, N, dtype):
         assert torch.equal(fused_rows.fp8_linear(x, fused_rows.Fp8Weight.quantize(w), b), y)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("P,K,N", [(420000, 128, 128), (13000, 640, 4100)])
+def test_results_past_the_caches(P, K, N, dtype):
+    """Over 96 MB of x or y: streamed loads and stores, in both ways through the kernels; 300 rows against the truth, all of
+    them against the same rows in parts.  A part of many rows is added in the same order; the one row that is left over
+    goes through another kernel, whose sums are off by what _check allows fp32 sums, as the others are: twice that."""
+    from graspbalance_amd import fused_rows
+    x, w, b, _ = (t.to("cuda:0") for t in _data(P, K, N, dtype))
+    held = fused_rows.Fp8Weight.quantize(w)
+    y = fused_rows.fp8_linear(x, held, b)
+    pick = torch.randperm(P, generator=torch.Generator().manual_seed(0))[:300]
+    _check(y[pick.to("cuda:0")], row_truth.in_8_bits(x[pick.to("cuda:0")].cpu().double(), 1),
+           row_truth.in_8_bits(w.cpu().double(), 128), b.cpu().double(), dtype, "y")
+    part = P // 3
+    for lo in range(0, P, part):
+        mine, whole = fused_rows.fp8_linear(x[lo:lo + part], held, b), y[lo:lo + part]
+        if mine.shape[0] > 64:
+            assert torch.equal(mine, whole)
+        else:
+            xq, wq = row_truth.in_8_bits(x[lo:].cpu().double(), 1), row_truth.in_8_bits(w.cpu().double(), 128)
+            bound = 2.0 ** -24 * (K / 8 + 64) * (xq.abs() @ wq.abs().t() + b.cpu().double().abs()) + HALF[dtype] * whole.abs().cpu().double()
+            if dtype != torch.float32:
+                bound = bound + 128 * 2.0 ** -14 * (_maxima(xq) @ _maxima(wq).t())
+            assert bool(((mine - whole).abs().cpu().double() <= 2 * bound).all())
+
+
 def _codes(x):
     from graspbalance_amd import fused_rows
     codes, scales, _ = fused_rows._quantise_rows(x)

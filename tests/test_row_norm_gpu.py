@@ -110,6 +110,85 @@ def test_norm_shapes(shape, groups, dtype):
     _check(_inputs(R, C, dtype, False, seed=R + C), groups, dtype, "silu", shape=shape)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,groups", [((1, 400, 4096), 1), ((1, 400, 4096), 4096), ((1, 90, 4096), 512), ((300, 40, 16), 2),
+                                          ((2, 20000, 1023), 33)])
+def test_norm_wide_and_many(shape, groups, dtype):
+    """The widest rows read twice, groups of one channel, many samples, odd rows of a thousand channels."""
+    R, C = math.prod(shape[:-1]), shape[-1]
+    _check(_inputs(R, C, dtype, True, seed=R + C), groups, dtype, "gelu", shape=shape, p=0.1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tensors_past_the_caches(dtype):
+    """Over 96 MB: the streamed loads and stores.  The truth in 64 bits on the GPU; bounds as in _check for terms of size one
+    to ten (|x|, |dy| < 8, rstd < 2, |w| < 3): 32 U * 40 on y, 256 U * 40 on dx."""
+    from graspbalance_amd import fused_rows
+    rows, C, G = (110000, 128, 8) if dtype == torch.float32 else (110000, 264, 8)
+    g = torch.Generator(device="cuda:0").manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda:0")   # noqa: E731
+    x, dy = r(2, rows, C).to(dtype).requires_grad_(), r(2, rows, C).to(dtype)
+    w, b = (1 + 0.2 * r(C)).requires_grad_(), (0.2 * r(C)).requires_grad_()
+    assert x.numel() * x.element_size() > 96 << 20
+    y = fused_rows.group_norm_act(x, G, w, b, act="silu")
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+    half = HALF[dtype]
+    tw, tb = torch.zeros(C, dtype=torch.float64, device="cuda:0"), torch.zeros(C, dtype=torch.float64, device="cuda:0")
+    with torch.no_grad():
+        for s in range(2):
+            p = x[s].double().view(rows, G, C // G)
+            mean = p.mean((0, 2), keepdim=True)
+            rstd = 1 / torch.sqrt(((p - mean) ** 2).mean((0, 2), keepdim=True) + 1e-5)
+            xh = ((p - mean) * rstd).view(rows, C)
+            z = xh * w.double() + b.double()
+            sig = torch.sigmoid(z)
+            want = z * sig
+            assert bool(((y[s].double() - want).abs() <= half * want.abs() + 32 * 40 * U).all())
+            gr = dy[s].double() * (sig + z * sig * (1 - sig))
+            h, v = (gr * w.double()).view(rows, G, C // G), xh.view(rows, G, C // G)
+            want = ((h - h.mean((0, 2), keepdim=True) - v * (h * v).mean((0, 2), keepdim=True)) * rstd).view(rows, C)
+            assert bool(((dx[s].double() - want).abs() <= half * want.abs() + 256 * 40 * U).all())
+            tw += (gr * xh).sum(0)
+            tb += gr.sum(0)
+    # sums of 220000 terms of size ~1: fp32 over at most 64 of them, then 64 bits
+    assert bool(((dw.double() - tw).abs() <= 128 * U * 220000).all()) and bool(((db.double() - tb).abs() <= 128 * U * 220000).all())
+    assert float((dw.double() - tw).norm() / tw.norm()) < 1e-5
+
+
+def test_many_packed_samples():
+    """A thousand clouds of 0 to 40 rows, some of one row, against the same clouds one by one."""
+    from graspbalance_amd import fused_rows
+    g = torch.Generator().manual_seed(8)
+    sizes = torch.randint(0, 40, (1000,), generator=g)
+    off = torch.cat([torch.zeros(1, dtype=torch.int64), sizes.cumsum(0)])
+    R = int(off[-1])
+    case = _inputs(R, 48, torch.float32, False, seed=8)
+    _check(case, 6, torch.float32, "silu", cuts=off.tolist())
+    x = case["x"].to("cuda:0")
+    y = fused_rows.group_norm_act(x, 6, offsets=off.to("cuda:0"))
+    for s in (0, 17, 500, 999):
+        lo, hi = int(off[s]), int(off[s + 1])
+        if hi > lo:
+            one = fused_rows.group_norm_act(x[lo:hi].unsqueeze(0), 6)[0]
+            assert float((one - y[lo:hi]).abs().max()) <= 64 * U * (1 + float(one.abs().max()) * 40)
+
+
+def test_two_streams_at_once():
+    """Two calls in flight on two streams, with workspaces of their own."""
+    from graspbalance_amd import fused_rows
+    x = [torch.randn(4, 20000, 64, device="cuda:0") for _ in range(2)]
+    want = [fused_rows.group_norm_act(t, 8, act="gelu") for t in x]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(fused_rows.group_norm_act(x[i], 8, act="gelu"))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want[i]) for i in range(2) for a in got[i])
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "leaky_relu", "silu", "gelu"])
 @pytest.mark.parametrize("p", [0.0, 0.3])
 @pytest.mark.parametrize("shape,groups,dtype", [((2, 100, 40), 5, torch.float32), ((2, 4000, 72), 4, torch.bfloat16),
