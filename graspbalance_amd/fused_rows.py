@@ -282,37 +282,32 @@ def _up(n, m):
     return (n + m - 1) // m * m
 
 
-def _code_buffers(P, K, dev):
-    """Uninitialised (codes, scales) of rows (P, K), in one allocation."""
-    Kp, S = _up(K, 128), _up(_up(K, 128) // 128, 4)
-    both = torch.empty(P * (Kp + S) + 16, dtype=torch.uint8, device=dev)
-    at = _up(P * Kp, 16)
-    return both[:P * Kp].view(P, Kp), both[at:at + P * S].view(P, S)
+def _row_bytes(P, K):
+    """(bytes of the codes of rows (P, K), bytes of their exponents): kept one behind the other in one allocation."""
+    Kp = _up(K, 128)
+    return P * Kp, P * _up(Kp // 128, 4)
 
 
-def _quantise_rows(x2, colsum=False):
-    """(codes, scales, column sums | None) of rows (P, K)."""
+def _quantise_rows(x2):
+    """(codes, scales) of rows (P, K)."""
     P, K = x2.shape
-    dev = x2.device
-    codes, scales = _code_buffers(P, K, dev)
-    sums = torch.empty(K, dtype=torch.float32, device=dev) if colsum else None
-    ws, size = _fp8_workspace(_WS_COLSUM, P, K, 1, dev) if colsum else (None, 0)
-    _call("gb_fp8_quant_rows", dev, _lib.ptr(x2), _TYPES[x2.dtype], P, K, _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(sums),
-          _lib.ptr(ws), size, _s(x2))
-    return codes, scales, sums
+    n, m = _row_bytes(P, K)
+    both = torch.empty(n + m, dtype=torch.uint8, device=x2.device)
+    _quantise_rows_to(x2, both.data_ptr(), None, None, 0)
+    return both[:n].view(P, -1), both[n:].view(P, -1)
 
 
-def _fp8_product(x2, w, w_scales, transposed, N, bias, keep, colsum):
-    """(y (P, N), codes, scales, column sums) of rows x2 and a weight's codes; what is not asked for is None."""
+def _quantise_rows_to(x2, at, sums, ws, size):
     P, K = x2.shape
-    dev = x2.device
-    y = torch.empty((P, N), dtype=x2.dtype, device=dev)
-    codes, scales = _code_buffers(P, K, dev) if keep else (None, None)
-    sums = torch.empty(K, dtype=torch.float32, device=dev) if colsum else None
-    ws, size = _fp8_workspace(_WS_LINEAR + _KEEP * keep + _SUM * colsum, P, N, K, dev)
-    _call("gb_fp8_linear", dev, _lib.ptr(x2), _TYPES[x2.dtype], P, K, _lib.ptr(w), _lib.ptr(w_scales), transposed, N,
-          _lib.ptr(bias), _lib.ptr(y), _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(sums), _lib.ptr(ws), size, _s(x2))
-    return y, codes, scales, sums
+    _call("gb_fp8_quant_rows", x2.device, x2.data_ptr(), _TYPES[x2.dtype], P, K, at, at + _row_bytes(P, K)[0], _lib.ptr(sums), ws,
+          size, _s(x2))
+
+
+def _product_to(x2, y, w, w_scales, transposed, N, bias, keep_at, sums, ws, size):
+    """gb_fp8_linear: y (P, N) of rows x2 and a weight's codes; keep_at: where x2's codes and exponents go, or None."""
+    P, K = x2.shape
+    _call("gb_fp8_linear", x2.device, x2.data_ptr(), _TYPES[x2.dtype], P, K, w, w_scales, transposed, N, _lib.ptr(bias),
+          y.data_ptr(), keep_at, None if keep_at is None else keep_at + _row_bytes(P, K)[0], _lib.ptr(sums), ws, size, _s(x2))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -322,21 +317,29 @@ def _fp8_workspace_bytes(what, P, N, K):
     return size.value
 
 
-def _fp8_workspace(what, P, N, K, dev):
-    size = _fp8_workspace_bytes(what, P, N, K)
-    return _bytes(size, dev), size
+class _Codes:
+    """Addresses of a weight's codes, transposed codes (None where nobody asked) and exponents, and what holds them."""
+    __slots__ = ("N", "K", "codes", "codes_t", "scales", "held")
 
+    @classmethod
+    def of(cls, weight):
+        """Of an Fp8Weight."""
+        c = cls()
+        c.N, c.K, c.held = weight.out_features, weight.in_features, (weight.codes, weight.scales, weight.codes_t)
+        c.codes, c.scales, c.codes_t = (_lib.ptr(t) for t in c.held)
+        return c
 
-def _quantise_weight(w, transposed):
-    """(codes, codes_t | None, scales) of a weight (N, K)."""
-    N, K = w.shape
-    dev = w.device
-    codes = torch.empty((N, _up(K, 128)), dtype=torch.uint8, device=dev)
-    codes_t = torch.empty((K, _up(N, 128)), dtype=torch.uint8, device=dev) if transposed else None
-    scales = torch.empty((_up(N, 128) // 128, _up(K, 128) // 128), dtype=torch.uint8, device=dev)
-    _call("gb_fp8_quant_weight", dev, _lib.ptr(w), _TYPES[w.dtype], N, K, _lib.ptr(codes), _lib.ptr(codes_t), _lib.ptr(scales),
-          _s(w))
-    return codes, codes_t, scales
+    @classmethod
+    def quantise(cls, w, transposed):
+        """Of a float weight (N, K), in one allocation (held) in that order."""
+        c = cls()
+        c.N, c.K = w.shape
+        n, m = c.N * _up(c.K, 128), c.K * _up(c.N, 128) if transposed else 0
+        c.held = torch.empty(n + m + _up(c.N, 128) // 128 * (_up(c.K, 128) // 128), dtype=torch.uint8, device=w.device)
+        c.codes = c.held.data_ptr()
+        c.codes_t, c.scales = c.codes + n if transposed else None, c.codes + n + m
+        _call("gb_fp8_quant_weight", w.device, w.data_ptr(), _TYPES[w.dtype], c.N, c.K, c.codes, c.codes_t, c.scales, _s(w))
+        return c
 
 
 class Fp8Weight:
@@ -366,9 +369,11 @@ class Fp8Weight:
     def quantize(cls, weight, input_gradients=False):
         """From a float weight (out_features, in_features); input_gradients: also what fp8_linear's backward pass needs."""
         w = _fp8_weight_tensor("Fp8Weight", weight.detach()).contiguous()
-        codes, codes_t, scales = _quantise_weight(w, input_gradients)
-        view = lambda t: None if t is None else t.view(torch.float8_e4m3fn)   # noqa: E731
-        return cls(view(codes), scales, w.shape[1], view(codes_t))
+        N, K = w.shape
+        held = _Codes.quantise(w, input_gradients).held
+        n, m = N * _up(K, 128), K * _up(N, 128) if input_gradients else 0
+        return cls(held[:n].view(N, -1).view(torch.float8_e4m3fn), held[n + m:].view(_up(N, 128) // 128, -1), K,
+                   held[n:n + m].view(K, -1).view(torch.float8_e4m3fn) if input_gradients else None)
 
 
 def _fp8_weight_tensor(what, w):
@@ -378,42 +383,60 @@ def _fp8_weight_tensor(what, w):
     return w.view(w.shape[0], w.shape[1]) if w.dim() > 2 else w
 
 
+def _fp8_forward(x, weight, bias, need_x, keep):
+    """(y, the weight's _Codes, x's codes and exponents | None)"""
+    dev = x.device
+    P, K = x.shape
+    w = _Codes.of(weight) if isinstance(weight, Fp8Weight) else _Codes.quantise(weight, need_x)
+    if need_x and w.codes_t is None:
+        _refuse("fp8_linear", "gradients of the input need Fp8Weight.quantize(weight, input_gradients=True)")
+    y = torch.empty((P, w.N), dtype=x.dtype, device=dev)
+    kept = torch.empty(sum(_row_bytes(P, K)), dtype=torch.uint8, device=dev) if keep else None
+    size = _fp8_workspace_bytes(_WS_LINEAR + _KEEP * keep, P, w.N, K)
+    ws = _bytes(size, dev)
+    _product_to(x, y, w.codes, w.scales, 0, w.N, bias, _lib.ptr(kept), None, _lib.ptr(ws), size)
+    return y, w, kept
+
+
 class _Fp8Linear(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, held):
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        if held is None:
-            weight = weight.contiguous()
-            N = weight.shape[0]
-            codes, codes_t, scales = _quantise_weight(weight, need_x)
-        else:
-            N, codes, codes_t, scales = held.out_features, held.codes, held.codes_t, held.scales
-            if need_x and codes_t is None:
-                _refuse("fp8_linear", "gradients of the input need Fp8Weight.quantize(weight, input_gradients=True)")
-        y, xq, xs, _ = _fp8_product(x, codes, scales, 0, N, bias, need_w, False)
+        need_x, need_w = ctx.needs_input_grad[:2]
+        y, w, kept = _fp8_forward(x, weight if held is None else held, bias, need_x, need_w)
         # one byte per element of x stays for the backward pass
-        ctx.save_for_backward(xq, xs, *((codes_t, scales) if need_x else (None, None)))
-        ctx.dims = (N, x.shape[1], None if held is not None else weight.dtype)
+        ctx.save_for_backward(kept)
+        ctx.w = w if need_x else None
+        ctx.dims = (w.N, w.K, None if held is not None else weight.dtype)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        xq, xs, codes_t, scales = ctx.saved_tensors
+        kept, = ctx.saved_tensors
         N, K, wtype = ctx.dims
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dy = dy.contiguous()
+        dev, P = dy.device, dy.shape[0]
+        # dy's codes, then a workspace for one kernel after the other
+        codes = sum(_row_bytes(P, N)) if need_w or not need_x else 0
+        first = _fp8_workspace_bytes(_WS_LINEAR + _KEEP * (codes > 0) + _SUM * need_b, P, K, N) if need_x else \
+            _fp8_workspace_bytes(_WS_COLSUM, P, N, 1) if need_b else 0
+        second = _fp8_workspace_bytes(_WS_WGRAD, P, N, K) if need_w else 0
+        room = _up(codes, 16)
+        scratch = torch.empty(room + max(first, second), dtype=torch.uint8, device=dev)
+        at = scratch.data_ptr()
         dx = dw = None
+        db = torch.empty(N, dtype=torch.float32, device=dev) if need_b else None
         if need_x:
-            dx, dq, ds, db = _fp8_product(dy, codes_t, scales, 1, K, None, need_w, need_b)
+            dx = torch.empty((P, K), dtype=dy.dtype, device=dev)
+            _product_to(dy, dx, ctx.w.codes_t, ctx.w.scales, 1, K, None, at if codes else None, db, at + room, first)
         else:
-            dq, ds, db = _quantise_rows(dy, colsum=need_b)
+            _quantise_rows_to(dy, at, db, at + room, first)
         if need_w:
-            dev, P = dy.device, dy.shape[0]
             dw = torch.empty((N, K), dtype=torch.float32, device=dev)
-            ws, size = _fp8_workspace(_WS_WGRAD, P, N, K, dev)
-            _call("gb_fp8_wgrad", dev, _lib.ptr(dq), _lib.ptr(ds), _lib.ptr(xq), _lib.ptr(xs), _lib.ptr(dw), P, N, K,
-                  _lib.ptr(ws), size, _s(dy))
+            x_at = kept.data_ptr()
+            _call("gb_fp8_wgrad", dev, at, at + _row_bytes(P, N)[0], x_at, x_at + _row_bytes(P, K)[0], dw.data_ptr(), P, N, K,
+                  at + room, second, _s(dy))
             dw = dw if wtype == torch.float32 else dw.to(wtype)
         return dx, dw, db, None
 
@@ -441,13 +464,12 @@ def fp8_linear(x, weight, bias=None):
     if x.dim() < 1 or x.shape[-1] != K:
         _refuse(what, "x must be (..., %d)" % K)
     bias = _channel_vector(what, "bias", bias, N, x)
-    weight = None if held is not None else weight
     rows = (x if x.dim() == 2 else x.reshape(-1, K)).contiguous()
+    weight = None if held is not None else weight.contiguous()
     if _grads(x, weight, bias):
         y = _Fp8Linear.apply(rows, weight, bias, held)
     else:
-        codes, scales = (held.codes, held.scales) if held is not None else _quantise_weight(weight.contiguous(), False)[::2]
-        y = _fp8_product(rows, codes, scales, 0, N, bias, False, False)[0]
+        y = _fp8_forward(rows, weight if held is None else held, bias, False, False)[0]
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (N,))
 
 
