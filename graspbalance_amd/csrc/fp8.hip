@@ -117,16 +117,18 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const T *__restrict__ x, 
   }
 }
 
+// the workgroups' sums of a column, joined: 8 columns x 32 lanes, in 64 bits
 __global__ __launch_bounds__(256) void fp8_colsum_kernel(const float *__restrict__ part, int chunks, int K, float *__restrict__ out) {
-  __shared__ double lds[8][32];
-  const int i = (int)threadIdx.x & 31, q = (int)threadIdx.x >> 5, c = (int)blockIdx.x * 32 + i;
+  __shared__ double lds[32][8];
+  const int i = (int)threadIdx.x & 7, q = (int)threadIdx.x >> 3, c = (int)blockIdx.x * 8 + i;
   double s = 0;
   if (c < K)
-    for (int j = q; j < chunks; j += 8) s += part[(long long)j * K + c];
+#pragma unroll 4
+    for (int j = q; j < chunks; j += 32) s += part[(long long)j * K + c];
   lds[q][i] = s;
   __syncthreads();
   if (q == 0 && c < K) {
-    for (int j = 1; j < 8; ++j) s += lds[j][i];
+    for (int j = 1; j < 32; ++j) s += lds[j][i];
     out[c] = (float)s;
   }
 }
@@ -569,18 +571,18 @@ __global__ __launch_bounds__(256, 2) void fp8_stream_kernel(StreamArgs8 g) {
 // reads 32 codes of W straight into the operand of a 16-row step (the four lanes of a row read one 128-byte line), and the
 // waves' sums meet in LDS.  FUSED: every workgroup quantises the few rows of X for itself (one launch instead of two); the
 // first one stores the codes where somebody wants them.
-template <typename T, int PT, bool FUSED>
-__global__ __launch_bounds__(256) void fp8_few_kernel(GemmArgs8 g, const T *__restrict__ x, int K, unsigned char *__restrict__ codes_out,
+template <typename T, int PT, int NW, bool FUSED>
+__global__ __launch_bounds__(64 * NW) void fp8_few_kernel(GemmArgs8 g, const T *__restrict__ x, int K, unsigned char *__restrict__ codes_out,
                                                       unsigned char *__restrict__ scales_out) {
   constexpr bool EXACT = Exact<T>::value;
-  __shared__ float sums[4][PT][64][4];
+  __shared__ float sums[NW][PT][64][4];
   extern __shared__ __attribute__((aligned(16))) unsigned char codes[];   // FUSED: P x Kp codes, P x Kb exponents
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, j = lane & 15, q = lane >> 4;
   const int n0 = (int)blockIdx.x * 16, Kp = g.Kb * 128, P = (int)g.P;
   const unsigned char *ex = codes + P * Kp;
   if (FUSED) {
     const int cl = (int)threadIdx.x & 15;
-    for (int i = (int)threadIdx.x >> 4; i < P * g.Kb; i += 16) {
+    for (int i = (int)threadIdx.x >> 4; i < P * g.Kb; i += 4 * NW) {
       const int r = i / g.Kb, kb = i - r * g.Kb, col = kb * 128 + cl * 8;
       const F8 f = load_upto8(x + (long long)r * K + col, K - col);
       const int e = block_exponent(row_max_f32(top8(f)));
@@ -603,7 +605,7 @@ __global__ __launch_bounds__(256) void fp8_few_kernel(GemmArgs8 g, const T *__re
     acc[t] = f32x4{};
     row[t] = 16 * t + j < P ? 16 * t + j : P - 1;
   }
-  for (int kb = wave; kb < g.Kb; kb += 4) {
+  for (int kb = wave; kb < g.Kb; kb += NW) {
     const i32x4 w0 = *reinterpret_cast<const i32x4 *>(w + kb * 128), w1 = *reinterpret_cast<const i32x4 *>(w + kb * 128 + 16);
     const int sw = bs[(long long)kb * g.bs_k];
 #pragma unroll
@@ -631,15 +633,16 @@ __global__ __launch_bounds__(256) void fp8_few_kernel(GemmArgs8 g, const T *__re
 #pragma unroll
     for (int i = 0; i < 4; ++i) sums[wave][t][lane][i] = acc[t][i];
   __syncthreads();
-  if (wave >= PT) return;
-  for (int t = wave; t < PT; t += 4) {   // lane: row 16 t + j, outputs n0 + 4 q ..
+  for (int t = wave; t < PT; t += NW) {   // lane: row 16 t + j, outputs n0 + 4 q ..
     const int r = 16 * t + j;
     if (r >= P) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int c = n0 + 4 * q + i;
       if (c >= g.N) break;
-      const float s = (sums[0][t][lane][i] + sums[1][t][lane][i]) + (sums[2][t][lane][i] + sums[3][t][lane][i]);
+      float s = sums[0][t][lane][i];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) s += sums[w][t][lane][i];
       ((T *)g.y)[(long long)r * g.N + c] = (T)(s + (g.bias ? g.bias[c] : 0.0f));
     }
   }
@@ -823,17 +826,25 @@ static int launch_tiles(const GemmArgs8 &g, hipStream_t st) {
 }
 
 static long long tiles_of(long long P, int N, int b) { return ((P + b - 1) / b) * ((N + b - 1) / b); }
+template <typename T, int PT, bool FUSED>
+static void launch_few(const GemmArgs8 &g, const T *x, int K, unsigned char *codes, unsigned char *scales, size_t lds, hipStream_t st) {
+  const unsigned grid = (unsigned)((g.N + 15) / 16);
+  if (g.Kb >= 8)   // (a wave per block of a long reduction: 4 x 4096 -> 4096 fp32 9.7 us with four waves, 6.7 with eight)
+    fp8_few_kernel<T, PT, 8, FUSED><<<grid, 512, lds, st>>>(g, x, K, codes, scales);
+  else
+    fp8_few_kernel<T, PT, 4, FUSED><<<grid, 256, lds, st>>>(g, x, K, codes, scales);
+}
+
 // y from codes and exponents in memory
 template <typename T>
 static int multiply_codes(const GemmArgs8 &g, int K, hipStream_t st) {
   if (g.P <= FP8_FEW_ROWS) {
-    const unsigned grid = (unsigned)((g.N + 15) / 16);
     if (g.P <= 16)
-      fp8_few_kernel<T, 1, false><<<grid, 256, 0, st>>>(g, nullptr, K, nullptr, nullptr);
+      launch_few<T, 1, false>(g, nullptr, K, nullptr, nullptr, 0, st);
     else if (g.P <= 32)
-      fp8_few_kernel<T, 2, false><<<grid, 256, 0, st>>>(g, nullptr, K, nullptr, nullptr);
+      launch_few<T, 2, false>(g, nullptr, K, nullptr, nullptr, 0, st);
     else
-      fp8_few_kernel<T, 4, false><<<grid, 256, 0, st>>>(g, nullptr, K, nullptr, nullptr);
+      launch_few<T, 4, false>(g, nullptr, K, nullptr, nullptr, 0, st);
     return check_launch("gb_fp8_linear");
   }
   // 256 x 256 where that still gives every CU a tile, the columns fill it as well as 128 do to a fifth, and there are steps
@@ -893,10 +904,12 @@ static bool fp8_dims_large(long long P, int N, int K) {   // int tile offsets: 2
   return N > (1 << 22) || K > (1 << 22) || P > (1ll << 40);
 }
 
-static int rows_per_chunk(long long P, bool sum) {
-  if (!sum) return 64;
+// Rows of a workgroup: sixteen (one access a lane) until that fills the device, then 64; with column sums as many as leave
+// at most 512 partial ones.  (64 x 4096 with 64 rows each: 32 workgroups of four accesses one after the other, 14 us.)
+static int rows_per_chunk(long long P, int K, bool sum) {
+  if (!sum) return P / 16 * blocks128(K) < 8192 ? 16 : 64;
   const long long per = (P + 511) / 512;
-  return (int)(per < 64 ? 64 : (per + 15) / 16 * 16);
+  return (int)(per < 16 ? 16 : (per + 15) / 16 * 16);
 }
 
 struct WgradPlan8 {
@@ -928,7 +941,7 @@ extern "C" int gb_fp8_quant_rows(const void *x, int dtype, long long P, int K, v
                                  long long ws_bytes, void *stream) {
   if (fp8_dims_bad(P, 1, K) || !known_type(dtype)) return GB_EINVAL;
   if (fp8_dims_large(P, 1, K)) return GB_ERANGE;
-  const int per = rows_per_chunk(P, colsum != nullptr);
+  const int per = rows_per_chunk(P, K, colsum != nullptr);
   const long long chunks = (P + per - 1) / per;
   if (chunks > 0x7fffffffll || blocks128(K) > 65535) return GB_ERANGE;
   if (P == 0 && !colsum) return GB_OK;
@@ -941,7 +954,7 @@ extern "C" int gb_fp8_quant_rows(const void *x, int dtype, long long P, int K, v
     if (colsum) {
       if (P > 0)
         fp8_rows_kernel<T, true><<<grid, 256, 0, st>>>((const T *)x, P, K, (unsigned char *)codes, (unsigned char *)scales, per, (float *)ws);
-      fp8_colsum_kernel<<<(K + 31) / 32, 256, 0, st>>>((const float *)ws, (int)chunks, K, colsum);
+      fp8_colsum_kernel<<<(K + 7) / 8, 256, 0, st>>>((const float *)ws, (int)chunks, K, colsum);
     } else {
       fp8_rows_kernel<T, false><<<grid, 256, 0, st>>>((const T *)x, P, K, (unsigned char *)codes, (unsigned char *)scales, per, nullptr);
     }
@@ -975,7 +988,7 @@ static long long linear_workspace(long long P, int N, int K, bool keeps, bool su
   const int route = linear_route(P, N, K);
   long long b = 0;
   if (sum) {
-    const long long per = rows_per_chunk(P, true),
+    const long long per = rows_per_chunk(P, K, true),
                     chunks = route == FP8_STREAM ? stream_plan(P, stream_columns(P, N, K), K, GB_T_BF16, true).grid : (P + per - 1) / per;
     b += up16(chunks * K * 4);
   }
@@ -997,7 +1010,7 @@ extern "C" int gb_fp8_linear(const void *x, int dtype, long long P, int K, const
   hipStream_t st = as_stream(stream);
   if (P == 0) {
     if (!colsum) return GB_OK;
-    fp8_colsum_kernel<<<(K + 31) / 32, 256, 0, st>>>((const float *)ws, 0, K, colsum);
+    fp8_colsum_kernel<<<(K + 7) / 8, 256, 0, st>>>((const float *)ws, 0, K, colsum);
     return check_launch("gb_fp8_linear");
   }
   const int route = linear_route(P, N, K), Kb = blocks128(K), bs_n = transposed ? 1 : Kb, bs_k = transposed ? blocks128(N) : 1;
@@ -1024,7 +1037,7 @@ extern "C" int gb_fp8_linear(const void *x, int dtype, long long P, int K, const
       return colsum ? stream_rows<T, true>(g, p, cols, st) : stream_rows<T, false>(g, p, cols, st);
     });
     if (rc || !colsum) return rc;
-    fp8_colsum_kernel<<<(K + 31) / 32, 256, 0, st>>>((const float *)ws, p.grid, K, colsum);
+    fp8_colsum_kernel<<<(K + 7) / 8, 256, 0, st>>>((const float *)ws, p.grid, K, colsum);
     return check_launch("gb_fp8_linear");
   }
   GemmArgs8 g = {};
@@ -1042,7 +1055,7 @@ extern "C" int gb_fp8_linear(const void *x, int dtype, long long P, int K, const
     const size_t lds = (size_t)up16(P * Kb * 129);
     return with_type(dtype, [&](auto z) {
       typedef decltype(z) T;
-      fp8_few_kernel<T, 1, true><<<(unsigned)((N + 15) / 16), 256, lds, st>>>(g, (const T *)x, K, (unsigned char *)codes, (unsigned char *)scales);
+      launch_few<T, 1, true>(g, (const T *)x, K, (unsigned char *)codes, (unsigned char *)scales, lds, st);
       return check_launch("gb_fp8_linear");
     });
   }
@@ -1066,7 +1079,7 @@ extern "C" int gb_fp8_workspace(int what, long long P, int N, int K, long long *
   if (fp8_dims_bad(P, N, K) || !bytes || (what != GB_FP8_WS_COLSUM && what != GB_FP8_WS_WGRAD && (what < GB_FP8_WS_LINEAR || what >= GB_FP8_WS_LINEAR + 4))) return GB_EINVAL;
   if (fp8_dims_large(P, N, K)) return GB_ERANGE;
   if (what == GB_FP8_WS_COLSUM) {
-    const int per = rows_per_chunk(P, true);
+    const int per = rows_per_chunk(P, K, true);
     *bytes = (P + per - 1) / per * N * 4;
   } else if (what >= GB_FP8_WS_LINEAR) {
     *bytes = linear_workspace(P, N, K, (what - GB_FP8_WS_LINEAR) & GB_FP8_KEEP, (what - GB_FP8_WS_LINEAR) & GB_FP8_SUM);

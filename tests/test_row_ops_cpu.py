@@ -131,12 +131,13 @@ def test_fp8_refuses_on_the_host():
     refused(L.gb_fp8_linear, big, [(13, None, -1), (14, size.value - 1, -1)])
     assert L.gb_fp8_workspace(5, 1000, 1024, 1024, ctypes.byref(size)) == 0 and size.value == 0
     big[12] = 64      # column sums
-    refused(L.gb_fp8_linear, big, [(14, 1000 * (1024 + 8) - 1, -1)])
+    assert L.gb_fp8_workspace(6, 1000, 1024, 1024, ctypes.byref(size)) == 0 and size.value > 1000 * (1024 + 8)
+    refused(L.gb_fp8_linear, big, [(14, size.value - 1, -1)])
     refused(L.gb_fp8_wgrad, [64, 64, 64, 64, 64, 8, 8, 8, None, 0, None],
             [(0, None, -1), (0, 72, -1), (1, None, -1), (2, None, -1), (2, 72, -1), (3, None, -1), (4, None, -1), (5, -1, -1),
              (6, 0, -1), (7, 0, -1), (7, 1 << 23, -3), (5, 100000, -1)])
     assert L.gb_fp8_linear(None, 0, 0, 8, None, None, 0, 8, None, None, None, None, None, None, 0, None) == 0
-    assert L.gb_fp8_workspace(0, 100, 30, 1, ctypes.byref(size)) == 0 and size.value == 2 * 30 * 4
+    assert L.gb_fp8_workspace(0, 100, 30, 1, ctypes.byref(size)) == 0 and size.value > 0 and size.value % (30 * 4) == 0
 
 
 def test_the_oracle_of_8_bits_agrees_with_torchs_cast():
