@@ -224,6 +224,31 @@ __device__ __forceinline__ void multiply64(f32x16 (&acc)[TM][TN], const i32x4 (&
   }
 }
 
+// The same for 128 codes from LDS: la, lb are the lane's rows of the operands (128 bytes each, chunks permuted as below).
+template <bool EXACT, int TM, int TN>
+__device__ __forceinline__ void multiply128(f32x16 (&acc)[TM][TN], const unsigned char *la, const unsigned char *lb, int lane,
+                                            const int (&sa)[TM], int sb) {
+  const int h = lane >> 5, x = lane >> 1 & 7;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {   // 64 codes: lane half h holds 32 of them
+    const int c0 = ((4 * s + 2 * h) ^ x) * 16, c1 = ((4 * s + 2 * h + 1) ^ x) * 16;
+    i32x4 fa[TM][2], fb[TN][2];
+#pragma unroll
+    for (int n = 0; n < TN; ++n) {
+      const unsigned char *r = lb + 32 * n * 128;
+      fb[n][0] = *reinterpret_cast<const i32x4 *>(r + c0);
+      fb[n][1] = *reinterpret_cast<const i32x4 *>(r + c1);
+    }
+#pragma unroll
+    for (int m = 0; m < TM; ++m) {
+      const unsigned char *r = la + 32 * m * 128;
+      fa[m][0] = *reinterpret_cast<const i32x4 *>(r + c0);
+      fa[m][1] = *reinterpret_cast<const i32x4 *>(r + c1);
+    }
+    multiply64<EXACT, TM, TN>(acc, fa, fb, sa, sb);
+  }
+}
+
 // A wave's results to memory: lane j of a pair of tiles has columns 2 j, 2 j + 1 of 64 (from col0 of N) and, of every eight
 // rows, 4 h .. 4 h + 3.  Eight rows at a time go through the wave's own LDS cell and leave as 16 bytes per lane, whole
 // 128-byte lines: stored from where they are (4 bytes a lane) they took 75 of the 120 us of 524288 x 128 -> 256 bf16.
@@ -306,13 +331,20 @@ __device__ __forceinline__ void dma16(const unsigned char *src, unsigned char *l
 // the row of W at place `at` of LDS
 __device__ __forceinline__ int weight_row(int at) { return (at & ~63) + 2 * (at & 31) + (at >> 5 & 1); }
 
-template <typename T, int TM, int TN, int WM, int WN, bool NT>
-__global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(GemmArgs8 g) {
+// G > 1 (few tiles, a long reduction): G groups of WM x WN waves with stages of their own take a range of the steps each, and
+// their sums meet in LDS, added in the groups' order.  A lone group is bound by its own steps, one after the other (~0.6 us
+// each: waits for LDS and the matrix pipe; four stages in flight instead of two gained 3 us in 21 for 16 bits and lost as much
+// for fp32).  128 x 4096 -> 4096 bf16 with its quantiser 21.0 -> 14.7 us, fp32 24.7 -> 16.3; 512 x 1024 -> 1024 8.8 -> 8.3.
+template <typename T, int TM, int TN, int WM, int WN, int G, bool NT>
+__global__ __launch_bounds__(64 * WM * WN * G) void fp8_gemm_kernel(GemmArgs8 g) {
   constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, WAVES = WM * WN, ROWS = BM + BN, LOADS = ROWS / (8 * WAVES);
   constexpr bool EXACT = Exact<T>::value;
   static_assert(TN % 2 == 0 && ROWS % (8 * WAVES) == 0 && (32 * TN) <= 128, "tile");
-  extern __shared__ __attribute__((aligned(128))) unsigned char stages[];   // one, or two where there is a second step
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave / WN, wn = wave % WN, j = lane & 31, h = lane >> 5;
+  static_assert((G - 1) * WAVES * TM * TN * 4096 + WAVES * Cell<T>::BYTES <= G * 2 * ROWS * 128, "the groups' sums");
+  extern __shared__ __attribute__((aligned(128))) unsigned char lds[];   // per group: one stage, or two where there is a second step
+  const int lane = (int)threadIdx.x & 63, at = (int)threadIdx.x >> 6, group = at / WAVES, wave = at % WAVES, wm = wave / WN, wn = wave % WN,
+            j = lane & 31;
+  unsigned char *stages = lds + group * (2 * ROWS * 128);
   // neighbouring tiles on one XCD (workgroups go to the eight XCDs in turn): its L2 then holds their common rows
   const long long per = g.tiles >> 3, extra = g.tiles & 7, x = blockIdx.x & 7;
   const long long tile = x * per + (x < extra ? x : extra) + (blockIdx.x >> 3);
@@ -343,6 +375,8 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(GemmArgs8 g) {
   for (int m = 0; m < TM; ++m)
 #pragma unroll
     for (int n = 0; n < TN; ++n) acc[m][n] = f32x16{};
+  const int steps = G > 1 ? ((g.Kb + G - 1) / G + 3) / 4 * 4 : g.Kb;   // (a range starts with a dword of four exponents)
+  const int k0 = G > 1 ? group * steps : 0, k1 = G > 1 && k0 + steps < g.Kb ? k0 + steps : g.Kb;
   const unsigned char *as[TM];
   unsigned sa[TM], sa_next[TM];
 #pragma unroll
@@ -352,52 +386,64 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(GemmArgs8 g) {
   }
   const int nb = (n0 + wn * 32 * TN) / 128, nbs = nb < (g.N + 127) / 128 ? nb : (g.N + 127) / 128 - 1;
   const unsigned char *bs = g.b_scales + (long long)nbs * g.bs_n;
-
-  request(0, stages);
+  unsigned sb_next = 0;
+  if (k0 < k1) {
+    request(k0, stages);
 #pragma unroll
-  for (int m = 0; m < TM; ++m) sa_next[m] = *reinterpret_cast<const unsigned *>(as[m]);
-  unsigned sb_next = bs[0];
-  for (int kb = 0; kb < g.Kb; ++kb) {
+    for (int m = 0; m < TM; ++m) sa_next[m] = *reinterpret_cast<const unsigned *>(as[m] + k0);
+    sb_next = bs[(long long)k0 * g.bs_k];
+  }
+  for (int i = 0; i < steps; ++i) {
+    const int kb = k0 + i;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();   // this stage is complete, and nobody reads the other one any more
+    if (G > 1 && kb >= k1) continue;   // (the last group's range may be shorter)
     const unsigned sb = sb_next;
     if ((kb & 3) == 0)
 #pragma unroll
       for (int m = 0; m < TM; ++m) sa[m] = sa_next[m];
-    if (kb + 1 < g.Kb) {   // the next step's codes and exponents travel while this one is multiplied
-      request(kb + 1, stages + ((kb + 1) & 1) * (ROWS * 128));
+    if (kb + 1 < k1) {   // the next step's codes and exponents travel while this one is multiplied
+      request(kb + 1, stages + ((i + 1) & 1) * (ROWS * 128));
       sb_next = bs[(long long)(kb + 1) * g.bs_k];
       if ((kb & 3) == 3)
 #pragma unroll
         for (int m = 0; m < TM; ++m) sa_next[m] = *reinterpret_cast<const unsigned *>(as[m] + kb + 1);
     }
-    const unsigned char *st = stages + (kb & 1) * (ROWS * 128);
+    const unsigned char *st = stages + (i & 1) * (ROWS * 128);
     int s8[TM];
 #pragma unroll
     for (int m = 0; m < TM; ++m) s8[m] = (int)(sa[m] >> (8 * (kb & 3)) & 0xff);
-    const unsigned char *la = st + (wm * 32 * TM + j) * 128, *lb = st + (BM + wn * 32 * TN + j) * 128;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {   // 64 codes: lane half h holds 32 of them
-      const int c0 = ((4 * s + 2 * h) ^ (j >> 1 & 7)) * 16, c1 = ((4 * s + 2 * h + 1) ^ (j >> 1 & 7)) * 16;
-      i32x4 fa[TM][2], fb[TN][2];
-#pragma unroll
-      for (int n = 0; n < TN; ++n) {
-        const unsigned char *r = lb + 32 * n * 128;
-        fb[n][0] = *reinterpret_cast<const i32x4 *>(r + c0);
-        fb[n][1] = *reinterpret_cast<const i32x4 *>(r + c1);
-      }
-#pragma unroll
-      for (int m = 0; m < TM; ++m) {
-        const unsigned char *r = la + 32 * m * 128;
-        fa[m][0] = *reinterpret_cast<const i32x4 *>(r + c0);
-        fa[m][1] = *reinterpret_cast<const i32x4 *>(r + c1);
-      }
-      multiply64<EXACT, TM, TN>(acc, fa, fb, s8, (int)sb);
-    }
+    multiply128<EXACT, TM, TN>(acc, st + (wm * 32 * TM + j) * 128, st + (BM + wn * 32 * TN + j) * 128, lane, s8, (int)sb);
   }
-  __syncthreads();   // (the stages become the waves' cells)
+  __syncthreads();   // (the stages become the groups' sums, then the waves' cells)
+  if (G > 1) {
+    f32x4 *sums = reinterpret_cast<f32x4 *>(lds) + wave * (TM * TN * 256) + lane;   // [group - 1][wave][tile][quarter][lane]
+    if (group > 0)
+#pragma unroll
+      for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int n = 0; n < TN; ++n)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            sums[(group - 1) * (WAVES * TM * TN * 256) + ((m * TN + n) * 4 + q) * 64] =
+                f32x4{acc[m][n][4 * q], acc[m][n][4 * q + 1], acc[m][n][4 * q + 2], acc[m][n][4 * q + 3]};
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int o = 0; o < G - 1; ++o)
+#pragma unroll
+      for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int n = 0; n < TN; ++n)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 v = sums[o * (WAVES * TM * TN * 256) + ((m * TN + n) * 4 + q) * 64];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[m][n][4 * q + i] += v[i];
+          }
+  }
   store_tiles<T, TM, TN, NT>(acc, (T *)g.y + p0 * g.N, g.bias, g.N, n0 + wn * 32 * TN, wm * 32 * TM, lane, last_a + 1,
-                             stages + wave * Cell<T>::BYTES);
+                             lds + (G > 1 ? (G - 1) * WAVES * TM * TN * 4096 : 0) + wave * Cell<T>::BYTES);
 }
 
 // ---- streamed rows --------------------------------------------------------------------------------------------------
@@ -430,7 +476,7 @@ __global__ __launch_bounds__(256, 2) void fp8_stream_kernel(StreamArgs8 g) {
   const int Kb = blocks128(g.K), Kp = Kb * 128, ss = scale_stride(g.K);
   unsigned char *ws = smem, *xs = ws + Kb * BN * 128, *es = xs + 2 * BM * 128;
   float *sums = reinterpret_cast<float *>(es + 2 * BM + 4 * Cell<T>::BYTES);   // SUM: [16][Kp]
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave / WN, wn = wave % WN, j = lane & 31, h = lane >> 5;
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave / WN, wn = wave % WN, j = lane & 31;
   const int cl = (int)threadIdx.x & 15, rl = (int)threadIdx.x >> 4;
   const T *x = (const T *)g.x;
 
@@ -523,24 +569,7 @@ __global__ __launch_bounds__(256, 2) void fp8_stream_kernel(StreamArgs8 g) {
     int sa[TM];
 #pragma unroll
     for (int m = 0; m < TM; ++m) sa[m] = es[buf * BM + wm * 32 * TM + 32 * m + j];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int c0 = ((4 * s + 2 * h) ^ (j >> 1 & 7)) * 16, c1 = ((4 * s + 2 * h + 1) ^ (j >> 1 & 7)) * 16;
-      i32x4 fa[TM][2], fb[TN][2];
-#pragma unroll
-      for (int n = 0; n < TN; ++n) {
-        const unsigned char *r = lb + 32 * n * 128;
-        fb[n][0] = *reinterpret_cast<const i32x4 *>(r + c0);
-        fb[n][1] = *reinterpret_cast<const i32x4 *>(r + c1);
-      }
-#pragma unroll
-      for (int m = 0; m < TM; ++m) {
-        const unsigned char *r = la + 32 * m * 128;
-        fa[m][0] = *reinterpret_cast<const i32x4 *>(r + c0);
-        fa[m][1] = *reinterpret_cast<const i32x4 *>(r + c1);
-      }
-      multiply64<EXACT, TM, TN>(acc, fa, fb, sa, sb);
-    }
+    multiply128<EXACT, TM, TN>(acc, la, lb, lane, sa, sb);
     if (last) {
       T *y = (T *)g.y + tile * BM * g.N;
       const int rows = (int)(g.P - tile * BM < BM ? g.P - tile * BM : BM);
@@ -806,23 +835,18 @@ __global__ __launch_bounds__(256) void fp8_wgrad_join_kernel(const float *__rest
 
 // ---- host -----------------------------------------------------------------------------------------------------------
 
-template <typename T, int TM, int TN, int WM, int WN, bool NT>
-static int launch_tiles_nt(GemmArgs8 g, hipStream_t st) {
+template <typename T, int TM, int TN, int WM, int WN, int G, bool NT>
+static int launch_tiles(GemmArgs8 g, hipStream_t st) {
   constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, STAGE = (BM + BN) * 128;
   g.tiles_n = (g.N + BN - 1) / BN;
   g.tiles = (g.P + BM - 1) / BM * g.tiles_n;
   if (g.tiles > 0x7fffffffll) return GB_ERANGE;
-  if (2 * STAGE > 65536) {
+  if (2 * G * STAGE > 65536) {
     static std::atomic<unsigned long long> done{0};
-    allow_dynamic_lds(fp8_gemm_kernel<T, TM, TN, WM, WN, NT>, 2 * STAGE, done);
+    allow_dynamic_lds(fp8_gemm_kernel<T, TM, TN, WM, WN, G, NT>, 2 * G * STAGE, done);
   }
-  fp8_gemm_kernel<T, TM, TN, WM, WN, NT><<<(unsigned)g.tiles, 64 * WM * WN, (g.Kb > 1 ? 2 : 1) * STAGE, st>>>(g);
+  fp8_gemm_kernel<T, TM, TN, WM, WN, G, NT><<<(unsigned)g.tiles, 64 * WM * WN * G, (g.Kb > 1 ? 2 * G : 1) * STAGE, st>>>(g);
   return check_launch("gb_fp8_linear");
-}
-template <typename T, int TM, int TN, int WM, int WN>
-static int launch_tiles(const GemmArgs8 &g, hipStream_t st) {
-  return streams(g.P * g.N * (long long)sizeof(T)) ? launch_tiles_nt<T, TM, TN, WM, WN, true>(g, st)
-                                                   : launch_tiles_nt<T, TM, TN, WM, WN, false>(g, st);
 }
 
 static long long tiles_of(long long P, int N, int b) { return ((P + b - 1) / b) * ((N + b - 1) / b); }
@@ -838,7 +862,8 @@ static void launch_few(const GemmArgs8 &g, const T *x, int K, unsigned char *cod
 // y from codes and exponents in memory
 template <typename T>
 static int multiply_codes(const GemmArgs8 &g, int K, hipStream_t st) {
-  if (g.P <= FP8_FEW_ROWS) {
+  // (64 x 4096 -> 4096 bf16: 18.2 us without tiles, 13.7 with four groups of waves a tile; 64 x 1024 -> 1024: 7.6, 8.4)
+  if (g.P <= FP8_FEW_ROWS && !(g.P > 32 && g.Kb >= 32)) {
     if (g.P <= 16)
       launch_few<T, 1, false>(g, nullptr, K, nullptr, nullptr, 0, st);
     else if (g.P <= 32)
@@ -848,10 +873,17 @@ static int multiply_codes(const GemmArgs8 &g, int K, hipStream_t st) {
     return check_launch("gb_fp8_linear");
   }
   // 256 x 256 where that still gives every CU a tile, the columns fill it as well as 128 do to a fifth, and there are steps
-  // enough to work through; short reductions live from several workgroups per CU, which only smaller tiles leave room for.
-  if (g.Kb >= 4 && tiles_of(g.P, g.N, 256) >= 256 && 5 * blocks128(g.N) >= 8 * ((g.N + 255) / 256)) return launch_tiles<T, 4, 2, 2, 4>(g, st);
-  if (tiles_of(g.P, g.N, 128) >= 256) return launch_tiles<T, 2, 2, 2, 2>(g, st);
-  return launch_tiles<T, 1, 2, 2, 1>(g, st);
+  // enough to work through; short reductions live from several workgroups per CU, which only smaller tiles leave room for.  Tiles of 64 x 64 that leave
+  // CUs idle get groups of waves: four up to a tile per CU, two up to two tiles (1024 x 4096 -> 4096 bf16: 34 us in tiles of
+  // 128 x 128, 46 in 1024 of these).
+  const bool nt = streams(g.P * g.N * (long long)sizeof(T));
+  if (g.Kb >= 4 && tiles_of(g.P, g.N, 256) >= 256 && 5 * blocks128(g.N) >= 8 * ((g.N + 255) / 256))
+    return nt ? launch_tiles<T, 4, 2, 2, 4, 1, true>(g, st) : launch_tiles<T, 4, 2, 2, 4, 1, false>(g, st);
+  if (tiles_of(g.P, g.N, 128) >= 256) return nt ? launch_tiles<T, 2, 2, 2, 2, 1, true>(g, st) : launch_tiles<T, 2, 2, 2, 2, 1, false>(g, st);
+  const long long tiles = tiles_of(g.P, g.N, 64);
+  if (g.Kb >= 8 && tiles <= 512)
+    return tiles <= 256 ? launch_tiles<T, 1, 2, 2, 1, 4, false>(g, st) : launch_tiles<T, 1, 2, 2, 1, 2, false>(g, st);
+  return launch_tiles<T, 1, 2, 2, 1, 1, false>(g, st);
 }
 
 // Columns of the streaming kernel's variant; 0: not one of its shapes.  A weight of 128 x 128 is in LDS at once, and one
@@ -905,9 +937,14 @@ static bool fp8_dims_large(long long P, int N, int K) {   // int tile offsets: 2
 }
 
 // Rows of a workgroup: sixteen (one access a lane) until that fills the device, then 64; with column sums as many as leave
-// at most 512 partial ones.  (64 x 4096 with 64 rows each: 32 workgroups of four accesses one after the other, 14 us.)
+// at most 512 partial ones.  (8192 x 128
+// fp32 in chunks of 64 rows 4.8 us, of sixteen 3.7.)
 static int rows_per_chunk(long long P, int K, bool sum) {
-  if (!sum) return P / 16 * blocks128(K) < 8192 ? 16 : 64;
+  if (!sum) {
+    if (P / 16 * blocks128(K) < 8192) return 16;
+    const long long per = (P >> 23) / 16 * 16 + 16;   // (a launch has fewer than 2^32 lanes)
+    return per < 64 ? 64 : (int)per;
+  }
   const long long per = (P + 511) / 512;
   return (int)(per < 16 ? 16 : (per + 15) / 16 * 16);
 }

@@ -22,7 +22,7 @@ namespace gb {
 
 static constexpr int GN_MAX_C = 4096;   // two doubles per channel in LDS while a workgroup's sums are joined
 static constexpr int GN_DIRECT = 32;    // workgroups per sample up to which every applying one adds their sums for itself:
-                                        // a launch less (4 x 1024 x 256 bf16: 40 -> 30 us of kernels and gaps a pass)
+                                        // a launch less each way (4 x 1024 x 256 bf16: 41 -> 37 us of kernels a pass)
 static constexpr int GN_DIRECT_GROUPS = 256;
 static constexpr int GN_MIN_STEPS = 4;  // of a workgroup: with fewer, joining the sums costs what the parallelism gains
 

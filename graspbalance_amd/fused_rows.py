@@ -132,8 +132,9 @@ def dropout(x, p, rng, residual=None):
 
 class Dropout(nn.Module):
     """dropout() as a layer: owns its [seed, call] pair on the device as the buffer ``rng`` (saved with the module) and moves
-    to the next call at every training forward - also at every replay of a captured one.  Without a seed, one is drawn from
-    torch's CPU generator."""
+    to the next call at every training forward - also at every replay of a captured one, and at a recomputed one: under
+    activation checkpointing call dropout() with a pair of your own.  Without a seed, one is drawn from torch's CPU generator;
+    ranks that draw the same one (or share their buffers) drop the same places of their own rows."""
 
     def __init__(self, p=0.5, seed=None):
         super().__init__()

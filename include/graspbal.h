@@ -760,9 +760,10 @@ int gb_group_norm_bwd(const GbGroupNorm *n, const void *dy, void *dx, void *dres
  * gb_fp8_quant_weight: w (N, K) -> codes (N, Kp), block scales, and codes_t (K, Np) = the transposed codes unless NULL.
  * gb_fp8_linear: y (P, N) = deq(Q(x)) deq(w)^T + bias, x (P, K) in floats, w (N, K) by blocks; transposed != 0: w is the
  *   codes_t of a weight (K, N) whose scales are given as they are.  fp32: codes multiplied as bf16 with fp32 sums (values
- *   below 2^-126 count as zero); 16 bits: 8-bit matrix instructions, whose steps add 64 or 128 products with about 14 bits
- *   below the largest before the fp32 sum.  codes, scales: NULL, or x's by rows are kept there; colsum: as above; bias:
- *   (N) fp32 or NULL.  ws: gb_fp8_workspace LINEAR (+ KEEP with codes, + SUM with colsum), 16-byte aligned.
+ *   below 2^-126 count as zero, those that round to 2^128 as infinite); 16 bits: 8-bit matrix instructions, whose steps add
+ *   64 or 128 products with about 14 bits below the largest before the fp32 sum.  codes, scales: NULL, or x's by rows are
+ *   kept there; colsum: as above; bias: (N) fp32 or NULL.  ws: gb_fp8_workspace LINEAR (+ KEEP with codes, + SUM with
+ *   colsum), 16-byte aligned.
  * gb_fp8_wgrad: dw (N, K) fp32 = deq(dy)^T deq(x), dy (P, N) and x (P, K) by rows (ws: gb_fp8_workspace WGRAD); bf16 products
  *   with fp32 sums in a fixed order.                                                                                    */
 #define GB_FP8_WS_COLSUM 0

@@ -122,6 +122,24 @@ def test_streamed_rows(P, K, N, dtype):
         assert torch.equal(fused_rows.fp8_linear(x, fused_rows.Fp8Weight.quantize(w), b), y)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("P,K,N", [(33, 4096, 70), (64, 4300, 130), (65, 1030, 64), (200, 1153, 321), (1000, 2100, 100),
+                                   (1100, 1100, 1100), (2100, 1664, 515)])
+def test_long_reductions_of_few_tiles(P, K, N, dtype):
+    """The steps split over groups of waves: two and four of them, ranges that are short or empty, tiles that end inside."""
+    from graspbalance_amd import fused_rows
+    x, w, b, _ = _data(P, K, N, dtype)
+    held = fused_rows.Fp8Weight.quantize(w.to("cuda:0"))
+    y = fused_rows.fp8_linear(x.to("cuda:0"), held, b.to("cuda:0"))
+    _check(y, row_truth.in_8_bits(x.double(), 1), row_truth.in_8_bits(w.double(), 128), b.double(), dtype, "y")
+    assert torch.equal(y, fused_rows.fp8_linear(x.to("cuda:0"), held, b.to("cuda:0")))
+    bad = x.clone()
+    bad[P // 2, K - 1] = float("nan")
+    again = fused_rows.fp8_linear(bad.to("cuda:0"), held, b.to("cuda:0"))
+    rest = torch.arange(P, device="cuda:0") != P // 2
+    assert bool(torch.isnan(again[P // 2]).all()) and torch.equal(again[rest], y[rest])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("P,K,N", [(420000, 128, 128), (13000, 640, 4100)])
 def test_results_past_the_caches(P, K, N, dtype):
