@@ -84,6 +84,15 @@ def _grads(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _once(backward):
+    """once_differentiable without its 3 - 5 us where no graph of the backward pass is being recorded."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, dy):
+        return guarded(ctx, dy) if torch.is_grad_enabled() else backward(ctx, dy)
+    return run
+
+
 def _dropout(x, residual, q, rng, keep):
     """(y, the pair that was used | None)"""
     y = torch.empty_like(x)
@@ -104,7 +113,7 @@ class _Dropout(Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         dx = None
         if ctx.needs_input_grad[0]:
@@ -196,7 +205,7 @@ class _GroupNormAct(Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, bias, residual, offsets, stats, used = ctx.saved_tensors
         samples, groups, _, act, _, q = cfg = ctx.cfg
@@ -411,7 +420,7 @@ class _Fp8Linear(Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         kept, = ctx.saved_tensors
         N, K, wtype = ctx.dims
