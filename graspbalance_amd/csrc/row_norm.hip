@@ -830,11 +830,15 @@ static int lds_tree(int T, int PL) {  // join_columns: most lanes that give thei
   return RL > 1 ? (RL - h > h / 2 ? RL - h : h / 2) * PL : 0;
 }
 
-// Workgroups per sample: as many as are resident at once (waves per SIMD by the kernel's registers), so that there is no
-// last round of a few (4 x 131072 x 128 fp32 statistics: 68 us with 2048 workgroups where 1536 fit, 45 with 2048 where
-// 2048 do).  Packed samples may be of very different lengths and are cut twice as fine.
-static int spread(const GbGroupNorm *n, long long steps, long long resident) {
-  const long long most = resident * (n->offsets ? 2 : 1) / n->samples, want = (steps + GN_MIN_STEPS - 1) / GN_MIN_STEPS;
+// Workgroups per sample: as many as fill the device with `waves` per SIMD, so that there is no last round of a few.  Where
+// bytes alone bind, two waves, each with a long stretch of its own (4 x 131072 x 128 fp32 relu forward / backward: with what
+// the registers allow 132 / 238 us, two 127 / 229, one 141 / 256; 8 x 131072 x 128 bf16: 144 / 244, 130 / 232, 159 / 291).  Where
+// there is arithmetic to hide, what the registers allow (4 x 131072 x 128 bf16 gelu + residual + dropout: 124 / 216 us, two
+// 133 / 233).  Packed samples may be of very different lengths: as many, cut twice as fine.
+static int spread(const GbGroupNorm *n, long long steps, int block, bool backward) {
+  const bool light = n->act <= GB_ACT_LEAKY_RELU && n->q == 0 && !n->offsets;
+  const int waves = light ? 2 : n->dtype == GB_T_F32 ? (backward ? 5 : 8) : (backward ? 4 : 6);
+  const long long most = 256ll * 4 * 64 * waves / block * (n->offsets ? 2 : 1) / n->samples, want = (steps + GN_MIN_STEPS - 1) / GN_MIN_STEPS;
   const long long ns = want < most ? want : most;
   return (int)(ns < 1 ? 1 : ns);
 }
@@ -873,10 +877,9 @@ static GnPlan gn_plan(const GbGroupNorm *n, bool backward) {
     p.block = p.PL <= 256 ? 256 : p.PL <= 512 ? 512 : 1024;
     const int T = p.block / p.PL * p.PL;
     const long long units = (longest * C + N - 1) / N, steps = (units + T - 1) / T;
-    const int waves = N == 4 ? (backward ? 5 : 8) : (backward ? 4 : 6);   // per SIMD, by the kernels' registers
-    p.ns = spread(n, steps, 256ll * 4 * waves * 64 / p.block);
-    // a few more steps each rather than a launch more
-    if (p.ns > GN_DIRECT && p.ns <= 2 * GN_DIRECT) p.ns = GN_DIRECT;
+    p.ns = spread(n, steps, p.block, backward);
+    // short samples: a few more steps each rather than a launch more
+    if (p.ns > GN_DIRECT && steps <= 2ll * GN_DIRECT * GN_MIN_STEPS) p.ns = GN_DIRECT;
   }
   p.direct = !p.sub && p.ns <= GN_DIRECT && (backward || n->groups <= GN_DIRECT_GROUPS);
   p.T = p.block / p.PL * p.PL;

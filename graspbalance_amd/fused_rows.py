@@ -189,7 +189,7 @@ def _norm(x, weight, bias, residual, offsets, cfg, rng, keep):
     at, seed, call = _rng_args(rng)
     used = torch.empty_like(rng) if keep and at is not None else None
     n = _norm_struct(x, weight, bias, residual, offsets, stats, at, _lib.ptr(used), seed, call, cfg)
-    size = _norm_workspace_bytes(n.rows, samples, n.channels, groups, n.dtype, offsets is not None, 0)
+    size = _norm_workspace_bytes(n.rows, samples, n.channels, groups, n.dtype, n.act, n.q, offsets is not None, 0)
     ws = _bytes(size, dev)
     _call("gb_group_norm_fwd", dev, ctypes.byref(n), y.data_ptr(), _lib.ptr(ws), size, _s(x))
     return y, stats, used
@@ -221,7 +221,7 @@ class _GroupNormAct(Function):
         db = make(C, dtype=torch.float32, device=dev) if need_b else None
         at, seed, call = _rng_args(used if ctx.rng is None else ctx.rng)
         n = _norm_struct(x, weight, bias, residual, offsets, stats, at, None, seed, call, cfg)
-        size = _norm_workspace_bytes(n.rows, samples, C, groups, n.dtype, offsets is not None, 1)
+        size = _norm_workspace_bytes(n.rows, samples, C, groups, n.dtype, act, q, offsets is not None, 1)
         ws = _bytes(size, dev)
         _call("gb_group_norm_bwd", dev, ctypes.byref(n), dy.data_ptr(), dx.data_ptr(), _lib.ptr(dres), _lib.ptr(dw),
               _lib.ptr(db), _lib.ptr(ws), size, _s(x))
@@ -229,8 +229,9 @@ class _GroupNormAct(Function):
 
 
 @functools.lru_cache(maxsize=1024)
-def _norm_workspace_bytes(rows, samples, channels, groups, dtype, packed, backward):
-    n = _lib.GroupNorm(rows=rows, samples=samples, channels=channels, groups=groups, dtype=dtype, offsets=8 if packed else None)
+def _norm_workspace_bytes(rows, samples, channels, groups, dtype, act, q, packed, backward):
+    n = _lib.GroupNorm(rows=rows, samples=samples, channels=channels, groups=groups, dtype=dtype, act=act, q=q,
+                       offsets=8 if packed else None)
     size = ctypes.c_longlong()
     _lib.check(_lib.lib().gb_group_norm_workspace(ctypes.byref(n), backward, ctypes.byref(size)), "group_norm_act")
     return size.value

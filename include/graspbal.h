@@ -730,7 +730,8 @@ int gb_dropout(const void *x, const void *residual, void *y, long long n, int dt
  *     - else GB_ERANGE.
  *   rng / seed / call / used: as gb_dropout; _bwd takes the pair that _fwd used (as rng or by value; `used` is not written).
  * _bwd: dx, dresidual (may be NULL) like x; dweight, dbias (channels) fp32 (either may be NULL).  x, residual (not read
- * under GB_ACT_NONE), act, q must be those of _fwd.  ws: gb_group_norm_workspace bytes, 16-byte aligned.  All sums are
+ * under GB_ACT_NONE), act, q must be those of _fwd.  ws: gb_group_norm_workspace bytes (of the same struct), 16-byte
+ * aligned.  All sums are
  * added in a fixed order: results repeat bit for bit.  rows == 0: nothing is launched or written.                      */
 typedef struct GbGroupNorm {
   const void *x, *residual;
