@@ -833,10 +833,12 @@ static int lds_tree(int T, int PL) {  // join_columns: most lanes that give thei
 // Workgroups per sample: as many as fill the device with `waves` per SIMD, so that there is no last round of a few.  Where
 // bytes alone bind, two waves, each with a long stretch of its own (4 x 131072 x 128 fp32 relu forward / backward: with what
 // the registers allow 132 / 238 us, two 127 / 229, one 141 / 256; 8 x 131072 x 128 bf16: 144 / 244, 130 / 232, 159 / 291).  Where
-// there is arithmetic to hide, what the registers allow (4 x 131072 x 128 bf16 gelu + residual + dropout: 124 / 216 us, two
-// 133 / 233).  Packed samples may be of very different lengths: as many, cut twice as fine.
+// there is arithmetic to hide - dropout, gelu on 16-bit elements - what the registers allow (4 x 131072 x 128 bf16 gelu +
+// residual: 110 / 210 us, two 114 / 214; with dropout 124 / 216, two 133 / 233; but 8 x 131072 x 128 bf16 silu + residual 180 /
+// 344, two 171 / 329, and 4 x 65536 x 128 fp32 gelu + residual 90 / 169, two 88 / 162).  Packed samples may be of very different
+// lengths: as many, cut twice as fine.
 static int spread(const GbGroupNorm *n, long long steps, int block, bool backward) {
-  const bool light = n->act <= GB_ACT_LEAKY_RELU && n->q == 0 && !n->offsets;
+  const bool light = n->q == 0 && !(n->act == GB_ACT_GELU && n->dtype != GB_T_F32) && !n->offsets;
   const int waves = light ? 2 : n->dtype == GB_T_F32 ? (backward ? 5 : 8) : (backward ? 4 : 6);
   const long long most = 256ll * 4 * 64 * waves / block * (n->offsets ? 2 : 1) / n->samples, want = (steps + GN_MIN_STEPS - 1) / GN_MIN_STEPS;
   const long long ns = want < most ? want : most;
