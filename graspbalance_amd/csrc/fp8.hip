@@ -7,14 +7,17 @@
 // floating format nothing (scaling by it is exact), is what the matrix instructions take beside their operands, and is
 // exact in bf16.
 //
-// Two inner products, chosen by the output's type:
-//   16-bit outputs: v_mfma_scale_f32_32x32x64_f8f6f4 - 4.0 PFLOP/s on this card with random codes (4.7 with zeros: the clock
-//     falls with the power), scales applied by the instruction.  It adds
-//     the products of a step with about 14 bits below the largest one (measured: 5e-5 of the result's norm for codes over
-//     the whole range, 0 where they span 2^4), then accumulates in fp32: a twentieth of bf16's half step, a quarter of
-//     fp16's.
-//   fp32 outputs: the codes are turned into bf16 (exact) in registers, scale included, and go through
-//     v_mfma_f32_32x32x16_bf16 (1.76 PFLOP/s with random values; 8e-8 of the norm).
+// Two inner products:
+//   EXACT (fp32 outputs, and 16-bit ones unless the caller asks for the other): the codes are turned into bf16 (exact) in
+//     registers, scale included, and go through v_mfma_f32_32x32x16_bf16, whose sums are fp32 (1.76 PFLOP/s on this card with
+//     random values; 8e-8 of the result's norm).
+//   GB_FP8_SHORT_SUMS (16-bit outputs): v_mfma_scale_f32_32x32x64_f8f6f4 - 4.0 PFLOP/s with random codes (4.7 with zeros: the
+//     clock falls with the power), scales applied by the instruction.  It adds the products of a step of 64 or 128 with
+//     about 14 bits below the largest one, then accumulates in fp32: measured 5e-5 of the result's norm for codes over the
+//     whole range, 0 where they span 2^4 - a twentieth of bf16's half step, a quarter of fp16's.  Fewer than 32 bits of a sum
+//     are the caller's choice, so this form is never taken unasked.
+#include <type_traits>
+
 #include "row_common.h"
 
 #pragma clang fp contract(on)
@@ -188,11 +191,6 @@ __device__ __forceinline__ bf16x8 decode8(unsigned lo, unsigned hi, float scale)
   return r;
 }
 
-template <typename T>
-struct Exact {  // fp32 outputs take the bf16 products
-  static constexpr bool value = sizeof(T) == 4;
-};
-
 // 64 codes of the reduction into TM x TN tiles: fa, fb are a lane's 32 codes of its rows, sa, sb their biased exponents
 template <bool EXACT, int TM, int TN>
 __device__ __forceinline__ void multiply64(f32x16 (&acc)[TM][TN], const i32x4 (&fa)[TM][2], const i32x4 (&fb)[TN][2], const int (&sa)[TM],
@@ -335,10 +333,9 @@ __device__ __forceinline__ int weight_row(int at) { return (at & ~63) + 2 * (at 
 // their sums meet in LDS, added in the groups' order.  A lone group is bound by its own steps, one after the other (~0.6 us
 // each: waits for LDS and the matrix pipe; four stages in flight instead of two gained 3 us in 21 for 16 bits and lost as much
 // for fp32).  128 x 4096 -> 4096 bf16 with its quantiser 21.0 -> 14.7 us, fp32 24.7 -> 16.3; 512 x 1024 -> 1024 8.8 -> 8.3.
-template <typename T, int TM, int TN, int WM, int WN, int G, bool NT>
+template <typename T, bool EXACT, int TM, int TN, int WM, int WN, int G, bool NT>
 __global__ __launch_bounds__(64 * WM * WN * G) void fp8_gemm_kernel(GemmArgs8 g) {
   constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, WAVES = WM * WN, ROWS = BM + BN, LOADS = ROWS / (8 * WAVES);
-  constexpr bool EXACT = Exact<T>::value;
   static_assert(TN % 2 == 0 && ROWS % (8 * WAVES) == 0 && (32 * TN) <= 128, "tile");
   static_assert((G - 1) * WAVES * TM * TN * 4096 + WAVES * Cell<T>::BYTES <= G * 2 * ROWS * 128, "the groups' sums");
   extern __shared__ __attribute__((aligned(128))) unsigned char lds[];   // per group: one stage, or two where there is a second step
@@ -467,10 +464,9 @@ struct Eight {
   T v[8];
 };
 
-template <typename T, int TM, int TN, int WM, int WN, bool SUM, bool NT>
+template <typename T, bool EXACT, int TM, int TN, int WM, int WN, bool SUM, bool NT>
 __global__ __launch_bounds__(256, 2) void fp8_stream_kernel(StreamArgs8 g) {
   constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, SLOTS = BM / 16;
-  constexpr bool EXACT = Exact<T>::value;
   static_assert(WM * WN == 4 && BM == 64 && TN % 2 == 0 && 32 * TN <= 128, "tile");
   extern __shared__ __attribute__((aligned(128))) unsigned char smem[];
   const int Kb = blocks128(g.K), Kp = Kb * 128, ss = scale_stride(g.K);
@@ -600,10 +596,9 @@ __global__ __launch_bounds__(256, 2) void fp8_stream_kernel(StreamArgs8 g) {
 // reads 32 codes of W straight into the operand of a 16-row step (the four lanes of a row read one 128-byte line), and the
 // waves' sums meet in LDS.  FUSED: every workgroup quantises the few rows of X for itself (one launch instead of two); the
 // first one stores the codes where somebody wants them.
-template <typename T, int PT, int NW, bool FUSED>
+template <typename T, bool EXACT, int PT, int NW, bool FUSED>
 __global__ __launch_bounds__(64 * NW) void fp8_few_kernel(GemmArgs8 g, const T *__restrict__ x, int K, unsigned char *__restrict__ codes_out,
                                                       unsigned char *__restrict__ scales_out) {
-  constexpr bool EXACT = Exact<T>::value;
   __shared__ float sums[NW][PT][64][4];
   extern __shared__ __attribute__((aligned(16))) unsigned char codes[];   // FUSED: P x Kp codes, P x Kb exponents
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, j = lane & 15, q = lane >> 4;
@@ -835,7 +830,7 @@ __global__ __launch_bounds__(256) void fp8_wgrad_join_kernel(const float *__rest
 
 // ---- host -----------------------------------------------------------------------------------------------------------
 
-template <typename T, int TM, int TN, int WM, int WN, int G, bool NT>
+template <typename T, bool EXACT, int TM, int TN, int WM, int WN, int G, bool NT>
 static int launch_tiles(GemmArgs8 g, hipStream_t st) {
   constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, STAGE = (BM + BN) * 128;
   g.tiles_n = (g.N + BN - 1) / BN;
@@ -843,33 +838,33 @@ static int launch_tiles(GemmArgs8 g, hipStream_t st) {
   if (g.tiles > 0x7fffffffll) return GB_ERANGE;
   if (2 * G * STAGE > 65536) {
     static std::atomic<unsigned long long> done{0};
-    allow_dynamic_lds(fp8_gemm_kernel<T, TM, TN, WM, WN, G, NT>, 2 * G * STAGE, done);
+    allow_dynamic_lds(fp8_gemm_kernel<T, EXACT, TM, TN, WM, WN, G, NT>, 2 * G * STAGE, done);
   }
-  fp8_gemm_kernel<T, TM, TN, WM, WN, G, NT><<<(unsigned)g.tiles, 64 * WM * WN * G, (g.Kb > 1 ? 2 * G : 1) * STAGE, st>>>(g);
+  fp8_gemm_kernel<T, EXACT, TM, TN, WM, WN, G, NT><<<(unsigned)g.tiles, 64 * WM * WN * G, (g.Kb > 1 ? 2 * G : 1) * STAGE, st>>>(g);
   return check_launch("gb_fp8_linear");
 }
 
 static long long tiles_of(long long P, int N, int b) { return ((P + b - 1) / b) * ((N + b - 1) / b); }
-template <typename T, int PT, bool FUSED>
+template <typename T, bool EXACT, int PT, bool FUSED>
 static void launch_few(const GemmArgs8 &g, const T *x, int K, unsigned char *codes, unsigned char *scales, size_t lds, hipStream_t st) {
   const unsigned grid = (unsigned)((g.N + 15) / 16);
   if (g.Kb >= 8)   // (a wave per block of a long reduction: 4 x 4096 -> 4096 fp32 9.7 us with four waves, 6.7 with eight)
-    fp8_few_kernel<T, PT, 8, FUSED><<<grid, 512, lds, st>>>(g, x, K, codes, scales);
+    fp8_few_kernel<T, EXACT, PT, 8, FUSED><<<grid, 512, lds, st>>>(g, x, K, codes, scales);
   else
-    fp8_few_kernel<T, PT, 4, FUSED><<<grid, 256, lds, st>>>(g, x, K, codes, scales);
+    fp8_few_kernel<T, EXACT, PT, 4, FUSED><<<grid, 256, lds, st>>>(g, x, K, codes, scales);
 }
 
 // y from codes and exponents in memory
-template <typename T>
+template <typename T, bool EXACT>
 static int multiply_codes(const GemmArgs8 &g, int K, hipStream_t st) {
   // (64 x 4096 -> 4096 bf16: 18.2 us without tiles, 13.7 with four groups of waves a tile; 64 x 1024 -> 1024: 7.6, 8.4)
   if (g.P <= FP8_FEW_ROWS && !(g.P > 32 && g.Kb >= 32)) {
     if (g.P <= 16)
-      launch_few<T, 1, false>(g, nullptr, K, nullptr, nullptr, 0, st);
+      launch_few<T, EXACT, 1, false>(g, nullptr, K, nullptr, nullptr, 0, st);
     else if (g.P <= 32)
-      launch_few<T, 2, false>(g, nullptr, K, nullptr, nullptr, 0, st);
+      launch_few<T, EXACT, 2, false>(g, nullptr, K, nullptr, nullptr, 0, st);
     else
-      launch_few<T, 4, false>(g, nullptr, K, nullptr, nullptr, 0, st);
+      launch_few<T, EXACT, 4, false>(g, nullptr, K, nullptr, nullptr, 0, st);
     return check_launch("gb_fp8_linear");
   }
   // 256 x 256 where that still gives every CU a tile, the columns fill it as well as 128 do to a fifth, and there are steps
@@ -878,12 +873,12 @@ static int multiply_codes(const GemmArgs8 &g, int K, hipStream_t st) {
   // 128 x 128, 46 in 1024 of these).
   const bool nt = streams(g.P * g.N * (long long)sizeof(T));
   if (g.Kb >= 4 && tiles_of(g.P, g.N, 256) >= 256 && 5 * blocks128(g.N) >= 8 * ((g.N + 255) / 256))
-    return nt ? launch_tiles<T, 4, 2, 2, 4, 1, true>(g, st) : launch_tiles<T, 4, 2, 2, 4, 1, false>(g, st);
-  if (tiles_of(g.P, g.N, 128) >= 256) return nt ? launch_tiles<T, 2, 2, 2, 2, 1, true>(g, st) : launch_tiles<T, 2, 2, 2, 2, 1, false>(g, st);
+    return nt ? launch_tiles<T, EXACT, 4, 2, 2, 4, 1, true>(g, st) : launch_tiles<T, EXACT, 4, 2, 2, 4, 1, false>(g, st);
+  if (tiles_of(g.P, g.N, 128) >= 256) return nt ? launch_tiles<T, EXACT, 2, 2, 2, 2, 1, true>(g, st) : launch_tiles<T, EXACT, 2, 2, 2, 2, 1, false>(g, st);
   const long long tiles = tiles_of(g.P, g.N, 64);
   if (g.Kb >= 8 && tiles <= 512)
-    return tiles <= 256 ? launch_tiles<T, 1, 2, 2, 1, 4, false>(g, st) : launch_tiles<T, 1, 2, 2, 1, 2, false>(g, st);
-  return launch_tiles<T, 1, 2, 2, 1, 1, false>(g, st);
+    return tiles <= 256 ? launch_tiles<T, EXACT, 1, 2, 2, 1, 4, false>(g, st) : launch_tiles<T, EXACT, 1, 2, 2, 1, 2, false>(g, st);
+  return launch_tiles<T, EXACT, 1, 2, 2, 1, 1, false>(g, st);
 }
 
 // Columns of the streaming kernel's variant; 0: not one of its shapes.  A weight of 128 x 128 is in LDS at once, and one
@@ -910,26 +905,37 @@ static StreamPlan8 stream_plan(long long P, int cols, int K, int dtype, bool sum
   p.grid = (int)(tiles < most ? tiles : most);
   return p;
 }
-template <typename T, int TM, int TN, int WM, int WN, bool SUM>
+template <typename T, bool EXACT, int TM, int TN, int WM, int WN, bool SUM>
 static int launch_stream(const StreamArgs8 &g, const StreamPlan8 &p, hipStream_t st) {
   const bool nt = streams(g.P * (g.N < g.K ? g.N : g.K) * (long long)sizeof(T));
   static std::atomic<unsigned long long> done[2];
   if (nt) {
-    allow_dynamic_lds(fp8_stream_kernel<T, TM, TN, WM, WN, SUM, true>, 163840, done[1]);
-    fp8_stream_kernel<T, TM, TN, WM, WN, SUM, true><<<(unsigned)p.grid, 256, p.lds, st>>>(g);
+    allow_dynamic_lds(fp8_stream_kernel<T, EXACT, TM, TN, WM, WN, SUM, true>, 163840, done[1]);
+    fp8_stream_kernel<T, EXACT, TM, TN, WM, WN, SUM, true><<<(unsigned)p.grid, 256, p.lds, st>>>(g);
   } else {
-    allow_dynamic_lds(fp8_stream_kernel<T, TM, TN, WM, WN, SUM, false>, 163840, done[0]);
-    fp8_stream_kernel<T, TM, TN, WM, WN, SUM, false><<<(unsigned)p.grid, 256, p.lds, st>>>(g);
+    allow_dynamic_lds(fp8_stream_kernel<T, EXACT, TM, TN, WM, WN, SUM, false>, 163840, done[0]);
+    fp8_stream_kernel<T, EXACT, TM, TN, WM, WN, SUM, false><<<(unsigned)p.grid, 256, p.lds, st>>>(g);
   }
   return check_launch("gb_fp8_linear");
 }
-template <typename T, bool SUM>
+template <typename T, bool EXACT, bool SUM>
 static int stream_rows(const StreamArgs8 &g, const StreamPlan8 &p, int cols, hipStream_t st) {
-  return cols == 128   ? launch_stream<T, 1, 2, 2, 2, SUM>(g, p, st)
-         : cols == 256 ? launch_stream<T, 2, 2, 1, 4, SUM>(g, p, st)
-                       : launch_stream<T, 2, 4, 1, 4, SUM>(g, p, st);
+  return cols == 128   ? launch_stream<T, EXACT, 1, 2, 2, 2, SUM>(g, p, st)
+         : cols == 256 ? launch_stream<T, EXACT, 2, 2, 1, 4, SUM>(g, p, st)
+                       : launch_stream<T, EXACT, 2, 4, 1, 4, SUM>(g, p, st);
 }
 
+
+// f(T(), EXACT) of a product's output type and GB_FP8_SHORT_SUMS
+template <typename F>
+static int with_form(int dtype, int flags, F f) {
+  return with_type(dtype, [&](auto z) {
+    typedef decltype(z) T;
+    if constexpr (sizeof(T) == 2)
+      if (flags & GB_FP8_SHORT_SUMS) return f(z, std::false_type());
+    return f(z, std::true_type());
+  });
+}
 
 static bool fp8_dims_bad(long long P, int N, int K) { return P < 0 || N <= 0 || K <= 0; }
 static bool fp8_dims_large(long long P, int N, int K) {   // int tile offsets: 256 rows of Kp bytes; 65535 blocks a grid axis
@@ -1033,10 +1039,10 @@ static long long linear_workspace(long long P, int N, int K, bool keeps, bool su
   return b;
 }
 
-extern "C" int gb_fp8_linear(const void *x, int dtype, long long P, int K, const void *w, const void *w_scales, int transposed, int N,
+extern "C" int gb_fp8_linear(const void *x, int dtype, long long P, int K, const void *w, const void *w_scales, int flags, int N,
                              const float *bias, void *y, void *codes, void *scales, float *colsum, void *ws, long long ws_bytes,
                              void *stream) {
-  if (fp8_dims_bad(P, N, K) || !known_type(dtype) || !codes != !scales) return GB_EINVAL;
+  if (fp8_dims_bad(P, N, K) || !known_type(dtype) || !codes != !scales || (flags & ~(GB_FP8_TRANSPOSED | GB_FP8_SHORT_SUMS))) return GB_EINVAL;
   if (fp8_dims_large(P, N, K)) return GB_ERANGE;
   if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(ws) |
        reinterpret_cast<uintptr_t>(w)) % 16)
@@ -1050,7 +1056,8 @@ extern "C" int gb_fp8_linear(const void *x, int dtype, long long P, int K, const
     fp8_colsum_kernel<<<(K + 7) / 8, 256, 0, st>>>((const float *)ws, 0, K, colsum);
     return check_launch("gb_fp8_linear");
   }
-  const int route = linear_route(P, N, K), Kb = blocks128(K), bs_n = transposed ? 1 : Kb, bs_k = transposed ? blocks128(N) : 1;
+  const int route = linear_route(P, N, K), Kb = blocks128(K), bs_n = flags & GB_FP8_TRANSPOSED ? 1 : Kb,
+            bs_k = flags & GB_FP8_TRANSPOSED ? blocks128(N) : 1;
   if (route == FP8_STREAM) {
     const int cols = stream_columns(P, N, K);
     const StreamPlan8 p = stream_plan(P, cols, K, dtype, colsum != nullptr);
@@ -1069,9 +1076,10 @@ extern "C" int gb_fp8_linear(const void *x, int dtype, long long P, int K, const
     g.K = K;
     g.bs_n = bs_n;
     g.bs_k = bs_k;
-    const int rc = with_type(dtype, [&](auto z) {
+    const int rc = with_form(dtype, flags, [&](auto z, auto exact) {
       typedef decltype(z) T;
-      return colsum ? stream_rows<T, true>(g, p, cols, st) : stream_rows<T, false>(g, p, cols, st);
+      constexpr bool EXACT = decltype(exact)::value;
+      return colsum ? stream_rows<T, EXACT, true>(g, p, cols, st) : stream_rows<T, EXACT, false>(g, p, cols, st);
     });
     if (rc || !colsum) return rc;
     fp8_colsum_kernel<<<(K + 7) / 8, 256, 0, st>>>((const float *)ws, p.grid, K, colsum);
@@ -1090,9 +1098,9 @@ extern "C" int gb_fp8_linear(const void *x, int dtype, long long P, int K, const
   g.bs_k = bs_k;
   if (route == FP8_FEW && !colsum) {
     const size_t lds = (size_t)up16(P * Kb * 129);
-    return with_type(dtype, [&](auto z) {
+    return with_form(dtype, flags, [&](auto z, auto exact) {
       typedef decltype(z) T;
-      launch_few<T, 1, true>(g, (const T *)x, K, (unsigned char *)codes, (unsigned char *)scales, lds, st);
+      launch_few<T, decltype(exact)::value, 1, true>(g, (const T *)x, K, (unsigned char *)codes, (unsigned char *)scales, lds, st);
       return check_launch("gb_fp8_linear");
     });
   }
@@ -1106,9 +1114,9 @@ extern "C" int gb_fp8_linear(const void *x, int dtype, long long P, int K, const
   if (rc) return rc;
   g.a = (const unsigned char *)codes;
   g.a_scales = (const unsigned char *)scales;
-  return with_type(dtype, [&](auto z) {
+  return with_form(dtype, flags, [&](auto z, auto exact) {
     typedef decltype(z) T;
-    return multiply_codes<T>(g, K, st);
+    return multiply_codes<T, decltype(exact)::value>(g, K, st);
   });
 }
 

@@ -287,6 +287,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
 # ---- products in 8-bit floats -----------------------------------------------------------------------------------------
 
 _WS_COLSUM, _WS_WGRAD, _WS_LINEAR, _KEEP, _SUM = 0, 1, 4, 1, 2     # GB_FP8_*
+_TRANSPOSED, _SHORT_SUMS = 1, 2
 
 
 def _up(n, m):
@@ -314,10 +315,10 @@ def _quantise_rows_to(x2, at, sums, ws, size):
           size, _s(x2))
 
 
-def _product_to(x2, y, w, w_scales, transposed, N, bias, keep_at, sums, ws, size):
+def _product_to(x2, y, w, w_scales, flags, N, bias, keep_at, sums, ws, size):
     """gb_fp8_linear: y (P, N) of rows x2 and a weight's codes; keep_at: where x2's codes and exponents go, or None."""
     P, K = x2.shape
-    _call("gb_fp8_linear", x2.device, x2.data_ptr(), _TYPES[x2.dtype], P, K, w, w_scales, transposed, N, _lib.ptr(bias),
+    _call("gb_fp8_linear", x2.device, x2.data_ptr(), _TYPES[x2.dtype], P, K, w, w_scales, flags, N, _lib.ptr(bias),
           y.data_ptr(), keep_at, None if keep_at is None else keep_at + _row_bytes(P, K)[0], _lib.ptr(sums), ws, size, _s(x2))
 
 
@@ -394,7 +395,7 @@ def _fp8_weight_tensor(what, w):
     return w.view(w.shape[0], w.shape[1]) if w.dim() > 2 else w
 
 
-def _fp8_forward(x, weight, bias, need_x, keep):
+def _fp8_forward(x, weight, bias, flags, need_x, keep):
     """(y, the weight's _Codes, x's codes and exponents | None)"""
     dev = x.device
     P, K = x.shape
@@ -405,19 +406,19 @@ def _fp8_forward(x, weight, bias, need_x, keep):
     kept = torch.empty(sum(_row_bytes(P, K)), dtype=torch.uint8, device=dev) if keep else None
     size = _fp8_workspace_bytes(_WS_LINEAR + _KEEP * keep, P, w.N, K)
     ws = _bytes(size, dev)
-    _product_to(x, y, w.codes, w.scales, 0, w.N, bias, _lib.ptr(kept), None, _lib.ptr(ws), size)
+    _product_to(x, y, w.codes, w.scales, flags, w.N, bias, _lib.ptr(kept), None, _lib.ptr(ws), size)
     return y, w, kept
 
 
 class _Fp8Linear(Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, held):
+    def forward(ctx, x, weight, bias, held, flags):
         need_x, need_w = ctx.needs_input_grad[:2]
-        y, w, kept = _fp8_forward(x, weight if held is None else held, bias, need_x, need_w)
+        y, w, kept = _fp8_forward(x, weight if held is None else held, bias, flags, need_x, need_w)
         # one byte per element of x stays for the backward pass
         ctx.save_for_backward(kept)
         ctx.w = w if need_x else None
-        ctx.dims = (w.N, w.K, None if held is not None else weight.dtype)
+        ctx.dims, ctx.flags = (w.N, w.K, None if held is not None else weight.dtype), flags
         return y
 
     @staticmethod
@@ -440,7 +441,7 @@ class _Fp8Linear(Function):
         db = torch.empty(N, dtype=torch.float32, device=dev) if need_b else None
         if need_x:
             dx = torch.empty((P, K), dtype=dy.dtype, device=dev)
-            _product_to(dy, dx, ctx.w.codes_t, ctx.w.scales, 1, K, None, at if codes else None, db, at + room, first)
+            _product_to(dy, dx, ctx.w.codes_t, ctx.w.scales, ctx.flags | _TRANSPOSED, K, None, at if codes else None, db, at + room, first)
         else:
             _quantise_rows_to(dy, at, db, at + room, first)
         if need_w:
@@ -449,18 +450,20 @@ class _Fp8Linear(Function):
             _call("gb_fp8_wgrad", dev, at, at + _row_bytes(P, N)[0], x_at, x_at + _row_bytes(P, K)[0], dw.data_ptr(), P, N, K,
                   at + room, second, _s(dy))
             dw = dw if wtype == torch.float32 else dw.to(wtype)
-        return dx, dw, db, None
+        return dx, dw, db, None, None
 
 
-def fp8_linear(x, weight, bias=None):
+def fp8_linear(x, weight, bias=None, short_sums=False):
     """x weight^T + bias with both operands in 8-bit floats (e4m3) under power-of-two scales: x (..., in_features) has one
     per 128 elements of a row, weight one per 128 x 128.  weight: (out_features, in_features) - a parameter, or that of a
     1x1 convolution - quantised in the call, or an Fp8Weight that is kept.  -> (..., out_features) like x; sums in fp32.
 
     Gradients are those of the products with the quantisers passed straight through: the incoming gradient is quantised
     like x, dx and dweight are products of the 8-bit operands, dbias sums the gradient as it came.  An element of x or
-    weight that is not finite makes every output it takes part in NaN.  16-bit x runs on the 8-bit matrix instructions
-    (about 14 bits of the largest product kept within a step of 64 or 128), fp32 x on the bf16 ones (exact operands)."""
+    weight that is not finite makes every output it takes part in NaN.  The codes are multiplied as bf16, which holds them
+    exactly, with fp32 sums.  short_sums: for 16-bit x, y and dx come from the 8-bit matrix instructions instead: faster where
+    the matrix cores bind, but a step of 64 or 128 products keeps only about 14 bits below its largest (measured 5e-5 of the
+    result's norm); fp32 x is computed as ever."""
     what = "fp8_linear"
     _rows_tensor(what, "x", x)
     held = weight if isinstance(weight, Fp8Weight) else None
@@ -477,10 +480,11 @@ def fp8_linear(x, weight, bias=None):
     bias = _channel_vector(what, "bias", bias, N, x)
     rows = (x if x.dim() == 2 else x.reshape(-1, K)).contiguous()
     weight = None if held is not None else weight.contiguous()
+    flags = _SHORT_SUMS if short_sums else 0
     if _grads(x, weight, bias):
-        y = _Fp8Linear.apply(rows, weight, bias, held)
+        y = _Fp8Linear.apply(rows, weight, bias, held, flags)
     else:
-        y = _fp8_forward(rows, weight if held is None else held, bias, False, False)[0]
+        y = _fp8_forward(rows, weight if held is None else held, bias, flags, False, False)[0]
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (N,))
 
 

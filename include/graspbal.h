@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define GB_ABI_VERSION 8
+#define GB_ABI_VERSION 9
 
 enum {
   GB_OK = 0,
@@ -759,12 +759,12 @@ int gb_group_norm_bwd(const GbGroupNorm *n, const void *dy, void *dx, void *dres
  * gb_fp8_quant_rows: x (P, K) -> codes, scales; colsum: NULL, or (K) fp32 = the columns' sums of x (ws: gb_fp8_workspace
  *   COLSUM with N = K).
  * gb_fp8_quant_weight: w (N, K) -> codes (N, Kp), block scales, and codes_t (K, Np) = the transposed codes unless NULL.
- * gb_fp8_linear: y (P, N) = deq(Q(x)) deq(w)^T + bias, x (P, K) in floats, w (N, K) by blocks; transposed != 0: w is the
- *   codes_t of a weight (K, N) whose scales are given as they are.  fp32: codes multiplied as bf16 with fp32 sums (values
- *   below 2^-126 count as zero, those that round to 2^128 as infinite); 16 bits: 8-bit matrix instructions, whose steps add
- *   64 or 128 products with about 14 bits below the largest before the fp32 sum.  codes, scales: NULL, or x's by rows are
- *   kept there; colsum: as above; bias: (N) fp32 or NULL.  ws: gb_fp8_workspace LINEAR (+ KEEP with codes, + SUM with
- *   colsum), 16-byte aligned.
+ * gb_fp8_linear: y (P, N) = deq(Q(x)) deq(w)^T + bias, x (P, K) in floats, w (N, K) by blocks; the codes are multiplied as
+ *   bf16 with fp32 sums (values below 2^-126 count as zero, those that round to 2^128 as infinite).  flags:
+ *   GB_FP8_TRANSPOSED: w is the codes_t of a weight (K, N) whose scales are given as they are; GB_FP8_SHORT_SUMS (ignored
+ *   for fp32 x): the 8-bit matrix instructions, whose steps add 64 or 128 products with about 14 bits below the largest
+ *   before the fp32 sum; other bits: GB_EINVAL.  codes, scales: NULL, or x's by rows are kept there; colsum: as above;
+ *   bias: (N) fp32 or NULL.  ws: gb_fp8_workspace LINEAR (+ KEEP with codes, + SUM with colsum), 16-byte aligned.
  * gb_fp8_wgrad: dw (N, K) fp32 = deq(dy)^T deq(x), dy (P, N) and x (P, K) by rows (ws: gb_fp8_workspace WGRAD); bf16 products
  *   with fp32 sums in a fixed order.                                                                                    */
 #define GB_FP8_WS_COLSUM 0
@@ -772,11 +772,13 @@ int gb_group_norm_bwd(const GbGroupNorm *n, const void *dy, void *dx, void *dres
 #define GB_FP8_WS_LINEAR 4
 #define GB_FP8_KEEP 1
 #define GB_FP8_SUM 2
+#define GB_FP8_TRANSPOSED 1
+#define GB_FP8_SHORT_SUMS 2
 int gb_fp8_workspace(int what, long long P, int N, int K, long long *bytes);
 int gb_fp8_quant_rows(const void *x, int dtype, long long P, int K, void *codes, void *scales, float *colsum, void *ws,
                       long long ws_bytes, void *stream);
 int gb_fp8_quant_weight(const void *w, int dtype, int N, int K, void *codes, void *codes_t, void *scales, void *stream);
-int gb_fp8_linear(const void *x, int dtype, long long P, int K, const void *w, const void *w_scales, int transposed, int N,
+int gb_fp8_linear(const void *x, int dtype, long long P, int K, const void *w, const void *w_scales, int flags, int N,
                   const float *bias, void *y, void *codes, void *scales, float *colsum, void *ws, long long ws_bytes,
                   void *stream);
 int gb_fp8_wgrad(const void *dy, const void *dy_scales, const void *x, const void *x_scales, float *dw, long long P, int N, int K,

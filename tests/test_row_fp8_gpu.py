@@ -332,3 +332,55 @@ def test_refusals():
                  lambda: fused_rows.Fp8Weight(held.codes.float(), held.scales, 64)):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("P,K,N", [(1, 1024, 1024), (40, 1300, 70), (200, 1153, 321), (1100, 1100, 1100), (16500, 256, 200),
+                                   (20000, 128, 128), (2500, 136, 4104)])
+def test_sums_of_16_bit_products_are_fp32(P, K, N, dtype):
+    """The bound of fp32 results (see _check: K / 8 roundings of 2^-24 and 64 where ranges are joined) and the one rounding to
+    the type, on every route: values and the input's gradient.  Outputs whose terms cancel show sums of fewer bits."""
+    from graspbalance_amd import fused_rows
+    x, w, b, dy = _data(P, K, N, dtype)
+    xg = x.to("cuda:0").requires_grad_()
+    y = fused_rows.fp8_linear(xg, fused_rows.Fp8Weight.quantize(w.to("cuda:0"), input_gradients=True), b.to("cuda:0"))
+    dx, = torch.autograd.grad(y, xg, dy.to("cuda:0"))
+    xq, wq, dq = row_truth.in_8_bits(x.double(), 1), row_truth.in_8_bits(w.double(), 128), row_truth.in_8_bits(dy.double(), 1)
+    for got, left, right, bias in ((y, xq, wq, b.double()), (dx, dq, wq.t().contiguous(), None)):
+        truth, terms = left @ right.t(), left.abs() @ right.abs().t()
+        if bias is not None:
+            truth, terms = truth + bias, terms + bias.abs()
+        bound = 2.0 ** -24 * (left.shape[1] / 8 + 64) * terms + HALF[dtype] * truth.abs() + TINY[dtype]
+        off = (got.detach().double().cpu() - truth).abs()
+        assert bool((off <= bound).all()), (off / bound).max().item()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("P,K,N", SHAPES + [(20000, 128, 192), (33001, 131, 100), (35000, 127, 470), (1100, 1100, 1100)])
+def test_short_sums_on_request(P, K, N, dtype):
+    """The 8-bit matrix instructions where they are asked for, within _check's bound for them; fp32 rows take no notice."""
+    from graspbalance_amd import fused_rows
+    x, w, b, dy = _data(P, K, N, dtype)
+    leaves = [t.to("cuda:0").requires_grad_() for t in (x, w, b)]
+    y = fused_rows.fp8_linear(*leaves, short_sums=True)
+    grads = torch.autograd.grad(y, leaves, dy.to("cuda:0"))
+    xq, wq, dq = row_truth.in_8_bits(x.double(), 1), row_truth.in_8_bits(w.double(), 128), row_truth.in_8_bits(dy.double(), 1)
+    _check(y, xq, wq, b.double(), dtype, "y")
+    _check(grads[0], dq, wq.t().contiguous(), None, dtype, "dx")
+    _check(grads[1], dq.t().contiguous(), xq.t().contiguous(), None, torch.float32, "dw", length=P)
+    if dtype == torch.float32:
+        plain = fused_rows.fp8_linear(*leaves)
+        assert torch.equal(y, plain)
+        assert all(torch.equal(a, c) for a, c in zip(grads, torch.autograd.grad(plain, leaves, dy.to("cuda:0"))))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("P,K,N", [(420000, 128, 128), (13000, 640, 4100)])
+def test_short_sums_past_the_caches(P, K, N, dtype):
+    """The streamed loads and stores of that form: 300 rows against the truth."""
+    from graspbalance_amd import fused_rows
+    x, w, b, _ = (t.to("cuda:0") for t in _data(P, K, N, dtype))
+    y = fused_rows.fp8_linear(x, w, b, short_sums=True)
+    pick = torch.randperm(P, generator=torch.Generator().manual_seed(0))[:300].to("cuda:0")
+    xq, wq = row_truth.in_8_bits(x[pick].cpu().double(), 1), row_truth.in_8_bits(w.cpu().double(), 128)
+    _check(y[pick], xq, wq, b.cpu().double(), dtype, "y")

@@ -155,3 +155,12 @@ def test_the_oracle_of_8_bits_agrees_with_torchs_cast():
             scale[i, j] = 2.0 ** e
     want = (blocks / scale.float()).to(torch.float8_e4m3fn).double() * scale
     assert torch.equal(got, want.view(64, 256))
+
+
+def test_fp8_refuses_unknown_flags():
+    from graspbalance_amd import _lib
+    for dtype in (0, 1, 2):
+        for flags in (4, 8, -1, 1 << 20):
+            assert _lib.lib().gb_fp8_linear(64, dtype, 8, 8, 64, 64, flags, 8, None, 64, None, None, None, 64, 1 << 20, None) == -1
+        for flags in (0, 1, 2, 3):      # (no rows: nothing is launched)
+            assert _lib.lib().gb_fp8_linear(None, dtype, 0, 8, None, None, flags, 8, None, None, None, None, None, None, 0, None) == 0
