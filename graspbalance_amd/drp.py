@@ -166,7 +166,8 @@ class InvResMLP(nn.Module):
         return fused_rows.conv_gn_act(x, pw1[0], pw1[1], fused_rows.activation_of(self.act), self.fp8, residual=f_cl)
 
     def _fused_on(self, f):
-        return fused_mlp.enabled(f) and (self.fusable() or (fused_rows.supports(f) and self.fusable_gn()))
+        # (the grouping and the fp32 products read fp32 rows; the row operators alone would take 16 bits)
+        return fused_mlp.enabled(f) and f.dtype == torch.float32 and (self.fusable() or self.fusable_gn())
 
     def forward(self, pf):
         p, f = pf
@@ -174,7 +175,7 @@ class InvResMLP(nn.Module):
             out = self.forward_cl(p, f.transpose(1, 2).contiguous())
             return [p, out.transpose(1, 2)]
         if self.fp8:
-            raise RuntimeError("InvResMLP: fp8 runs on the GPU only")
+            raise RuntimeError("InvResMLP: fp8 takes float32 features on the GPU only")
         identity = f
         f = self.convs([p, f])
         if self.dropout is not None:

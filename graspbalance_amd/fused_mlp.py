@@ -178,6 +178,20 @@ def _s(t):
     return _lib.current_stream(t.device)
 
 
+def _fp32(what, *tensors):
+    """The kernels of this module read fp32 by address: a tensor of another type is refused before anything is launched (a
+    16-bit one has half the bytes that a kernel would read).  None passes."""
+    for t in tensors:
+        if t is not None and t.dtype != torch.float32:
+            raise RuntimeError("%s: tensors must be float32, not %s" % (what, t.dtype))
+
+
+def _columns(what, X, W):
+    """Rows X (P, K) and a weight (N, K) that go together."""
+    if X.dim() != 2 or X.shape[1] != W.shape[1]:
+        raise RuntimeError("%s: rows %s do not go with a weight of %d input channels" % (what, tuple(X.shape), W.shape[1]))
+
+
 _FN = {}
 
 # ---- per-step zero arena for the small fp64 reduction buffers --------------------------------------------------
@@ -559,11 +573,13 @@ class InterpConcatCL(Function):
 
 
 def interp_concat_cl(known_cl, idx, weight, skip_cl=None):
+    _fp32("interp_concat_cl", known_cl, weight, skip_cl)
     return InterpConcatCL.apply(known_cl.contiguous(), idx.contiguous(), weight.contiguous(),
                                 None if skip_cl is None else skip_cl.contiguous())
 
 
 def group_concat_cl(xyz, new_xyz, idx, feat_cl=None, mode=0, scale=1.0, rot=None):
+    _fp32("group_concat_cl", xyz, new_xyz, feat_cl, rot)
     return GroupConcatCL.apply(xyz.contiguous(), new_xyz.contiguous(), idx.contiguous(),
                                None if feat_cl is None else feat_cl.contiguous(), mode, scale, rot)
 
@@ -1130,6 +1146,7 @@ class LocalGeometry:
     sum dp dp^T].  A stage of InvResMLP blocks over the same points and radius shares one."""
 
     def __init__(self, xyz, centres, idx, mode=0, scale=1.0):
+        _fp32("LocalGeometry", xyz, centres)
         self.xyz, self.centres, self.idx = xyz.contiguous(), centres.contiguous(), idx.contiguous()
         self.b, self.n = self.xyz.shape[0], self.xyz.shape[1]
         self.m, self.ns = self.idx.shape[1], self.idx.shape[2]
@@ -1254,6 +1271,7 @@ def local_agg_pool(f_cl, conv, bn, geo):
     """conv (1x1, 3+C -> N, no bias) + bn + ReLU + max over the neighbours of `geo`, from point features (b*n, C)."""
     if conv.bias is not None:
         raise NotImplementedError("fused path expects bias-free convs followed by BatchNorm")
+    _fp32("local_agg_pool", f_cl, geo.xyz, geo.centres, conv.weight, bn.weight, bn.bias, bn.running_mean)
     _count_batch(bn)
     W = conv.weight.view(conv.weight.shape[0], -1)
     return LocalAggPool.apply(f_cl, W, bn.weight, bn.bias, geo, _LayerCfg(bn))
@@ -1347,6 +1365,7 @@ def _stack(X, convs_bns, pool_ns=0, residual=None, relu_last=True, rows=None):
     moves by momentum * bias (applied afterwards); in eval mode it is folded into the running mean handed to the
     finalisation."""
     params, layers, biased, shifts = [], [], [], []
+    _fp32("conv_bn_act", X, residual, *[t for conv, bn in convs_bns for t in (conv.weight, bn.weight, bn.bias, bn.running_mean)])
     for conv, bn in convs_bns:
         _count_batch(bn)
         params += [conv.weight.view(conv.weight.shape[0], -1), bn.weight, bn.bias]
@@ -1418,6 +1437,8 @@ class LinearBias(Function):
 def linear_bias(X, conv):
     """A 1x1 Conv1d / Conv2d (with or without bias) applied to rows X (P, Cin) -> (P, Cout)."""
     W = conv.weight.view(conv.weight.shape[0], -1)
+    _fp32("linear_bias", X, W, conv.bias)
+    _columns("linear_bias", X, W)
     return LinearBias.apply(X, W, conv.bias)
 
 
@@ -1429,6 +1450,7 @@ def conv_bn_act(X, conv, bn, relu=True, pool_ns=0, residual=None):
     W = conv.weight.view(conv.weight.shape[0], -1)
     if conv.bias is not None:
         raise NotImplementedError("the torch.mm comparison path expects bias-free convs followed by BatchNorm")
+    _fp32("conv_bn_act", X, residual, W, bn.weight, bn.bias, bn.running_mean)
     _count_batch(bn)
     momentum = 0.0 if bn.momentum is None else bn.momentum
     training = bn.training or not bn.track_running_stats

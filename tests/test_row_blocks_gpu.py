@@ -231,3 +231,28 @@ def test_refusals_of_the_blocks():
             blk([torch.randn(1, 64, 3, device=DEV), torch.randn(1, 32, 64, device=DEV)])
     finally:
         fused_mlp.set_enabled(True)
+
+
+@pytest.mark.parametrize("norm", ["bn", "gn", "gn fp8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_blocks_refuse_16_bit_features(norm, dtype):
+    """The host refuses them, fused and plain, whatever the parameters' type; the device has nothing to report afterwards."""
+    from graspbalance_amd import fused_mlp
+    from graspbalance_amd.drp import run_stage
+    blk = _block(norm={'norm': 'bn'} if norm == "bn" else None, act='relu', fp8=norm == "gn fp8").to(DEV)
+    p, f = torch.rand(1, 64, 3, device=DEV), torch.randn(1, 32, 64, device=DEV)
+    for module in (blk, copy.deepcopy(blk).to(dtype)):
+        for flag in (True, False):
+            fused_mlp.set_enabled(flag)
+            try:
+                with pytest.raises(RuntimeError, match="float32"):
+                    module([p, f.to(dtype)])
+                with pytest.raises(RuntimeError, match="float32"):
+                    run_stage(nn.Sequential(module), p, f.to(dtype))
+            finally:
+                fused_mlp.set_enabled(True)
+    if norm != "gn fp8":       # (8-bit products take weights of any type)
+        with pytest.raises(RuntimeError, match="float32"):
+            copy.deepcopy(blk).to(dtype)([p, f])
+    torch.cuda.synchronize()
+    assert bool(torch.isfinite(blk([p, f])[1]).all())
