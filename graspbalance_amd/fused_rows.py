@@ -4,14 +4,14 @@ activation, dropout from a counter-based generator, products in 8-bit floats wit
 Rows are (..., C) tensors in fp32, bf16 or fp16 with the channels last, as everywhere on the fused path.  Kernels run on the
 current stream of the tensors' device; workspaces come from torch's allocator inside the call, so that every captured graph
 has its own.  CPU tensors raise, like every operator of this package.  Gradients are exact to rounding and repeat bit for
-bit (no atomics); differentiating them again is refused.
+bit (no atomics); differentiating them again is refused, and so are operands of forward-mode differentiation.
 """
 import ctypes
 import functools
 
 import torch
 import torch.nn as nn
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -80,7 +80,10 @@ def _rng_args(rng):
 
 
 def _grads(*tensors):
-    """Whether a call has to be recorded for a backward pass."""
+    """Whether a call goes through autograd: to be recorded for a backward pass, or because an operand carries a tangent of
+    forward-mode differentiation, which the autograd functions refuse (a tangent must not vanish)."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
