@@ -356,6 +356,18 @@ class _Codes:
         _call("gb_fp8_quant_weight", w.device, w.data_ptr(), _TYPES[w.dtype], c.N, c.K, c.codes, c.codes_t, c.scales, _s(w))
         return c
 
+    def for_backward(self):
+        """What the backward pass reads of it, as tensors for autograd to keep (and to watch)."""
+        return (self.held,) if isinstance(self.held, torch.Tensor) else (self.held[2], self.held[1])
+
+    @staticmethod
+    def of_backward(kept, N, K):
+        """(address of the transposed codes, of the exponents) in what for_backward gave."""
+        if len(kept) == 2:
+            return kept[0].data_ptr(), kept[1].data_ptr()
+        n, m = N * _up(K, 128), K * _up(N, 128)
+        return kept[0].data_ptr() + n, kept[0].data_ptr() + n + m
+
 
 class Fp8Weight:
     """A weight (out_features, in_features) held in 8 bits for fp8_linear: ``codes`` (out_features, in_features up to whole
@@ -419,15 +431,14 @@ class _Fp8Linear(Function):
         need_x, need_w = ctx.needs_input_grad[:2]
         y, w, kept = _fp8_forward(x, weight if held is None else held, bias, flags, need_x, need_w)
         # one byte per element of x stays for the backward pass
-        ctx.save_for_backward(kept)
-        ctx.w = w if need_x else None
+        ctx.save_for_backward(kept, *(w.for_backward() if need_x else ()))
         ctx.dims, ctx.flags = (w.N, w.K, None if held is not None else weight.dtype), flags
         return y
 
     @staticmethod
     @_once
     def backward(ctx, dy):
-        kept, = ctx.saved_tensors
+        kept, *codes_w = ctx.saved_tensors
         N, K, wtype = ctx.dims
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dy = dy.contiguous()
@@ -444,7 +455,8 @@ class _Fp8Linear(Function):
         db = torch.empty(N, dtype=torch.float32, device=dev) if need_b else None
         if need_x:
             dx = torch.empty((P, K), dtype=dy.dtype, device=dev)
-            _product_to(dy, dx, ctx.w.codes_t, ctx.w.scales, ctx.flags | _TRANSPOSED, K, None, at if codes else None, db, at + room, first)
+            _product_to(dy, dx, *_Codes.of_backward(codes_w, N, K), ctx.flags | _TRANSPOSED, K, None, at if codes else None, db,
+                        at + room, first)
         else:
             _quantise_rows_to(dy, at, db, at + room, first)
         if need_w:

@@ -384,3 +384,30 @@ def test_short_sums_past_the_caches(P, K, N, dtype):
     pick = torch.randperm(P, generator=torch.Generator().manual_seed(0))[:300].to("cuda:0")
     xq, wq = row_truth.in_8_bits(x[pick].cpu().double(), 1), row_truth.in_8_bits(w.cpu().double(), 128)
     _check(y[pick], xq, wq, b.cpu().double(), dtype, "y")
+
+
+def test_kept_codes_are_autograds_to_watch():
+    """Codes or exponents of a kept weight rewritten between the passes raise; saved-tensor hooks see what is kept."""
+    from graspbalance_amd import fused_rows
+    x, w, b, dy = (t.to("cuda:0") for t in _data(40, 130, 70, torch.float32))
+    x.requires_grad_()
+    for change in (lambda h: h.codes_t.view(torch.uint8).zero_(), lambda h: h.scales.add_(1)):
+        held = fused_rows.Fp8Weight.quantize(w, input_gradients=True)
+        parts = [t.clone() for t in (held.codes, held.scales, held.codes_t)]
+        for h in (held, fused_rows.Fp8Weight(parts[0], parts[1], 130, parts[2])):
+            y = fused_rows.fp8_linear(x, h, b)
+            change(h)
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(y, x, dy)
+    held = fused_rows.Fp8Weight.quantize(w, input_gradients=True)
+    for weight in (held, w):
+        want, = torch.autograd.grad(fused_rows.fp8_linear(x, weight, b), x, dy)
+        seen = []
+
+        def unpack(t):
+            seen.append(t)
+            return t.to("cuda:0")
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), unpack):
+            y = fused_rows.fp8_linear(x, weight, b)
+        got, = torch.autograd.grad(y, x, dy)
+        assert torch.equal(got, want) and sum(t.numel() for t in seen) >= held.codes_t.numel() + held.scales.numel()
