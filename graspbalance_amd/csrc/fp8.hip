@@ -89,7 +89,7 @@ __device__ __forceinline__ uint2 encode8(const F8 &f, int biased) {
   return r;
 }
 // Rows [r0, r0 + per) x block kb of 128 columns: sixteen lanes x eight elements a row.  SUM: also the column sums of these
-// rows, fp32 over per / 16 rows a lane, to part[chunk][K].
+// rows, fp32 over per / 16 rows a lane (64 at most) joined in 64 bits, to part[chunk][K].
 template <typename T, bool SUM>
 __global__ __launch_bounds__(256) void fp8_rows_kernel(const T *__restrict__ x, long long P, int K, unsigned char *__restrict__ codes,
                                                        unsigned char *__restrict__ scales, int per, float *__restrict__ part) {
@@ -113,9 +113,9 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const T *__restrict__ x, 
     __syncthreads();
     const int c = (int)threadIdx.x;
     if (c < 128 && kb * 128 + c < K) {
-      float s = 0;
+      double s = 0;
       for (int i = 0; i < 16; ++i) s += lds[i][c];
-      part[(long long)blockIdx.x * K + kb * 128 + c] = s;
+      part[(long long)blockIdx.x * K + kb * 128 + c] = (float)s;
     }
   }
 }
@@ -448,7 +448,9 @@ __global__ __launch_bounds__(64 * WM * WN * G) void fp8_gemm_kernel(GemmArgs8 g)
 // keeps the weight and walks over tiles of 64 rows, 128 columns of X at a step: the next step's rows travel in registers
 // while this one is multiplied, are quantised into the other LDS buffer, and go to memory as codes only where the backward
 // pass wants them.  Against a quantising kernel and the tiles above: X's codes are not read back and there is one launch
-// (524288 x 128 -> 256 bf16: 123 us in two launches, 100 here: 470 MB at 4.7 TB/s, a large copy's rate).  SUM: also the column sums of X, one LDS cell per lane.
+// (524288 x 128 -> 256 bf16: 123 us in two launches, 100 here: 470 MB at 4.7 TB/s, a large copy's rate).  SUM: also the
+// column sums of X, a tile's four rows of a lane in registers, then fp32 in the lane's LDS cells over STREAM_RUN tiles at most.
+static constexpr int STREAM_RUN = 60;
 struct StreamArgs8 {
   const void *x;
   const unsigned char *w, *w_scales;
@@ -585,9 +587,9 @@ __global__ __launch_bounds__(256, 2) void fp8_stream_kernel(StreamArgs8 g) {
   }
   if (SUM)
     for (int c = (int)threadIdx.x; c < g.K; c += 256) {
-      float s = 0;
+      double s = 0;
       for (int i = 0; i < 16; ++i) s += sums[i * Kp + c];
-      g.part[(long long)blockIdx.x * g.K + c] = s;
+      g.part[(long long)blockIdx.x * g.K + c] = (float)s;
     }
 }
 
@@ -901,7 +903,8 @@ static StreamPlan8 stream_plan(long long P, int cols, int K, int dtype, bool sum
   p.lds = (size_t)cols * Kp + 2 * 64 * 128 + 2 * 64 + 4 * (dtype == GB_T_F32 ? Cell<float>::BYTES : Cell<__bf16>::BYTES) + (sum ? (size_t)16 * Kp * 4 : 0);
   const int by_lds = (int)(163840 / p.lds), by_regs = (cols == 128 ? 4 : cols == 256 ? 3 : 2) - (dtype == GB_T_F32 && cols < 512),
              per_cu = by_lds < by_regs ? by_lds : by_regs;
-  const long long tiles = (P + 63) / 64, most = 256ll * (per_cu < 1 ? 1 : per_cu);
+  const long long tiles = (P + 63) / 64, fill = 256ll * (per_cu < 1 ? 1 : per_cu), runs = sum ? (tiles + STREAM_RUN - 1) / STREAM_RUN : 0,
+                  most = fill > runs ? fill : runs;
   p.grid = (int)(tiles < most ? tiles : most);
   return p;
 }
@@ -942,9 +945,8 @@ static bool fp8_dims_large(long long P, int N, int K) {   // int tile offsets: 2
   return N > (1 << 22) || K > (1 << 22) || P > (1ll << 40);
 }
 
-// Rows of a workgroup: sixteen (one access a lane) until that fills the device, then 64; with column sums as many as leave
-// at most 512 partial ones.  (8192 x 128
-// fp32 in chunks of 64 rows 4.8 us, of sixteen 3.7.)
+// Rows of a workgroup: sixteen (one access a lane) until that fills the device, then 64 (8192 x 128 fp32 in chunks of 64 rows
+// 4.8 us, of sixteen 3.7); with column sums as many as leave at most 512 partial ones, but no lane adds more than 64.
 static int rows_per_chunk(long long P, int K, bool sum) {
   if (!sum) {
     if (P / 16 * blocks128(K) < 8192) return 16;
@@ -952,7 +954,7 @@ static int rows_per_chunk(long long P, int K, bool sum) {
     return per < 64 ? 64 : (int)per;
   }
   const long long per = (P + 511) / 512;
-  return (int)(per < 16 ? 16 : (per + 15) / 16 * 16);
+  return (int)(per < 16 ? 16 : per > 1024 ? 1024 : (per + 15) / 16 * 16);
 }
 
 struct WgradPlan8 {

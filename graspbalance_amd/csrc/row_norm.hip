@@ -25,6 +25,7 @@ static constexpr int GN_DIRECT = 32;    // workgroups per sample up to which eve
                                         // a launch less each way (4 x 1024 x 256 bf16: 41 -> 37 us of kernels a pass)
 static constexpr int GN_DIRECT_GROUPS = 256;
 static constexpr int GN_MIN_STEPS = 4;  // of a workgroup: with fewer, joining the sums costs what the parallelism gains
+static constexpr int GN_RUN = 64;       // terms that a lane of the backward pass adds in fp32 before they join a sum in 64 bits
 
 struct GnShape {
   long long R;         // rows of the whole tensor
@@ -52,6 +53,7 @@ struct GnArgs {
   unsigned q;
   int sub;             // columns of a workgroup that holds them in registers
   int direct;          // the applying kernel joins the workgroups' sums itself
+  int fold;            // backward: a lane adds more than GN_RUN steps
 };
 
 // Rows of sample s.  Offsets come from the device and are taken as they are within [0, R]: no value of theirs leads
@@ -603,6 +605,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_stats_kernel(GnArgs a) {
   if (u.none) return;
   const T *x = (const T *)a.x + u.base, *dy = (const T *)a.dy + u.base, *res = a.res ? (const T *)a.res + u.base : nullptr;
   float sg[N] = {}, sx[N] = {};
+  double *whole = reinterpret_cast<double *>(gn_lds) + 2 * N * threadIdx.x;   // fold: sums of 64 bits
   if (l.on) {
     Coef<N> co;
     load_coef<N>(sh, a.w, a.b, l.p, a.mean + (long long)s * sh.G, a.rstd + (long long)s * sh.G, co);
@@ -614,13 +617,27 @@ __global__ __launch_bounds__(1024) void gn_bwd_stats_kernel(GnArgs a) {
     };
     const long long step = sh.T;
     long long v = u.v;
-    for (; v + step < u.end; v += 2 * step) {
-      const Raw<T> f0 = load_raw(x + N * v), f1 = load_raw(x + N * (v + step)), d0 = load_raw(dy + N * v),
-                   d1 = load_raw(dy + N * (v + step));
-      VecOf<T> r0 = {}, r1 = {};
-      if (res) r0 = load_unit(res + N * v), r1 = load_unit(res + N * (v + step));
-      add(widen(f0), r0, widen(d0), v);
-      add(widen(f1), r1, widen(d1), v + step);
+    if (a.fold)
+#pragma unroll
+      for (int k = 0; k < 2 * N; ++k) whole[k] = 0;
+    for (bool more = true; more;) {   // with `fold`, every GN_RUN steps the lane's sums go to its place in LDS
+      const long long stop = a.fold && v + GN_RUN * step < u.end ? v + GN_RUN * step : u.end;
+      for (; v + step < stop; v += 2 * step) {
+        const Raw<T> f0 = load_raw(x + N * v), f1 = load_raw(x + N * (v + step)), d0 = load_raw(dy + N * v),
+                     d1 = load_raw(dy + N * (v + step));
+        VecOf<T> r0 = {}, r1 = {};
+        if (res) r0 = load_unit(res + N * v), r1 = load_unit(res + N * (v + step));
+        add(widen(f0), r0, widen(d0), v);
+        add(widen(f1), r1, widen(d1), v + step);
+      }
+      more = stop < u.end;
+      if (more)
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          whole[2 * k] += sg[k];
+          whole[2 * k + 1] += sx[k];
+          sg[k] = sx[k] = 0;
+        }
     }
     if (v < u.end) {
       VecOf<T> r = {};
@@ -636,7 +653,14 @@ __global__ __launch_bounds__(1024) void gn_bwd_stats_kernel(GnArgs a) {
       for (int k = 0; k < N; ++k)
         if (k < u.tail) sg[k] += g.v[k], sx[k] += g.v[k] * xh.v[k];
     }
+    if (a.fold)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        sg[k] = (float)(whole[2 * k] + sg[k]);
+        sx[k] = (float)(whole[2 * k + 1] + sx[k]);
+      }
   }
+  if (a.fold) __syncthreads();   // (the joins take the same LDS)
   float *lds = reinterpret_cast<float *>(gn_lds);
   join_columns<N, float>(sh, l, sg, sx, lds, lds, lds + sh.C);
   float2 *out = reinterpret_cast<float2 *>(a.cpart) + ((long long)s * sh.ns + chunk) * sh.C;
@@ -820,7 +844,8 @@ struct GnPlan {
   int ns;    // workgroups per sample
   int direct;
   int sub;   // columns per workgroup of the one-pass kernel; 0: the sample is read twice
-  size_t lds, ws;
+  int fold;
+  size_t lds, lds_stats, ws;
 };
 
 static int lds_tree(int T, int PL) {  // join_columns: most lanes that give theirs away at a step (RL - h first, then h / 2, ...)
@@ -849,7 +874,7 @@ static GnPlan gn_plan(const GbGroupNorm *n, bool backward) {
   GnPlan p;
   const long long longest = n->offsets ? n->rows : n->rows / n->samples;
   const int C = n->channels, cpg = C / n->groups, N = unit_of(n->dtype), size = 16 / N;
-  p.sub = 0;
+  p.sub = p.fold = 0;
   if (!backward) {
     // The one-pass kernel wherever a sample's columns fit: no second read and one launch instead of three.  Columns: all
     // of them when C is no multiple of N, else the fewest whole groups that divide C into full 128-byte lines of units, or
@@ -882,6 +907,7 @@ static GnPlan gn_plan(const GbGroupNorm *n, bool backward) {
     p.ns = spread(n, steps, p.block, backward);
     // short samples: a few more steps each rather than a launch more
     if (p.ns > GN_DIRECT && steps <= 2ll * GN_DIRECT * GN_MIN_STEPS) p.ns = GN_DIRECT;
+    p.fold = backward && (steps + p.ns - 1) / p.ns > GN_RUN;
   }
   p.direct = !p.sub && p.ns <= GN_DIRECT && (backward || n->groups <= GN_DIRECT_GROUPS);
   p.T = p.block / p.PL * p.PL;
@@ -894,6 +920,8 @@ static GnPlan gn_plan(const GbGroupNorm *n, bool backward) {
     if (apply > p.lds) p.lds = apply;
     const size_t joined = (size_t)p.block * 2 * sizeof(double);  // (channel_gradients)
     if (joined > p.lds) p.lds = joined;
+    const size_t whole = p.fold ? (size_t)p.block * 2 * N * sizeof(double) : 0;
+    p.lds_stats = whole > p.lds ? whole : p.lds;
     p.ws = ((size_t)n->samples * p.ns + n->samples) * C * 2 * sizeof(float);
   } else {
     p.ws = p.sub ? 0 : (size_t)n->samples * p.ns * n->groups * 2 * sizeof(double);
@@ -939,6 +967,7 @@ static GnArgs gn_args(const GbGroupNorm *n, const GnPlan &p) {
   a.sh.ns = p.ns;
   a.sub = p.sub;
   a.direct = p.direct;
+  a.fold = p.fold;
   a.x = n->x;
   a.res = n->residual;
   a.w = n->weight;
@@ -1020,7 +1049,11 @@ extern "C" int gb_group_norm_bwd(const GbGroupNorm *n, const void *dy, void *dx,
     typedef decltype(z) T;
     constexpr int ACT = decltype(act)::value;
     const dim3 grid((unsigned)p.ns, (unsigned)n->samples), all((unsigned)p.ns, (unsigned)n->samples + 1);
-    gn_bwd_stats_kernel<T, ACT><<<grid, p.block, p.lds, st>>>(a);
+    if (p.lds_stats > 65536) {
+      static std::atomic<unsigned long long> done{0};
+      allow_dynamic_lds(gn_bwd_stats_kernel<T, ACT>, 131072, done);   // (1024 lanes of 2 x 8 sums)
+    }
+    gn_bwd_stats_kernel<T, ACT><<<grid, p.block, p.lds_stats, st>>>(a);
     if (!p.direct) gn_bwd_join_kernel<Unit<T>::N><<<dim3((unsigned)((n->channels + 7) / 8), (unsigned)n->samples), 256, 0, st>>>(a);
     if (nt)
       gn_bwd_apply_kernel<T, ACT, true><<<all, p.block, p.lds, st>>>(a);

@@ -411,3 +411,18 @@ def test_kept_codes_are_autograds_to_watch():
             y = fused_rows.fp8_linear(x, weight, b)
         got, = torch.autograd.grad(y, x, dy)
         assert torch.equal(got, want) and sum(t.numel() for t in seen) >= held.codes_t.numel() + held.scales.numel()
+
+
+@pytest.mark.parametrize("rows,excess,needs_x", [(1 << 23, 0.99 * 2.0 ** -15, False), (1 << 25, 0.99 * 2.0 ** -17, True)])
+def test_bias_gradient_of_many_rows(rows, excess, needs_x):
+    """Equal terms 1 + excess lose their tail at every addition to a sum of 512 or more (there a lane's four rows are added
+    first, hence the smaller excess), all in one direction: over 100 U of 2^-24 where a lane adds a thousand rows in fp32.
+    The bound: at most 64 such additions, the workgroups' sums and the result rounded once.  Both ways through the kernels."""
+    from graspbalance_amd import fused_rows
+    x = torch.ones(rows, 1, device="cuda:0").requires_grad_(needs_x)
+    bias = torch.zeros(128, device="cuda:0").requires_grad_()
+    y = fused_rows.fp8_linear(x, fused_rows.Fp8Weight.quantize(torch.ones(128, 1, device="cuda:0"), input_gradients=True), bias)
+    c = torch.tensor(1 + excess, device="cuda:0")
+    db = torch.autograd.grad(y, [bias] + [x] * needs_x, c.expand_as(y))[0]
+    total = float(c) * rows
+    assert bool(((db.double() - total).abs() <= 68 * 2.0 ** -24 * total).all()), float((db.double() / total - 1).abs().max()) * 2 ** 24

@@ -379,3 +379,22 @@ def test_empty_tensors():
         y = fused_rows.group_norm_act(x, 4, w, None, act="relu")
         gx, gw = torch.autograd.grad(y.sum(), [x, w])
         assert y.shape == shape and gx.shape == shape and bool((gw == 0).all())
+
+
+def test_long_runs_keep_their_bits():
+    """512 samples of 8000 x 128: a lane adds 1000 terms.  Equal terms 1 + 0.99 * 2^-15 lose their tail at every addition to a
+    sum of 512 or more, all in one direction: 250 U in plain fp32.  The bound: 64 additions in fp32 (and the two that end a
+    range) before they join a sum of 64 bits, trees of depth under 10, the workgroups' sums and the result rounded once."""
+    from graspbalance_amd import fused_rows
+    S, rows, C = 512, 8000, 128
+    x = torch.randn(S, rows, C, device="cuda:0", generator=torch.Generator("cuda:0").manual_seed(0))
+    w, b = (torch.ones(C, device="cuda:0").requires_grad_() for _ in range(2))
+    y = fused_rows.group_norm_act(x, 8, w, b)
+    c = torch.tensor(1 + 0.99 * 2.0 ** -15, device="cuda:0")
+    dw, db = torch.autograd.grad(y, [w, b], c.expand_as(y))
+    total = float(c) * S * rows
+    assert bool(((db.double() - total).abs() <= 80 * U * total).all()), float((db.double() / total - 1).abs().max() / U)
+    # z = xh + 1, so xh is y - 1 to a few U
+    xh = sum((y[s].double() - 1).sum(0) for s in range(S)) * float(c)
+    mag = sum((y[s].double() - 1).abs().sum(0) for s in range(S)) * float(c)
+    assert bool(((dw.double() - xh).abs() <= 90 * U * mag).all())
