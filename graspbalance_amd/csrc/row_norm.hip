@@ -54,6 +54,8 @@ struct GnArgs {
   int sub;             // columns of a workgroup that holds them in registers
   int direct;          // the applying kernel joins the workgroups' sums itself
   int fold;            // backward: a lane adds more than GN_RUN steps
+  int gather, zero;    // dweight / dbias, the rows outside every sample: kernels of their own
+  double *zpart;       // gather: (gridDim.y, C, 2) sums over a share of the samples
 };
 
 // Rows of sample s.  Offsets come from the device and are taken as they are within [0, R]: no value of theirs leads
@@ -737,6 +739,64 @@ __device__ __forceinline__ void channel_gradients(const GnArgs &a, int part, int
   }
 }
 
+// The same where samples are many: 32 channels x 8 lanes over every gridDim.y-th block of eight samples, so that no lane waits
+// for more than a few loads one after the other (in the applying kernel's last row, 4096 samples of 64 x 128 kept one workgroup
+// busy for 1.2 ms).
+template <int N>
+__global__ __launch_bounds__(256) void gn_bwd_gather_kernel(GnArgs a) {
+  __shared__ double lds[8][32][2];
+  const GnShape &sh = a.sh;
+  const int i = (int)threadIdx.x & 31, q = (int)threadIdx.x >> 5, c = (int)blockIdx.x * 32 + i;
+  double s0 = 0, s1 = 0;
+  if (c < sh.C) {
+    if (sh.ns == 1) {
+#pragma unroll 4
+      for (int s = (int)blockIdx.y * 8 + q; s < sh.S; s += 8 * (int)gridDim.y) {
+        const float2 f = reinterpret_cast<const float2 *>(a.cpart)[(long long)s * sh.C + c];
+        s0 += f.x;
+        s1 += f.y;
+      }
+    } else {
+      for (int s = (int)blockIdx.y * 8 + q; s < sh.S; s += 8 * (int)gridDim.y) channel_sums<N>(a, s, c, s0, s1);
+    }
+  }
+  lds[q][i][0] = s0;
+  lds[q][i][1] = s1;
+  __syncthreads();
+  if (q > 0 || c >= sh.C) return;
+  for (int j = 1; j < 8; ++j) s0 += lds[j][i][0], s1 += lds[j][i][1];
+  if (gridDim.y > 1) {
+    double *to = a.zpart + ((long long)blockIdx.y * sh.C + c) * 2;
+    to[0] = s0;
+    to[1] = s1;
+  } else {
+    if (a.db) a.db[c] = (float)s0;
+    if (a.dw) a.dw[c] = (float)s1;
+  }
+}
+__global__ __launch_bounds__(256) void gn_bwd_channels_kernel(GnArgs a, int parts) {
+  __shared__ double lds[8][32][2];
+  const int i = (int)threadIdx.x & 31, q = (int)threadIdx.x >> 5, c = (int)blockIdx.x * 32 + i, C = a.sh.C;
+  double s0 = 0, s1 = 0;
+  if (c < C)
+#pragma unroll 4
+    for (int z = q; z < parts; z += 8) {
+      s0 += a.zpart[((long long)z * C + c) * 2];
+      s1 += a.zpart[((long long)z * C + c) * 2 + 1];
+    }
+  lds[q][i][0] = s0;
+  lds[q][i][1] = s1;
+  __syncthreads();
+  if (q > 0 || c >= C) return;
+  for (int j = 1; j < 8; ++j) s0 += lds[j][i][0], s1 += lds[j][i][1];
+  if (a.db) a.db[c] = (float)s0;
+  if (a.dw) a.dw[c] = (float)s1;
+}
+template <typename T>
+__global__ __launch_bounds__(256) void gn_zero_kernel(GnArgs a, T *y, T *y2) {
+  zero_outside<T>(a.sh, y, y2, blockIdx.x, gridDim.x);
+}
+
 // S1 / n and S2 / n of every group into k1, k2 (LDS, G entries each) from the channels' sums v0, v1 (LDS, scaled by w here)
 __device__ __forceinline__ void group_terms(const GnArgs &a, float *v0, float *v1, float *k1, float *k2, double n) {
   const GnShape &sh = a.sh;
@@ -768,8 +828,8 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnArgs a) {
   const GnShape &sh = a.sh;
   const int s = (int)blockIdx.y, chunk = (int)blockIdx.x;
   if (s == sh.S) {
-    channel_gradients<N>(a, chunk, sh.ns);
-    if (sh.offs) zero_outside<T>(sh, (T *)a.dx, (T *)a.dres, chunk, sh.ns);
+    if (!a.gather) channel_gradients<N>(a, chunk, sh.ns);
+    if (sh.offs && !a.zero) zero_outside<T>(sh, (T *)a.dx, (T *)a.dres, chunk, sh.ns);
     return;
   }
   const RowRng rng = load_rng(a.rng, a.seed, a.call);
@@ -845,7 +905,8 @@ struct GnPlan {
   int direct;
   int sub;   // columns per workgroup of the one-pass kernel; 0: the sample is read twice
   int fold;
-  size_t lds, lds_stats, ws;
+  int gather, zero;   // workgroups over the samples that add dweight / dbias, over the rows outside them; 0: the last row's
+  size_t lds, lds_stats, ws, zpart;
 };
 
 static int lds_tree(int T, int PL) {  // join_columns: most lanes that give theirs away at a step (RL - h first, then h / 2, ...)
@@ -874,7 +935,7 @@ static GnPlan gn_plan(const GbGroupNorm *n, bool backward) {
   GnPlan p;
   const long long longest = n->offsets ? n->rows : n->rows / n->samples;
   const int C = n->channels, cpg = C / n->groups, N = unit_of(n->dtype), size = 16 / N;
-  p.sub = p.fold = 0;
+  p.sub = p.fold = p.gather = p.zero = 0;
   if (!backward) {
     // The one-pass kernel wherever a sample's columns fit: no second read and one launch instead of three.  Columns: all
     // of them when C is no multiple of N, else the fewest whole groups that divide C into full 128-byte lines of units, or
@@ -907,6 +968,11 @@ static GnPlan gn_plan(const GbGroupNorm *n, bool backward) {
     p.ns = spread(n, steps, p.block, backward);
     // short samples: a few more steps each rather than a launch more
     if (p.ns > GN_DIRECT && steps <= 2ll * GN_DIRECT * GN_MIN_STEPS) p.ns = GN_DIRECT;
+    // Steps of the one row of workgroups that would add the samples' sums, some 0.6 us each: from 16 on, two launches are less.
+    const long long groups = (C + 31) / 32, lanes = p.block / 32,
+                    chain = (groups + p.ns - 1) / p.ns * ((n->samples + lanes - 1) / lanes);
+    if (backward && chain > 16) p.gather = n->samples <= 128 ? 1 : n->samples < 256 * 64 ? (n->samples + 63) / 64 : 256;
+    if (n->offsets && p.ns < 32 && n->samples >= 64) p.zero = 512;
     p.fold = backward && (steps + p.ns - 1) / p.ns > GN_RUN;
   }
   p.direct = !p.sub && p.ns <= GN_DIRECT && (backward || n->groups <= GN_DIRECT_GROUPS);
@@ -922,7 +988,8 @@ static GnPlan gn_plan(const GbGroupNorm *n, bool backward) {
     if (joined > p.lds) p.lds = joined;
     const size_t whole = p.fold ? (size_t)p.block * 2 * N * sizeof(double) : 0;
     p.lds_stats = whole > p.lds ? whole : p.lds;
-    p.ws = ((size_t)n->samples * p.ns + n->samples) * C * 2 * sizeof(float);
+    p.zpart = ((size_t)n->samples * p.ns + n->samples) * C * 2 * sizeof(float);
+    p.ws = p.zpart + (p.gather > 1 ? (size_t)p.gather * C * 2 * sizeof(double) : 0);
   } else {
     p.ws = p.sub ? 0 : (size_t)n->samples * p.ns * n->groups * 2 * sizeof(double);
   }
@@ -968,6 +1035,8 @@ static GnArgs gn_args(const GbGroupNorm *n, const GnPlan &p) {
   a.sub = p.sub;
   a.direct = p.direct;
   a.fold = p.fold;
+  a.gather = p.gather;
+  a.zero = p.zero;
   a.x = n->x;
   a.res = n->residual;
   a.w = n->weight;
@@ -1008,7 +1077,7 @@ extern "C" int gb_group_norm_fwd(const GbGroupNorm *n, void *y, void *ws, long l
   a.gpart = (double *)ws;
   hipStream_t st = as_stream(stream);
   const bool nt = streams(n->rows * n->channels * (16 / unit_of(n->dtype)));
-  const dim3 all((unsigned)p.ns, (unsigned)(n->samples + (n->offsets ? 1 : 0)));
+  const dim3 all((unsigned)p.ns, (unsigned)(n->samples + (n->offsets && !p.zero ? 1 : 0)));
   return with_type_and_act(n, [&](auto z, auto act) {
     typedef decltype(z) T;
     constexpr int ACT = decltype(act)::value;
@@ -1022,6 +1091,7 @@ extern "C" int gb_group_norm_fwd(const GbGroupNorm *n, void *y, void *ws, long l
         gn_apply_kernel<T, ACT, true><<<all, p.block, 0, st>>>(a);
       else
         gn_apply_kernel<T, ACT, false><<<all, p.block, 0, st>>>(a);
+      if (p.zero) gn_zero_kernel<T><<<(unsigned)p.zero, 256, 0, st>>>(a, (T *)y, (T *)nullptr);
     }
     return check_launch("gb_group_norm_fwd");
   });
@@ -1043,12 +1113,14 @@ extern "C" int gb_group_norm_bwd(const GbGroupNorm *n, const void *dy, void *dx,
   a.db = dbias;
   a.cpart = (float *)ws;
   a.csum = a.cpart + (size_t)n->samples * p.ns * n->channels * 2;
+  a.zpart = (double *)((char *)ws + p.zpart);
   hipStream_t st = as_stream(stream);
   const bool nt = streams(n->rows * n->channels * (16 / unit_of(n->dtype)));
   return with_type_and_act(n, [&](auto z, auto act) {
     typedef decltype(z) T;
     constexpr int ACT = decltype(act)::value;
-    const dim3 grid((unsigned)p.ns, (unsigned)n->samples), all((unsigned)p.ns, (unsigned)n->samples + 1);
+    const dim3 grid((unsigned)p.ns, (unsigned)n->samples), 
+               all((unsigned)p.ns, (unsigned)n->samples + (!p.gather || (n->offsets && !p.zero) ? 1 : 0));
     if (p.lds_stats > 65536) {
       static std::atomic<unsigned long long> done{0};
       allow_dynamic_lds(gn_bwd_stats_kernel<T, ACT>, 131072, done);   // (1024 lanes of 2 x 8 sums)
@@ -1059,6 +1131,12 @@ extern "C" int gb_group_norm_bwd(const GbGroupNorm *n, const void *dy, void *dx,
       gn_bwd_apply_kernel<T, ACT, true><<<all, p.block, p.lds, st>>>(a);
     else
       gn_bwd_apply_kernel<T, ACT, false><<<all, p.block, p.lds, st>>>(a);
+    if (p.gather && (dweight || dbias)) {
+      const unsigned groups = (unsigned)((n->channels + 31) / 32);
+      gn_bwd_gather_kernel<Unit<T>::N><<<dim3(groups, (unsigned)p.gather), 256, 0, st>>>(a);
+      if (p.gather > 1) gn_bwd_channels_kernel<<<groups, 256, 0, st>>>(a, p.gather);
+    }
+    if (p.zero) gn_zero_kernel<T><<<(unsigned)p.zero, 256, 0, st>>>(a, (T *)dx, (T *)dresidual);
     return check_launch("gb_group_norm_bwd");
   });
 }

@@ -398,3 +398,47 @@ def test_long_runs_keep_their_bits():
     xh = sum((y[s].double() - 1).sum(0) for s in range(S)) * float(c)
     mag = sum((y[s].double() - 1).abs().sum(0) for s in range(S)) * float(c)
     assert bool(((dw.double() - xh).abs() <= 90 * U * mag).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,groups", [((9, 16, 1024), 8), ((64, 3, 40), 4), ((129, 3, 65), 5), ((3000, 2, 33), 3), ((17000, 1, 24), 2),
+                                          ((40, 700, 1021), 1)])
+def test_many_samples(shape, groups, dtype):
+    """The samples' sums added by the applying kernel's last row, by one workgroup a column block, by several."""
+    R, C = math.prod(shape[:-1]), shape[-1]
+    _check(_inputs(R, C, dtype, False, seed=R), groups, dtype, "silu", shape=shape)
+
+
+@pytest.mark.parametrize("S,before,behind", [(64, 5, 0), (700, 0, 9000), (2500, 30, 70)])
+def test_many_packed_samples_and_rows_outside(S, before, behind):
+    """Rows in front of the first and behind the last of many samples, some of them empty, some long."""
+    g = torch.Generator().manual_seed(S)
+    sizes = torch.randint(0, 7, (S,), generator=g)
+    sizes[S // 3] = 3000
+    cuts = (torch.cat([torch.zeros(1, dtype=torch.int64), sizes.cumsum(0)]) + before).tolist()
+    _check(_inputs(cuts[-1] + behind, 40, torch.float32, True, seed=S), 4, torch.float32, "gelu", cuts=cuts, p=0.25)
+
+
+def test_many_samples_take_no_longer_than_few():
+    """The same rows as 4096 samples and as 64, dense and packed with as many rows again behind the last, the best of seven
+    passes: about the same time; 7.5 times as long where one workgroup adds the samples' sums (1.58 ms against 0.21), and longer
+    still where one clears the rows behind them."""
+    from graspbalance_amd import fused_rows
+
+    def best(S, rows, pad):
+        x = torch.randn(S * rows + pad, 128, device="cuda:0") if pad else torch.randn(S, rows, 128, device="cuda:0")
+        off = torch.arange(S + 1, device="cuda:0") * rows if pad else None
+        leaves = [x.requires_grad_()] + [torch.ones(128, device="cuda:0").requires_grad_() for _ in range(2)]
+        dy, times = torch.randn_like(x), []
+        for _ in range(7):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            y = fused_rows.group_norm_act(leaves[0], 8, *leaves[1:], act="silu", offsets=off)
+            torch.autograd.grad(y, leaves, dy)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+    for pad in (0, 1 << 18):
+        few, many = best(64, 4096, pad), best(4096, 64, pad)
+        assert many <= 4 * few, (pad, many, few)
