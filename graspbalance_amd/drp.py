@@ -144,7 +144,7 @@ class InvResMLP(nn.Module):
         else:
             x0 = fused_mlp.group_concat_cl(p, p, idx, f_cl, mode=0)               # [dp, fj] rows
             agg = fused_mlp.conv_bn_act(x0, agg_conv, agg_bn, relu=True, pool_ns=g.nsample)   # (B*N, C)
-        if self.dropout is not None and self.training:   # (the pair in two, the expanded features dropped in between)
+        if self.dropout is not None and self.dropout.training:   # (the pair in two, the expanded features dropped in between)
             hidden = self.dropout(fused_mlp.conv_bn_act(agg, self.pwconv[0][0], self.pwconv[0][1]))
             out = fused_mlp.conv_bn_act(hidden, self.pwconv[1][0], self.pwconv[1][1], relu=True,
                                         residual=f_cl.reshape(B * N, C))

@@ -256,3 +256,25 @@ def test_blocks_refuse_16_bit_features(norm, dtype):
             copy.deepcopy(blk).to(dtype)([p, f])
     torch.cuda.synchronize()
     assert bool(torch.isfinite(blk([p, f])[1]).all())
+
+
+@pytest.mark.parametrize("norm,act", [({'norm': 'bn'}, 'relu'), ({'norm': 'gn', 'num_groups': 4}, 'silu')])
+def test_dropout_follows_its_own_mode(norm, act):
+    """A block in evaluation whose dropout alone trains (samples of a prediction) drops, fused as composed; the other way
+    round it does not."""
+    from graspbalance_amd import fused_mlp
+    from graspbalance_amd.scene import make_batch
+    blk = fill_by_key(_block(norm=norm, act=act, dropout=0.3), seed=2).to(DEV).eval()
+    p, f = torch.from_numpy(make_batch([0], 1024)).to(DEV), torch.randn(1, 32, 1024, device=DEV)
+    with torch.no_grad():
+        still = blk([p, f])[1]
+        for flag in (True, False):
+            fused_mlp.set_enabled(flag)
+            try:
+                blk.dropout.train()
+                blk.dropout.rng.copy_(torch.tensor([5, 0]))
+                assert _rel(blk([p, f])[1], still) > 1e-3 and blk.dropout.rng.tolist() == [5, 1], flag
+                blk.dropout.eval()
+                assert _rel(blk([p, f])[1], still) < 1e-5 and blk.dropout.rng.tolist() == [5, 1], flag
+            finally:
+                fused_mlp.set_enabled(True)
