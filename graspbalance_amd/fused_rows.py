@@ -521,12 +521,12 @@ def activation_of(module):
 
 
 def conv_gn_act(x, conv, gn, act=("none", 0.0), fp8=False, residual=None, dropout=None):
-    """A 1x1 ``conv`` without bias, ``gn`` (nn.GroupNorm), an activation (activation_of) and optionally a Dropout on
+    """A 1x1 ``conv`` (with or without bias), ``gn`` (nn.GroupNorm), an activation (activation_of) and optionally a Dropout on
     channel-last rows x (samples, rows, Cin) -> (samples, rows, Cout), with the modules' own parameters; residual joins
     in front of the activation.  fp8: the product in 8-bit floats; else x and the weight must be fp32 (linear_bias)."""
     W = conv.weight.view(conv.weight.shape[0], -1)
     if fp8:
-        y = fp8_linear(x, W)
+        y = fp8_linear(x, W, conv.bias)
     else:
         y = linear_bias(x.reshape(-1, x.shape[-1]), conv).view(x.shape[:-1] + (W.shape[0],))
     drop = dropout is not None and dropout.training and dropout.p > 0

@@ -278,3 +278,23 @@ def test_dropout_follows_its_own_mode(norm, act):
                 assert _rel(blk([p, f])[1], still) < 1e-5 and blk.dropout.rng.tolist() == [5, 1], flag
             finally:
                 fused_mlp.set_enabled(True)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_convolution_keeps_its_bias(fp8):
+    """conv_gn_act with a bias in front of the norm, values and the bias's gradient; bounds as in the run of the operators."""
+    from graspbalance_amd import fused_rows
+    torch.manual_seed(3)
+    conv, gn = nn.Conv1d(96, 64, 1).to(DEV), nn.GroupNorm(8, 64).to(DEV)
+    nn.init.normal_(conv.bias, 0.0, 2.0)
+    x, dy = torch.randn(2, 100, 96, device=DEV), torch.randn(2, 100, 64, device=DEV)
+    y = fused_rows.conv_gn_act(x, conv, gn, ("silu", 0.0), fp8)
+    got, = torch.autograd.grad(y, conv.bias, dy)
+    twin = copy.deepcopy(nn.ModuleList([conv, gn])).double().cpu()
+    rows = x.double().cpu().reshape(200, 96)
+    w = twin[0].weight[:, :, 0]
+    z = (_CodedGradient.apply(_Codes.apply(rows, 1) @ _Codes.apply(w, 128).t()) if fp8 else rows @ w.t()) + twin[0].bias
+    z = F.group_norm(z.view(2, 100, 64).transpose(1, 2), 8, twin[1].weight, twin[1].bias, gn.eps).transpose(1, 2)
+    want_y = row_truth.act(z, "silu", 0.0)
+    want, = torch.autograd.grad(want_y, twin[0].bias, dy.double().cpu())
+    assert _rel(y, want_y) <= (1e-3 if fp8 else 1e-5) and _rel(got, want) <= (1e-3 if fp8 else 1e-5)
