@@ -62,6 +62,12 @@ def _pointwise(channels, norm_args, act_args, conv_args, less_act):
         for i in range(len(channels) - 1)])
 
 
+def _is_pointwise(conv):
+    """A convolution that is one product on rows: 1x1 without bias, stride, padding or groups."""
+    return (isinstance(conv, (nn.Conv1d, nn.Conv2d)) and conv.bias is None and all(k == 1 for k in conv.kernel_size + conv.stride)
+            and conv.groups == 1 and (conv.padding in ("same", "valid") or all(p == 0 for p in conv.padding)))
+
+
 class InvResMLP(nn.Module):
     """LocalAggregation(C->C) -> pointwise C->expansion*C->C -> residual add -> act.
 
@@ -107,8 +113,7 @@ class InvResMLP(nn.Module):
         """conv + group norm + an activation that the row kernels have, after the aggregation, the expansion and the sum."""
         def is_block(seq, with_act):
             mods = list(seq.children())
-            return (len(mods) == (3 if with_act else 2) and isinstance(mods[0], (nn.Conv1d, nn.Conv2d)) and mods[0].bias is None
-                    and all(k == 1 for k in mods[0].kernel_size) and isinstance(mods[1], nn.GroupNorm)
+            return (len(mods) == (3 if with_act else 2) and _is_pointwise(mods[0]) and isinstance(mods[1], nn.GroupNorm)
                     and (not with_act or fused_rows.activation_of(mods[2]) is not None))
         return (self._standard() and is_block(self.convs.convs[0], True) and is_block(self.pwconv[0], True)
                 and is_block(self.pwconv[1], False) and fused_rows.activation_of(self.act) is not None)
@@ -119,7 +124,7 @@ class InvResMLP(nn.Module):
         def is_block(seq, with_act):
             mods = list(seq.children())
             want = 3 if with_act else 2
-            return (len(mods) == want and isinstance(mods[0], (nn.Conv1d, nn.Conv2d)) and mods[0].bias is None
+            return (len(mods) == want and _is_pointwise(mods[0])
                     and isinstance(mods[1], (nn.BatchNorm1d, nn.BatchNorm2d))
                     and not (mods[1].momentum is None and mods[1].track_running_stats)
                     and (not with_act or isinstance(mods[2], nn.ReLU)))

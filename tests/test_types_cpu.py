@@ -116,3 +116,16 @@ def test_blocks_take_fp32_features_alone(launches, norm, dtype):
     with pytest.raises(RuntimeError, match="float32"):
         pb.group_points_wrapper(1, 32, 64, 64, 16, _Tensor(dtype, 1, 32, 64), _Tensor(torch.int32, 1, 64, 16), _Tensor(torch.float32, 1, 32, 64, 16))
     assert launches == []
+
+
+@pytest.mark.parametrize("norm", ["bn", "gn"])
+@pytest.mark.parametrize("extra", [{'groups': 3}, {'padding': 1}, {'stride': 1}, {'padding': 'same'}, {}], ids=str)
+def test_blocks_fuse_plain_products_alone(norm, extra):
+    """Grouped or padded 1x1 convolutions are no product on rows: such a block runs its modules."""
+    from graspbalance_amd.drp import InvResMLP
+    blk = InvResMLP(in_channels=24, aggr_args={'feature_type': 'dp_fj', "reduction": 'max'},
+                    norm_args={'norm': 'gn', 'num_groups': 3} if norm == "gn" else {'norm': 'bn'}, act_args={'act': 'relu'},
+                    group_args={'NAME': 'ballquery', 'radius': 0.1, 'nsample': 16}, conv_args={'order': 'conv-norm-act', **extra},
+                    expansion=4, use_res=True)
+    fused = extra in ({}, {'stride': 1}, {'padding': 'same'})
+    assert (blk.fusable() or blk.fusable_gn()) is fused and blk._fused_on(_Tensor(torch.float32, 1, 24, 64)) is fused
