@@ -331,8 +331,9 @@ __device__ __forceinline__ int weight_row(int at) { return (at & ~63) + 2 * (at 
 
 // G > 1 (few tiles, a long reduction): G groups of WM x WN waves with stages of their own take a range of the steps each, and
 // their sums meet in LDS, added in the groups' order.  A lone group is bound by its own steps, one after the other (~0.6 us
-// each: waits for LDS and the matrix pipe; four stages in flight instead of two gained 3 us in 21 for 16 bits and lost as much
-// for fp32).  128 x 4096 -> 4096 bf16 with its quantiser 21.0 -> 14.7 us, fp32 24.7 -> 16.3; 512 x 1024 -> 1024 8.8 -> 8.3.
+// each: waits for LDS and the matrix pipe; four stages in flight instead of two gained 3 us in 21 with the 8-bit instructions and
+// lost as much with bf16 products).  128 x 4096 -> 4096 with its quantiser bf16 25.3 -> 16.1 us, fp32 26.1 -> 16.7; 512 x 1024 -> 1024
+// bf16 9.8 -> 8.5.
 template <typename T, bool EXACT, int TM, int TN, int WM, int WN, int G, bool NT>
 __global__ __launch_bounds__(64 * WM * WN * G) void fp8_gemm_kernel(GemmArgs8 g) {
   constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, WAVES = WM * WN, ROWS = BM + BN, LOADS = ROWS / (8 * WAVES);
@@ -448,7 +449,7 @@ __global__ __launch_bounds__(64 * WM * WN * G) void fp8_gemm_kernel(GemmArgs8 g)
 // keeps the weight and walks over tiles of 64 rows, 128 columns of X at a step: the next step's rows travel in registers
 // while this one is multiplied, are quantised into the other LDS buffer, and go to memory as codes only where the backward
 // pass wants them.  Against a quantising kernel and the tiles above: X's codes are not read back and there is one launch
-// (524288 x 128 -> 256 bf16: 123 us in two launches, 100 here: 470 MB at 4.7 TB/s, a large copy's rate).  SUM: also the
+// (524288 x 256 -> 128 bf16: 137 us in two launches, 107 here: 403 MB at 3.8 TB/s; 524288 x 128 -> 256: 92, 86).  SUM: also the
 // column sums of X, a tile's four rows of a lane in registers, then fp32 in the lane's LDS cells over STREAM_RUN tiles at most.
 static constexpr int STREAM_RUN = 60;
 struct StreamArgs8 {
@@ -859,7 +860,7 @@ static void launch_few(const GemmArgs8 &g, const T *x, int K, unsigned char *cod
 // y from codes and exponents in memory
 template <typename T, bool EXACT>
 static int multiply_codes(const GemmArgs8 &g, int K, hipStream_t st) {
-  // (64 x 4096 -> 4096 bf16: 18.2 us without tiles, 13.7 with four groups of waves a tile; 64 x 1024 -> 1024: 7.6, 8.4)
+  // (64 x 4096 -> 4096 bf16: 18.6 us without tiles, 14.9 with four groups of waves a tile; 64 x 1024 -> 1024: 7.3, 8.4)
   if (g.P <= FP8_FEW_ROWS && !(g.P > 32 && g.Kb >= 32)) {
     if (g.P <= 16)
       launch_few<T, EXACT, 1, false>(g, nullptr, K, nullptr, nullptr, 0, st);
@@ -871,8 +872,8 @@ static int multiply_codes(const GemmArgs8 &g, int K, hipStream_t st) {
   }
   // 256 x 256 where that still gives every CU a tile, the columns fill it as well as 128 do to a fifth, and there are steps
   // enough to work through; short reductions live from several workgroups per CU, which only smaller tiles leave room for.  Tiles of 64 x 64 that leave
-  // CUs idle get groups of waves: four up to a tile per CU, two up to two tiles (1024 x 4096 -> 4096 bf16: 34 us in tiles of
-  // 128 x 128, 46 in 1024 of these).
+  // CUs idle get groups of waves: four up to a tile per CU, two up to two tiles (1024 x 4096 -> 4096 bf16: 45.6 us in tiles
+  // of 128 x 128, 48.4 in 1024 of these; with the 8-bit instructions 34, 46).
   const bool nt = streams(g.P * g.N * (long long)sizeof(T));
   if (g.Kb >= 4 && tiles_of(g.P, g.N, 256) >= 256 && 5 * blocks128(g.N) >= 8 * ((g.N + 255) / 256))
     return nt ? launch_tiles<T, EXACT, 4, 2, 2, 4, 1, true>(g, st) : launch_tiles<T, EXACT, 4, 2, 2, 4, 1, false>(g, st);
@@ -884,9 +885,10 @@ static int multiply_codes(const GemmArgs8 &g, int K, hipStream_t st) {
 }
 
 // Columns of the streaming kernel's variant; 0: not one of its shapes.  A weight of 128 x 128 is in LDS at once, and one
-// launch beats two from the first rows on (1024 rows fp32: 5.4 us against 6.7; 16384: 7.0, 9.4); a larger one has to be worth
-// its loading by every workgroup (8192 x 512 -> 128 bf16: 15.2 against 10.1, 16384 x 256 -> 256 fp32: 12.4 against 13.5,
-// 524288 x 256 -> 128 bf16: 120 against 212).
+// launch beats two from the first rows on (1024 rows fp32: 5.2 us against 5.8; 16384: 6.4, 8.7); a larger one has to be worth
+// its loading by every workgroup (8192 x 512 -> 128 bf16: 12.8 against 10.6, 16384 x 256 -> 256 fp32: 12.2 against 14.0,
+// 524288 x 256 -> 128 bf16: 107 against 137, fp32 165 against 211; the worst is 65536 x 256 -> 256: bf16 34 against 26, fp32 35
+// against 33).
 static int stream_columns(long long P, int N, int K) {
   if (P <= FP8_FEW_ROWS || N > 512) return 0;
   const int cols = N <= 128 ? 128 : N <= 256 ? 256 : 512;
@@ -897,12 +899,15 @@ struct StreamPlan8 {
   size_t lds;
   int grid;
 };
+// Workgroups per CU that walk over the tiles.  A 128 x 128 weight: three for fp32, four for 16 bits (700001 rows bf16: two 82 us, three
+// 72, four 67); larger ones: two, although registers and LDS would often hold three (524288 x 128 -> 256 bf16: two 86 us, three
+// 96, four in turns 88; 524288 x 256 -> 128: 107, 121, 108; 100000 x 128 -> 256: 24.6, 27.3, 25.5; a training pass of
+// 524288 x 128 -> 256: 262, 290, 276).
 static StreamPlan8 stream_plan(long long P, int cols, int K, int dtype, bool sum) {
   StreamPlan8 p;
   const int Kp = blocks128(K) * 128;
   p.lds = (size_t)cols * Kp + 2 * 64 * 128 + 2 * 64 + 4 * (dtype == GB_T_F32 ? Cell<float>::BYTES : Cell<__bf16>::BYTES) + (sum ? (size_t)16 * Kp * 4 : 0);
-  const int by_lds = (int)(163840 / p.lds), by_regs = (cols == 128 ? 4 : cols == 256 ? 3 : 2) - (dtype == GB_T_F32 && cols < 512),
-             per_cu = by_lds < by_regs ? by_lds : by_regs;
+  const int by_lds = (int)(163840 / p.lds), want = cols * Kp <= 16384 ? (dtype == GB_T_F32 ? 3 : 4) : 2, per_cu = by_lds < want ? by_lds : want;
   const long long tiles = (P + 63) / 64, fill = 256ll * (per_cu < 1 ? 1 : per_cu), runs = sum ? (tiles + STREAM_RUN - 1) / STREAM_RUN : 0,
                   most = fill > runs ? fill : runs;
   p.grid = (int)(tiles < most ? tiles : most);
