@@ -417,8 +417,8 @@ __device__ __forceinline__ void grad_act(const GnArgs &a, const Coef<N> &co, con
     xh.v[k] = d0 * co.rstd[k];
     float z = d0 * co.a[k] + co.b[k];
     z += res.v[k];
-    const float d = a.q ? ((m >> k & 1) ? dy.v[k] * a.scale : 0.0f) : dy.v[k];
-    g.v[k] = d * act_slope<ACT>(z, a.slope);
+    const float d = (a.q ? dy.v[k] * a.scale : dy.v[k]) * act_slope<ACT>(z, a.slope);
+    g.v[k] = m >> k & 1 ? d : 0.0f;   // (a dropped element has no gradient, whatever the residual holds there)
   }
 }
 

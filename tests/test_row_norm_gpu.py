@@ -442,3 +442,26 @@ def test_many_samples_take_no_longer_than_few():
     for pad in (0, 1 << 18):
         few, many = best(64, 4096, pad), best(4096, 64, pad)
         assert many <= 4 * few, (pad, many, few)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", ["none", "relu", "leaky_relu", "silu", "gelu"])
+@pytest.mark.parametrize("shape", [(2, 60, 48), (1, 9000, 45)])
+def test_dropped_places_hide_the_residual(shape, act, dtype):
+    """Infinities and NaN of the residual and of dy in dropped places reach no output and no gradient: the same bits as zeros."""
+    from graspbalance_amd import fused_rows
+    n, C = math.prod(shape), shape[-1]
+    keep, _ = row_truth.keep_mask(n, 0.5, 4, 7)
+    keep = keep.view(shape).to("cuda:0")
+    case = _inputs(n // C, C, dtype, True, seed=n)
+    x, w, b, res, dy = (case[k].to("cuda:0") for k in ("x", "weight", "bias", "residual", "dy"))
+    x, res, dy = x.view(shape), res.view(shape), dy.view(shape)
+
+    def run(fill):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, torch.where(keep, res, fill))]
+        y = fused_rows.group_norm_act(leaves[0], 3, *leaves[1:3], act=act, residual=leaves[3], dropout_p=0.5, rng=(4, 7))
+        return [y.detach()] + list(torch.autograd.grad(y, leaves, torch.where(keep, dy, fill)))
+    clean = run(torch.zeros((), dtype=dtype, device="cuda:0"))
+    assert all(bool(torch.isfinite(t).all()) for t in clean)
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        assert all(torch.equal(a, c) for a, c in zip(run(torch.tensor(bad, dtype=dtype, device="cuda:0")), clean)), bad
