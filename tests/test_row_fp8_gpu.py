@@ -426,3 +426,22 @@ def test_bias_gradient_of_many_rows(rows, excess, needs_x):
     db = torch.autograd.grad(y, [bias] + [x] * needs_x, c.expand_as(y))[0]
     total = float(c) * rows
     assert bool(((db.double() - total).abs() <= 68 * 2.0 ** -24 * total).all()), float((db.double() / total - 1).abs().max()) * 2 ** 24
+
+
+@pytest.mark.parametrize("P,K,N", [((1 << 20) + 77, 4104, 8), ((1 << 25) + 5, 128, 130)])
+def test_products_past_32_bits_of_elements(P, K, N):
+    """Codes, rows and outputs behind 2^32 elements, in tiles and streamed: the first and last rows of y and dx; in tiles the last columns of dw too."""
+    from graspbalance_amd import fused_rows
+    g = torch.Generator(device="cuda:0").manual_seed(1)
+    x, dy = (torch.randn(P, n, generator=g, device="cuda:0", dtype=torch.bfloat16) for n in (K, N))
+    w = (torch.randn(N, K, generator=g, device="cuda:0") * (2.0 / K) ** 0.5).requires_grad_()
+    y = fused_rows.fp8_linear(x.requires_grad_(), w)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    wq = row_truth.in_8_bits(w.detach().cpu().double(), 128)
+    for at in (slice(0, 150), slice(P - 150, P)):
+        _check(y[at], row_truth.in_8_bits(x[at].detach().cpu().double(), 1), wq, None, torch.bfloat16, "y")
+        _check(dx[at], row_truth.in_8_bits(dy[at].cpu().double(), 1), wq.t().contiguous(), None, torch.bfloat16, "dx")
+    if K > 128:      # (the truth of every row of the last block of columns: a minute of the CPU for 2^25 of them)
+        xq = row_truth.in_8_bits(x[:, (K - 1) // 128 * 128:].detach().cpu().double(), 1)
+        _check(dw[:, -xq.shape[1]:], row_truth.in_8_bits(dy.cpu().double(), 1).t().contiguous(), xq.t().contiguous(), None,
+               torch.float32, "dw", length=P)

@@ -465,3 +465,51 @@ def test_dropped_places_hide_the_residual(shape, act, dtype):
     assert all(bool(torch.isfinite(t).all()) for t in clean)
     for bad in (float("inf"), -float("inf"), float("nan")):
         assert all(torch.equal(a, c) for a, c in zip(run(torch.tensor(bad, dtype=dtype, device="cuda:0")), clean)), bad
+
+
+def test_tensors_past_32_bits_of_elements():
+    """Two samples of 2^31 elements and more: the ends of both against the formulas (statistics in 64 bits, on the GPU), dweight
+    and dbias; bounds as in test_tensors_past_the_caches."""
+    from graspbalance_amd import fused_rows
+    rows, C, G = (1 << 24) + 3, 128, 4
+    g = torch.Generator(device="cuda:0").manual_seed(5)
+    x, dy = (torch.randn(2, rows, C, generator=g, device="cuda:0", dtype=torch.bfloat16) for _ in range(2))
+    x[1] += 0.5
+    w, b = (1 + 0.2 * torch.randn(C, generator=g, device="cuda:0")).requires_grad_(), torch.zeros(C, device="cuda:0").requires_grad_()
+    x.requires_grad_()
+    y = fused_rows.group_norm_act(x, G, w, b, act="relu")
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+    tw, tb, mw, mb = (torch.zeros(C, dtype=torch.float64, device="cuda:0") for _ in range(4))
+    step = 1 << 20
+    with torch.no_grad():
+        for s in range(2):
+            part = lambda t, i: t[s, i:i + step].double().view(-1, G, C // G)   # noqa: E731
+            n, sums = rows * (C // G), torch.zeros(4, G, 1, dtype=torch.float64, device="cuda:0")
+            for i in range(0, rows, step):
+                sums[0] += part(x, i).sum((0, 2)).view(G, 1)
+            mean = sums[0] / n
+            for i in range(0, rows, step):
+                sums[1] += ((part(x, i) - mean) ** 2).sum((0, 2)).view(G, 1)
+            rstd = 1 / torch.sqrt(sums[1] / n + 1e-5)
+            wd = w.double().view(G, -1)
+            for i in range(0, rows, step):
+                xh = (part(x, i) - mean) * rstd
+                gr = part(dy, i) * (xh * wd > 0)
+                sums[2] += (gr * wd).sum((0, 2)).view(G, 1)
+                sums[3] += (gr * wd * xh).sum((0, 2)).view(G, 1)
+                tw += (gr * xh).sum(0).view(C)
+                tb += gr.sum(0).view(C)
+                mw += (gr * xh).abs().sum(0).view(C)
+                mb += gr.abs().sum(0).view(C)
+            for at in (slice(0, 1000), slice(rows - 1000, rows)):
+                xh = (x[s, at].double().view(-1, G, C // G) - mean) * rstd
+                z = xh * wd
+                want = z.clamp(min=0).view(-1, C)
+                assert bool(((y[s, at].double() - want).abs() <= HALF[torch.bfloat16] * want + 32 * 40 * U).all()), s
+                gr = dy[s, at].double().view(-1, G, C // G) * (z > 0)
+                want = ((gr * wd - sums[2] / n - xh * sums[3] / n) * rstd).view(-1, C)
+                clear = (z.abs() > 1e-4).view(-1, C)     # (relu's slope jumps at zero)
+                off = (dx[s, at].double() - want).abs()
+                assert bool((off <= HALF[torch.bfloat16] * want.abs() + 256 * 40 * U)[clear].all()), s
+    # (elements within rounding of relu's corner, 1e-6 of them, may fall on the other side)
+    assert bool(((dw.double() - tw).abs() <= 128 * U * mw).all()) and bool(((db.double() - tb).abs() <= 128 * U * mb + 1e-5 * mb).all())
