@@ -921,8 +921,10 @@ static int lds_tree(int T, int PL) {  // join_columns: most lanes that give thei
 // the registers allow 132 / 238 us, two 127 / 229, one 141 / 256; 8 x 131072 x 128 bf16: 144 / 244, 130 / 232, 159 / 291).  Where
 // there is arithmetic to hide - dropout, gelu on 16-bit elements - what the registers allow (4 x 131072 x 128 bf16 gelu +
 // residual: 110 / 210 us, two 114 / 214; with dropout 124 / 216, two 133 / 233; but 8 x 131072 x 128 bf16 silu + residual 180 /
-// 344, two 171 / 329, and 4 x 65536 x 128 fp32 gelu + residual 90 / 169, two 88 / 162).  Packed samples may be of very different
-// lengths: as many, cut twice as fine.
+// 344, two 171 / 329, and 4 x 65536 x 128 fp32 gelu + residual 90 / 169, two 88 / 162).  What the registers allow: 512 over the
+// applying kernels' 60 (fp32) and 78 (16 bits) forward, 94 and 126 backward, in steps of eight; a build that took more would
+// have a last round of a few, not other results.  Packed samples may be of very different lengths: as many, cut twice as fine.
+// (The plan does not see the lengths: one cloud of 262144 rows x 64 among 1000 of 8 rows gets four workgroups, 6.4 ms a training pass.)
 static int spread(const GbGroupNorm *n, long long steps, int block, bool backward) {
   const bool light = n->q == 0 && !(n->act == GB_ACT_GELU && n->dtype != GB_T_F32) && !n->offsets;
   const int waves = light ? 2 : n->dtype == GB_T_F32 ? (backward ? 5 : 8) : (backward ? 4 : 6);

@@ -513,3 +513,24 @@ def test_tensors_past_32_bits_of_elements():
                 assert bool((off <= HALF[torch.bfloat16] * want.abs() + 256 * 40 * U)[clear].all()), s
     # (elements within rounding of relu's corner, 1e-6 of them, may fall on the other side)
     assert bool(((dw.double() - tw).abs() <= 128 * U * mw).all()) and bool(((db.double() - tb).abs() <= 128 * U * mb + 1e-5 * mb).all())
+
+
+def test_gelu_over_its_range():
+    """gelu and its slope by themselves (weight 0: z is the bias), relative to the true values: the polynomial's 1.1e-7, the
+    roundings of the exponent (two of z^2 / 2, which exp multiplies by) and twelve more - down to z = -9, where the value is 1e-18."""
+    from graspbalance_amd import fused_rows
+    C = 4096
+    z = torch.linspace(-9, 9, C)
+    z[C // 2] = 0.0
+    b = z.to("cuda:0").requires_grad_()
+    x = torch.ones(1, 1, C, device="cuda:0")
+    y = fused_rows.group_norm_act(x, C, torch.zeros(C, device="cuda:0"), b, act="gelu")
+    slope, = torch.autograd.grad(y, b, torch.ones_like(y))
+    zd = z.double()
+    cdf = 0.5 * torch.special.erfc(-zd / math.sqrt(2.0))
+    pdf = torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi)
+    part = 1.1e-7 + (zd * zd + 12) * U
+    off = (y.detach().double().cpu().view(C) - zd * cdf).abs()
+    assert bool((off <= part * (zd * cdf).abs()).all()), (off / (zd * cdf).abs()).max()
+    off = (slope.double().cpu() - (cdf + zd * pdf)).abs()
+    assert bool((off <= part * (cdf + zd.abs() * pdf)).all())
