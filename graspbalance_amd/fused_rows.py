@@ -476,9 +476,9 @@ def fp8_linear(x, weight, bias=None, short_sums=False):
     Gradients are those of the products with the quantisers passed straight through: the incoming gradient is quantised
     like x, dx and dweight are products of the 8-bit operands, dbias sums the gradient as it came.  An element of x or
     weight that is not finite makes every output it takes part in NaN.  The codes are multiplied as bf16, which holds them
-    exactly (what rounds to 2^128 counts as infinite, what is below 2^-126 as zero), with fp32 sums.  short_sums: for 16-bit x, y and dx come from the 8-bit matrix instructions instead: faster where
-    the matrix cores bind, but a step of 64 or 128 products keeps only about 14 bits below its largest (measured 5e-5 of the
-    result's norm); fp32 x is computed as ever."""
+    exactly (what rounds to 2^128 counts as infinite, what is below 2^-126 as zero), with fp32 sums.  short_sums: for 16-bit
+    x, y and dx come from the 8-bit matrix instructions instead: faster where the matrix cores bind, but a step of 64 or 128
+    products keeps only about 14 bits below its largest (measured 5e-5 of the result's norm); fp32 x is computed as ever."""
     what = "fp8_linear"
     _rows_tensor(what, "x", x)
     held = weight if isinstance(weight, Fp8Weight) else None
